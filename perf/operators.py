@@ -148,9 +148,10 @@ def _rows(g, shape, dtype):
 def _encode(x, codes):
     """Rows of whole blocks (..., blocks, block, D), float32: their codes and scales."""
     top = x.abs().amax(dim=(-2, -1))
-    inv = torch.where(top > 0, TOP[codes] / top, torch.zeros_like(top))
+    largest = torch.full_like(top, TOP[codes])             # (a number over a tensor would be the number times a rounded reciprocal)
+    inv = torch.where(top > 0, largest / top, torch.zeros_like(top))
     y = x * inv[..., None, None]
-    return (torch.round(y) if codes == "int8" else y).to(CODES[codes]), top / TOP[codes]
+    return (torch.round(y) if codes == "int8" else y).to(CODES[codes]), top / largest
 
 
 def _cache(g, c, tokens):
