@@ -363,6 +363,71 @@ int tq_decode_kernel_choice(const tq_decode_args* a);
 /* The CTAs per cache lane of kernel 4, or 0 where another one runs.  Negative: the arguments are invalid. */
 int tq_decode_one_launch(const tq_decode_args* a);
 
+/* ---- rotary positions ---------------------------------------------------------------------- */
+
+/* Queries and keys turned to their positions, one launch.  Of every row the first `dims` coordinates (even, <= d) are turned in pairs,
+ * (x[i], x[i + dims/2]) or, interleaved, (x[2i], x[2i+1]), by position * freqs[i]; the others are copied:
+ *   a' = factor (a cos - b sin), b' = factor (b cos + a sin).
+ * The angle is formed in float64 (float32 is a radian off at a million positions), the products in float32, one rounding to dtype. */
+typedef struct {
+    const void* x;              /* element (b, h, t, i) at x + b*sb + h*sh + t*st + i */
+    int64_t sb, sh, st;         /* elements */
+    void* out;                  /* (batch, heads, length, d), contiguous */
+    int heads;                  /* 0: this tensor is absent */
+} tq_rotary_rows;
+typedef struct {
+    tq_rotary_rows part[2];     /* queries, keys */
+    int dtype, batch, d, dims, interleaved;
+    int64_t length;
+    const double* freqs;        /* (dims / 2), device: radians per position */
+    float factor;
+    int64_t offset;             /* token t sits at position offset + t, or */
+    const int64_t* positions;   /* at positions[b * pos_sb + t] (device) where that is not NULL */
+    int64_t pos_sb;
+} tq_rotary_args;
+int tq_rotary(const tq_rotary_args* a, void* stream);
+
+/* ---- cache in 8-bit blocks ----------------------------------------------------------------- */
+
+/* Keys and values of a cache whose whole blocks of `block` tokens are held in 8 bits, a scale for each block and head.  Lane = b*n_kv_heads + h;
+ * token t < length / block * block is row t of the lane's codes and stands for code * scale[t / block]; the tokens behind are rows t % block of
+ * the lane's tail, as they came.  Contiguous arrays, 16-byte aligned. */
+enum { TQ_CODE_INT8 = 0, TQ_CODE_E4M3 = 1 };
+typedef struct {
+    int batch, n_kv_heads, d, block;      /* d a multiple of 32 up to 256; block 16, 32, 64 or 128 */
+    int code_type, dtype;                 /* dtype: of the tails, TQ_F16 / TQ_BF16 / TQ_F32 */
+    void *k_codes, *v_codes;              /* (batch, n_kv_heads, capacity, d) bytes */
+    float *k_scales, *v_scales;           /* (batch, n_kv_heads, capacity / block) */
+    void *k_tail, *v_tail;                /* (batch, n_kv_heads, block, d) of dtype */
+    int64_t capacity, length;             /* tokens */
+} tq_block_store;
+/* Rows of new tokens: element (b, h, t, i) at x + b*sb + h*sh + t*st + i (strides in elements), 16-byte aligned rows. */
+typedef struct { const void* x; int64_t sb, sh, st; } tq_new_rows;
+
+/* Appends n_new tokens of s->dtype behind s->length others: with those of the tail they fill blocks, which are quantised
+ * (A = max |x| of the block; int8: round to even of x * (127 / A), scale A / 127; e4m3: x * (448 / A), scale A / 448; float32 throughout),
+ * and the rest is left in the tail.  A block that holds a NaN or an infinity reads back as NaN. */
+int tq_blocks_write(const tq_block_store* s, const tq_new_rows* k_new, const tq_new_rows* v_new, int64_t n_new, void* stream);
+/* The s->length tokens as dense rows, (batch, n_kv_heads, length, d) of out_dtype. */
+int tq_blocks_read(const tq_block_store* s, void* k_out, void* v_out, int out_dtype, void* stream);
+
+/* Attention of the last t_q tokens over the cache, causal; a token j is visible from position p if j <= p and (window == 0, p - j < window or
+ * j < sinks).  With k_new / v_new (t_q == 1) that token's rows join the tail in the same launch (store.length counts it not yet, and
+ * store.length % block + 1 < block). */
+typedef struct {
+    tq_block_store store;
+    int n_q_heads;
+    int64_t t_q;
+    tq_new_rows q;                        /* (batch, n_q_heads, t_q, d) of store.dtype */
+    float scale;
+    int64_t window, sinks;
+    tq_new_rows k_new, v_new;             /* (batch, n_kv_heads, 1, d), or x == NULL */
+    void* out;                            /* (batch, n_q_heads, t_q, d) of store.dtype, contiguous */
+    void* workspace; size_t workspace_bytes;      /* tq_blocks_attend_workspace(...) bytes, 256-byte aligned, any content */
+} tq_blocks_attend_args;
+size_t tq_blocks_attend_workspace(const tq_blocks_attend_args* a);
+int tq_blocks_attend(const tq_blocks_attend_args* a, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -87,6 +87,40 @@ class DecodeArgs(C.Structure):
     ]
 
 
+class RotaryRows(C.Structure):
+    _fields_ = [("x", _vp), ("sb", _i64), ("sh", _i64), ("st", _i64), ("out", _vp), ("heads", _i)]
+
+
+class RotaryArgs(C.Structure):
+    _fields_ = [
+        ("part", RotaryRows * 2), ("dtype", _i), ("batch", _i), ("d", _i), ("dims", _i), ("interleaved", _i), ("length", _i64),
+        ("freqs", _vp), ("factor", _f), ("offset", _i64), ("positions", _vp), ("pos_sb", _i64),
+    ]
+
+
+TQ_CODE_INT8, TQ_CODE_E4M3 = 0, 1
+
+
+class BlockStore(C.Structure):
+    """tq_block_store: keys and values in 8-bit blocks, and their tails."""
+    _fields_ = [
+        ("batch", _i), ("n_kv_heads", _i), ("d", _i), ("block", _i), ("code_type", _i), ("dtype", _i),
+        ("k_codes", _vp), ("v_codes", _vp), ("k_scales", _vp), ("v_scales", _vp), ("k_tail", _vp), ("v_tail", _vp),
+        ("capacity", _i64), ("length", _i64),
+    ]
+
+
+class NewRows(C.Structure):
+    _fields_ = [("x", _vp), ("sb", _i64), ("sh", _i64), ("st", _i64)]
+
+
+class BlocksAttendArgs(C.Structure):
+    _fields_ = [
+        ("store", BlockStore), ("n_q_heads", _i), ("t_q", _i64), ("q", NewRows), ("scale", _f), ("window", _i64), ("sinks", _i64),
+        ("k_new", NewRows), ("v_new", NewRows), ("out", _vp), ("workspace", _vp), ("workspace_bytes", _sz),
+    ]
+
+
 # name -> (restype, argtypes); every symbol include/tq_abi.h declares
 PROTOTYPES = {
     "tq_version": (_i, []),
@@ -124,6 +158,11 @@ PROTOTYPES = {
     "tq_device_status_clear": (_i, []),
     "tq_gather_groups": (_i64, [_i, _i, _i]),
     "tq_gather_wait": (_i, [_vp, _vp, _i64, _vp, _vp]),
+    "tq_rotary": (_i, [C.POINTER(RotaryArgs), _vp]),
+    "tq_blocks_write": (_i, [C.POINTER(BlockStore), C.POINTER(NewRows), C.POINTER(NewRows), _i64, _vp]),
+    "tq_blocks_read": (_i, [C.POINTER(BlockStore), _vp, _vp, _i, _vp]),
+    "tq_blocks_attend_workspace": (_sz, [C.POINTER(BlocksAttendArgs)]),
+    "tq_blocks_attend": (_i, [C.POINTER(BlocksAttendArgs), _vp]),
     "tq_peer_buffer_create": (_i, [_sz, C.POINTER(_vp), C.c_char_p]),
     "tq_peer_buffer_open": (_i, [C.c_char_p, _i, C.POINTER(_vp)]),
     "tq_peer_buffer_close": (_i, [_vp]),

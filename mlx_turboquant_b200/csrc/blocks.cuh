@@ -1,0 +1,53 @@
+// Declarations shared by the kernels of the 8-bit block cache.
+#pragma once
+
+#include "decode_dev.cuh"
+
+namespace tq {
+
+constexpr int BLOCKS_MAX_D = 256;
+
+inline bool block_ok(int n) { return n == 16 || n == 32 || n == 64 || n == 128; }
+inline int log2_of(int n) { return 31 - __builtin_clz(unsigned(n)); }
+// What every entry point of the cache asks of its storage; `what` opens the error's text
+int check_store(const tq_block_store* s, const char* what);
+int blocks_sm_count();
+
+// blocks_attend.cu: float32 tokens and head dims without a kernel of their own; one new token, and a few, per sequence
+// blocks_fa.cu: many query rows per lane
+struct BlockAttendParams {
+    const uint8_t *kc, *vc;                  // codes
+    const float *ks, *vs;                    // scales
+    const void *kt, *vt;                     // tails
+    void *kt_w, *vt_w;                       // tails, writable (append)
+    const void *kn, *vn;                     // the appended token's rows, or null
+    int64_t kn_sb, kn_sh, vn_sb, vn_sh;
+    const void* q;
+    int64_t q_sb, q_sh, q_st;
+    void* out;
+    int dtype, e4m3;
+    int B, Hq, Hkv, G, D, Tq;
+    int block, shift;                        // tokens of a block, log2 of that
+    int64_t cap;                             // tokens of a lane's codes; cap >> shift scales
+    int n8, total;                           // tokens in blocks; all tokens, the appended one included
+    int window, sinks;                       // window: INT_MAX / 2 without one
+    float scale_log2;                        // scale * log2(e)
+    float* part;                             // workspace
+};
+
+int launch_blocks_plain(const BlockAttendParams& p, cudaStream_t s);
+
+// The first token that some query sees through its window, and how many sink tokens lie before it
+struct Visible { int low, sinks; };
+inline __host__ __device__ Visible visible_of(int total, int t_q, int window, int sinks) {
+    const int first = total - t_q, low = first - window + 1 > 0 ? first - window + 1 : 0;
+    return Visible{low, sinks < low ? sinks : low};
+}
+
+__device__ __forceinline__ float e4m3_to_f32(uint8_t c) {
+    uint32_t h;
+    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"(uint16_t(c)));
+    return __half2float(__ushort_as_half(uint16_t(h & 0xffffu)));
+}
+
+}  // namespace tq

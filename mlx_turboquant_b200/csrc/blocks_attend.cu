@@ -1,0 +1,631 @@
+// Attention over the 8-bit block cache: one new token per sequence, and few query rows per KV head; sliding window and sinks.
+//
+//   out = sum_j softmax_j(scale q.k_j) v_j,   k_j = kc_j ks, v_j = vc_j vs with one ks, vs for each block of tokens, tokens of the tail as they are
+//
+// The integers are exact as fp16, and so are the 8-bit floats: scores are products of codes with the query as it came (a bfloat16 one under a
+// power of two), the scales follow in float32, the values' scale on the softmax weights.  Only those are rounded, to fp16.
+//
+// blocks_attend_kernel: bound by the codes' bytes.  Work is a flat sequence of units (16 or 32 tokens) of all (lane, group of 8 query rows); a CTA of four warps
+// takes an equal run of it, whatever lanes that touches, a warp every fourth unit of a lane.  A warp reads its next unit's codes straight into registers
+// (16 bytes a lane, whole sectors) while it computes on this one: mma.sync m16n8k16 with the tokens as M (scores) and the coordinates as M (values), so
+// that eight query rows share every converted code.  Which coordinate a fragment's row or column stands for is free as long as queries and results agree:
+// a lane's 16 bytes are four fragments.  (The products are tiny, N = 8: tcgen05 would want 64 rows of operands staged in shared memory as fp16.)
+// blocks_merge_kernel: joins the partials of a row that several CTAs worked on, in their order: results do not depend on which one came first.
+// blocks_plain_kernel: a warp per token on CUDA cores, float32 throughout: float32 tokens, head dims without a layout above.
+#include <algorithm>
+#include <atomic>
+#include <climits>
+
+#include "blocks.cuh"
+
+namespace tq {
+
+bool blocks_fa_takes(const BlockAttendParams& p);
+size_t blocks_fa_workspace(const BlockAttendParams& p);
+int launch_blocks_fa(const BlockAttendParams& p, cudaStream_t s);
+
+namespace {
+
+// ---------------------------------------------------------------------------------------------------- float32, any head_dim
+constexpr int PL_W = 4;                                // warps of a CTA: one query row
+__global__ void __launch_bounds__(PL_W * 32) blocks_plain_kernel(const __grid_constant__ BlockAttendParams p) {
+    constexpr int NV = BLOCKS_MAX_D / 32;
+    __shared__ float so[PL_W][BLOCKS_MAX_D], sm[PL_W], sl[PL_W];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int ti = blockIdx.x % p.Tq, h = blockIdx.x / p.Tq % p.Hq, b = blockIdx.x / p.Tq / p.Hq, kv = h / p.G, nv = p.D / 32;
+    const int64_t lane_c = int64_t(b) * p.Hkv + kv;
+    pdl_wait();
+    float q[NV], o[NV], m = -INFINITY, l = 0.f;
+    for (int i = 0; i < nv; ++i) {
+        q[i] = load_as_f32(p.q, p.dtype, b * p.q_sb + h * p.q_sh + ti * p.q_st + i * 32 + lane) * p.scale_log2;
+        o[i] = 0.f;
+    }
+    const int pos = p.total - p.Tq + ti;
+    const int low = max(0, pos - p.window + 1), sinks = min(p.sinks, low), n = sinks + pos + 1 - low;
+    for (int i = warp; i < n; i += PL_W) {
+        const int j = i < sinks ? i : low + i - sinks;
+        const bool in8 = j < p.n8, fresh = p.kn != nullptr && j == p.total - 1;
+        const int64_t code = (lane_c * p.cap + j) * p.D + lane, sc = lane_c * (p.cap >> p.shift) + (j >> p.shift), row = (lane_c * p.block + (j - p.n8)) * p.D + lane;
+        float s = 0.f;
+        for (int e = 0; e < nv; ++e) {
+            const float k = in8 ? (p.e4m3 ? e4m3_to_f32(p.kc[code + e * 32]) : float(int8_t(p.kc[code + e * 32])))
+                                : fresh ? load_as_f32(p.kn, p.dtype, b * p.kn_sb + kv * p.kn_sh + e * 32 + lane) : load_as_f32(p.kt, p.dtype, row + e * 32);
+            s = fmaf(q[e], k, s);
+        }
+#pragma unroll
+        for (int off = 16; off; off >>= 1) s += __shfl_xor_sync(0xffffffffu, s, off);
+        if (in8) s *= p.ks[sc];
+        const float mn = fmaxf(fmaxf(m, s), -1e30f), a = exp2f(m - mn), w = exp2f(s - mn), vs = in8 ? w * p.vs[sc] : w;
+        m = mn;
+        l = l * a + w;
+        for (int e = 0; e < nv; ++e) {
+            const float v = in8 ? (p.e4m3 ? e4m3_to_f32(p.vc[code + e * 32]) : float(int8_t(p.vc[code + e * 32])))
+                                : fresh ? load_as_f32(p.vn, p.dtype, b * p.vn_sb + kv * p.vn_sh + e * 32 + lane) : load_as_f32(p.vt, p.dtype, row + e * 32);
+            o[e] = fmaf(vs, v, o[e] * a);
+        }
+    }
+    for (int e = 0; e < nv; ++e) so[warp][e * 32 + lane] = o[e];
+    if (lane == 0) { sm[warp] = m; sl[warp] = l; }
+    __syncthreads();
+    float top = -1e30f, sum = 0.f;
+    for (int w = 0; w < PL_W; ++w) top = fmaxf(top, sm[w]);
+    for (int w = 0; w < PL_W; ++w) sum += sl[w] * exp2f(sm[w] - top);
+    for (int i = threadIdx.x; i < p.D; i += PL_W * 32) {
+        float x = 0.f;
+        for (int w = 0; w < PL_W; ++w) x += so[w][i] * exp2f(sm[w] - top);
+        store_from_f32(p.out, p.dtype, ((int64_t(b) * p.Hq + h) * p.Tq + ti) * p.D + i, x / sum);
+        if (p.kn != nullptr && h % p.G == 0) {         // the appended row joins the tail (every reader takes it from where it came)
+            const int64_t row = (lane_c * p.block + (p.total - 1 - p.n8)) * p.D + i;
+            store_from_f32(p.kt_w, p.dtype, row, load_as_f32(p.kn, p.dtype, b * p.kn_sb + kv * p.kn_sh + i));
+            store_from_f32(p.vt_w, p.dtype, row, load_as_f32(p.vn, p.dtype, b * p.vn_sb + kv * p.vn_sh + i));
+        }
+    }
+}
+
+// ---------------------------------------------------------------------------------------------------- 16-bit tokens
+constexpr int AW = 4;                                  // warps of a CTA
+
+// A code row's bytes of a lane: pieces of the row, each shared evenly by the four (keys) or eight (values) lanes that hold parts of the row
+template <int D> struct Pieces {
+    static constexpr int K = 64, V = D >= 128 ? 128 : 64;      // bytes of a piece; the last one may be shorter (d = 96)
+    static __host__ __device__ constexpr int key_bytes(int i) { return D - K * i < K ? (D - K * i) / 4 : K / 4; }
+    static __host__ __device__ constexpr int value_bytes(int i) { return D - V * i < V ? (D - V * i) / 8 : V / 8; }
+};
+
+template <int D> struct AttendPlan {
+    static constexpr int TILES = D == 256 ? 1 : 2;     // 16-token tiles of a unit
+    static constexpr int UNIT = 16 * TILES;
+    static constexpr int PER_SM = D == 64 ? 4 : D == 96 ? 3 : 2;
+    static constexpr int KW = D / 16, VW = D / 32;     // words of a lane per key row (two a tile) and value row (four)
+    static constexpr int RS = D + 4;                   // floats of a partial row: sums, maximum, sum of weights
+};
+
+struct AttendGrid {
+    int n_units, n_sink, n_win, low_unit, tail_unit;   // units of a (lane, group): sink tokens, window tokens in blocks, the tail's from tail_unit on
+    int groups, slots;                                 // groups of 8 query rows per lane; partials of one
+    int merge;                                         // the merge kernel follows
+    int64_t per;                                       // units of a CTA
+    int64_t jobs;                                      // lanes x groups
+};
+
+template <int BYTES> __device__ __forceinline__ void ld_bytes(const uint8_t* p, uint32_t* w) {
+    if constexpr (BYTES == 16) asm volatile("ld.global.L1::no_allocate.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "l"(p) : "memory");
+    else if constexpr (BYTES == 8) asm volatile("ld.global.L1::no_allocate.v2.b32 {%0,%1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "l"(p) : "memory");
+    else asm volatile("ld.global.L1::no_allocate.b32 %0, [%1];" : "=r"(w[0]) : "l"(p) : "memory");
+}
+template <int D, int I = 0> __device__ __forceinline__ void ld_key_row(const uint8_t* row, int t, uint32_t* w) {
+    if constexpr (Pieces<D>::K * I < D) {
+        ld_bytes<Pieces<D>::key_bytes(I)>(row + Pieces<D>::K * I + Pieces<D>::key_bytes(I) * t, w);
+        ld_key_row<D, I + 1>(row, t, w + Pieces<D>::key_bytes(I) / 4);
+    }
+}
+template <int D, int I = 0> __device__ __forceinline__ void ld_value_row(const uint8_t* row, int g, uint32_t* w) {
+    if constexpr (Pieces<D>::V * I < D) {
+        ld_bytes<Pieces<D>::value_bytes(I)>(row + Pieces<D>::V * I + Pieces<D>::value_bytes(I) * g, w);
+        ld_value_row<D, I + 1>(row, g, w + Pieces<D>::value_bytes(I) / 4);
+    }
+}
+// first of the four coordinates of word w of a lane's part of a key row / value row
+template <int D> __device__ __forceinline__ int key_dim(int w, int t) {
+    const int i = w / (Pieces<D>::K / 16);
+    return Pieces<D>::K * i + Pieces<D>::key_bytes(i) * t + 4 * (w - i * (Pieces<D>::K / 16));
+}
+template <int D> __device__ __forceinline__ int value_dim(int w, int g) {
+    const int i = w / (Pieces<D>::V / 32);
+    return Pieces<D>::V * i + Pieces<D>::value_bytes(i) * g + 4 * (w - i * (Pieces<D>::V / 32));
+}
+
+// four codes as two pairs of fp16.  int8: biased by 128 they are the low bytes of 1024 + code + 128
+template <bool E4M3> __device__ __forceinline__ void halves(uint32_t w, uint32_t& lo, uint32_t& hi) {
+    if constexpr (E4M3) {
+        asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, a;\n\tcvt.rn.f16x2.e4m3x2 %1, b;\n\t}" : "=r"(lo), "=r"(hi) : "r"(w));
+    } else {
+        const uint32_t u = w ^ 0x80808080u;
+        const uint32_t k = 0x64806480u;
+        uint32_t a = __byte_perm(u, 0x64646464u, 0x4140), b = __byte_perm(u, 0x64646464u, 0x4342);
+        asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(lo) : "r"(a), "r"(k));
+        asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(hi) : "r"(b), "r"(k));
+    }
+}
+
+template <int D> struct Unit {                         // a unit's codes and scales in a lane's registers
+    uint32_t k[AttendPlan<D>::TILES][2][AttendPlan<D>::KW], v[AttendPlan<D>::TILES][4][AttendPlan<D>::VW];
+    float ks[AttendPlan<D>::TILES], vs[AttendPlan<D>::TILES];
+};
+
+// What a lane knows of the query columns 2 t and 2 t + 1 of its group
+struct Cols {
+    float scale[2];                                    // softmax scale * log2(e) over the query's power of two
+    int pos[2];                                        // position; below every token where the column is empty
+    int pos_min, pos_max;                              // of the group
+};
+
+// Scores of 16 tokens (rows g, g + 8) times their scales -> running softmax -> the weights as the value products' operand.  tok: token of row g.
+template <int D, bool MASKED>
+__device__ __forceinline__ void weights(float (&s)[4], float kn0, float kn1, float vn0, float vn1, int tok, const Cols& c, int window, int sinks, WarpAcc<D, 0>& st, uint32_t (&bp)[2]) {
+    s[0] *= kn0 * c.scale[0]; s[1] *= kn0 * c.scale[1];
+    s[2] *= kn1 * c.scale[0]; s[3] *= kn1 * c.scale[1];
+    bool hide[4] = {false, false, false, false};
+    if (MASKED) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int j = tok + 8 * (i >> 1), pos = c.pos[i & 1];
+            hide[i] = j > pos || (pos - j >= window && j >= sinks);
+            if (hide[i]) s[i] = -INFINITY;
+        }
+        if (hide[0] && hide[1]) vn0 = 0.f;
+        if (hide[2] && hide[3]) vn1 = 0.f;
+    }
+    const float mx0 = fmaxf(s[0], s[2]), mx1 = fmaxf(s[1], s[3]), vmax = fmaxf(vn0, vn1);
+    if (__any_sync(0xffffffffu, mx0 > st.mt[0] || mx1 > st.mt[1] || vmax > st.vt)) softmax_refresh<D, 0>(mx0, mx1, vmax, st);
+    const float p0 = ex2(s[0] - st.m[0]), p1 = ex2(s[1] - st.m[1]), p2 = ex2(s[2] - st.m[0]), p3 = ex2(s[3] - st.m[1]);
+    st.l[0] += p0 + p2;
+    st.l[1] += p1 + p3;
+    const float w0 = vn0 * st.vsc, w1 = vn1 * st.vsc;
+    float x0 = p0 * w0, x1 = p1 * w0, x2 = p2 * w1, x3 = p3 * w1;
+    if (MASKED) {                                      // (a hidden token's scale may be a NaN)
+        if (hide[0]) x0 = 0.f;
+        if (hide[1]) x1 = 0.f;
+        if (hide[2]) x2 = 0.f;
+        if (hide[3]) x3 = 0.f;
+    }
+    bp[0] = movm_t(pack_h2(x0, x1));
+    bp[1] = movm_t(pack_h2(x2, x3));
+}
+
+template <int D, bool E4M3> __global__ void __launch_bounds__(AW * 32, AttendPlan<D>::PER_SM) blocks_attend_kernel(const __grid_constant__ BlockAttendParams p, const __grid_constant__ AttendGrid z) {
+    using P = AttendPlan<D>;
+    __shared__ __align__(16) float red[AW][HPG][P::RS];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
+    const int64_t u_first = int64_t(blockIdx.x) * z.per, u_last = min(u_first + z.per, z.jobs * z.n_units);
+    const bool bf = p.dtype == TQ_BF16;
+    pdl_wait();
+    if (z.merge) pdl_trigger();                        // (the grid is one wave: the merge's CTAs take nobody's place)
+
+    for (int64_t at = u_first; at < u_last;) {
+        const int64_t job = at / z.n_units, lane_c = job / z.groups;
+        const int u0 = int(at - job * z.n_units), u1 = int(min(int64_t(z.n_units), u0 + (u_last - at)));
+        at += u1 - u0;
+        const int grp = int(job - lane_c * z.groups), b = int(lane_c / p.Hkv), kv = int(lane_c - int64_t(b) * p.Hkv);
+        const int rows = min(HPG, p.Tq * p.G - grp * HPG), r0 = grp * HPG;
+        Cols c;
+        uint32_t bq[D / 16][2];
+        {
+            // ---- the group's queries as B operands (row g's coordinates in the order of the key codes), bfloat16 under a power of two
+            const bool has = g < rows;
+            const int r = r0 + g, ti = r / p.G, h = kv * p.G + r - ti * p.G;
+            const char* q = static_cast<const char*>(p.q) + 2 * (b * p.q_sb + h * p.q_sh + ti * p.q_st);
+            uint2 x[D / 16];
+            uint32_t mx = 0;
+#pragma unroll
+            for (int w = 0; w < D / 16; ++w) {
+                x[w] = has ? *reinterpret_cast<const uint2*>(q + 2 * key_dim<D>(w, t)) : make_uint2(0u, 0u);
+                const uint32_t m = 0x7fff7fffu, y = __vmaxu2(x[w].x & m, x[w].y & m);
+                mx = max(mx, max(y & 0xffffu, y >> 16));
+            }
+            float f = 1.f;
+            if (bf) {
+                mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+                mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+                f = stage_scale(mx << 16);
+            }
+#pragma unroll
+            for (int w = 0; w < D / 16; ++w) {
+                if (bf) {
+                    auto two = [&](uint32_t v) { return pack_h2(__uint_as_float(v << 16) * f, __uint_as_float(v & 0xffff0000u) * f); };
+                    bq[w][0] = two(x[w].x); bq[w][1] = two(x[w].y);
+                } else {
+                    bq[w][0] = x[w].x; bq[w][1] = x[w].y;
+                }
+            }
+            const float inv = p.scale_log2 / f;
+            const int first = p.total - p.Tq;
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                c.scale[i] = __shfl_sync(0xffffffffu, inv, 4 * (2 * t + i));
+                c.pos[i] = 2 * t + i < rows ? first + (r0 + 2 * t + i) / p.G : -1;
+            }
+            c.pos_min = first + r0 / p.G;
+            c.pos_max = first + (r0 + rows - 1) / p.G;
+        }
+        WarpAcc<D, 0> st;
+        st.init();
+        st.m[0] = st.m[1] = -1e30f;
+        const int lo_min = c.pos_min - p.window + 1, lo_max = c.pos_max - p.window + 1;      // (the window's first token of the first and the last query)
+        auto hidden = [&](int base) { return base > c.pos_max || (base + 15 < lo_min && base >= p.sinks); };
+        auto whole = [&](int base) { return base + 15 <= c.pos_min && (base >= lo_max || base + 15 < p.sinks); };
+
+        // ---- blocks
+        const int n_code = z.n_sink + z.n_win;
+        const uint8_t* kc = p.kc + lane_c * p.cap * D;
+        const uint8_t* vc = p.vc + lane_c * p.cap * D;
+        const float* ksc = p.ks + lane_c * (p.cap >> p.shift);
+        const float* vsc = p.vs + lane_c * (p.cap >> p.shift);
+        auto base_of = [&](int u) { return (u < z.n_sink ? u : z.low_unit + u - z.n_sink) * P::UNIT; };
+        auto load = [&](int u, Unit<D>& x) {
+            const int base = base_of(u);
+#pragma unroll
+            for (int i = 0; i < P::TILES; ++i) {
+                const int tok = min(base + 16 * i, p.n8 - 16);         // (a tile behind the last block: read again, not used)
+                const uint8_t* kr = kc + int64_t(tok + g) * D;
+                const uint8_t* vr = vc + int64_t(tok + 2 * t) * D;
+                ld_key_row<D>(kr, t, x.k[i][0]);
+                ld_key_row<D>(kr + 8 * D, t, x.k[i][1]);
+#pragma unroll
+                for (int r = 0; r < 4; ++r) ld_value_row<D>(vr + ((r & 1) + 8 * (r >> 1)) * D, g, x.v[i][r]);
+                x.ks[i] = ksc[tok >> p.shift];
+                x.vs[i] = vsc[tok >> p.shift];
+            }
+        };
+        auto compute = [&](int u, const Unit<D>& x) {
+            const int base = base_of(u);
+#pragma unroll
+            for (int i = 0; i < P::TILES; ++i) {
+                const int tok = base + 16 * i;
+                if (tok >= p.n8 || hidden(tok)) continue;
+                float s[4] = {0.f, 0.f, 0.f, 0.f}, s2[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int w = 0; w < P::KW; ++w) {
+                    uint32_t a[4];
+                    halves<E4M3>(x.k[i][0][w], a[0], a[2]);
+                    halves<E4M3>(x.k[i][1][w], a[1], a[3]);
+                    mma16816((w & 1) ? s2 : s, a[0], a[1], a[2], a[3], bq[w][0], bq[w][1]);
+                }
+#pragma unroll
+                for (int k = 0; k < 4; ++k) s[k] += s2[k];
+                uint32_t bp[2];
+                if (whole(tok)) weights<D, false>(s, x.ks[i], x.ks[i], x.vs[i], x.vs[i], tok + g, c, p.window, p.sinks, st, bp);
+                else weights<D, true>(s, x.ks[i], x.ks[i], x.vs[i], x.vs[i], tok + g, c, p.window, p.sinks, st, bp);
+                // two tokens' bytes side by side are the pairs of the transposed operand: coordinates w, w + 1 and w + 2, w + 3
+#pragma unroll
+                for (int w = 0; w < P::VW; ++w) {
+                    uint32_t a[4], e[4];
+                    halves<E4M3>(__byte_perm(x.v[i][0][w], x.v[i][1][w], 0x5140), a[0], a[1]);
+                    halves<E4M3>(__byte_perm(x.v[i][2][w], x.v[i][3][w], 0x5140), a[2], a[3]);
+                    halves<E4M3>(__byte_perm(x.v[i][0][w], x.v[i][1][w], 0x7362), e[0], e[1]);
+                    halves<E4M3>(__byte_perm(x.v[i][2][w], x.v[i][3][w], 0x7362), e[2], e[3]);
+                    mma16816(st.o[2 * w], a[0], a[1], a[2], a[3], bp[0], bp[1]);
+                    mma16816(st.o[2 * w + 1], e[0], e[1], e[2], e[3], bp[0], bp[1]);
+                }
+            }
+        };
+        {
+            int u = u0 + warp;
+            const int end = min(u1, n_code);
+            Unit<D> x, y;
+            if (u < end) load(u, x);
+            while (u < end) {
+                if (u + AW < end) load(u + AW, y);
+                compute(u, x);
+                u += AW;
+                if (u >= end) break;
+                if (u + AW < end) load(u + AW, x);
+                compute(u, y);
+                u += AW;
+            }
+        }
+        // ---- the tail: 16-bit rows, bfloat16 ones each under its power of two
+        for (int u = max(u0, n_code) + (warp + AW - (max(u0, n_code) - u0) % AW) % AW; u < u1; u += AW) {
+#pragma unroll 1
+            for (int i = 0; i < P::TILES; ++i) {
+                const int tok = p.n8 + (z.tail_unit + u - n_code) * P::UNIT + 16 * i;
+                if (tok >= p.total || hidden(tok)) continue;
+                // (rows that no query sees are not read: what they hold must not reach the sums)
+                auto row = [&](int j, bool keys) -> const char* {
+                    if (j >= p.total || (j < lo_min && j >= p.sinks)) return nullptr;
+                    if (p.kn != nullptr && j == p.total - 1)
+                        return keys ? static_cast<const char*>(p.kn) + 2 * (b * p.kn_sb + kv * p.kn_sh) : static_cast<const char*>(p.vn) + 2 * (b * p.vn_sb + kv * p.vn_sh);
+                    return static_cast<const char*>(keys ? p.kt : p.vt) + 2 * (lane_c * p.block + (j - p.n8)) * D;
+                };
+                auto mag = [](uint2 v) { const uint32_t m = 0x7fff7fffu, y = __vmaxu2(v.x & m, v.y & m); return max(y & 0xffffu, y >> 16); };
+                auto half4 = [&](uint2& v, float f) {
+                    if (!bf) return;
+                    v.x = pack_h2(__uint_as_float(v.x << 16) * f, __uint_as_float(v.x & 0xffff0000u) * f);
+                    v.y = pack_h2(__uint_as_float(v.y << 16) * f, __uint_as_float(v.y & 0xffff0000u) * f);
+                };
+                float kn[2] = {1.f, 1.f}, s[4] = {0.f, 0.f, 0.f, 0.f};
+                {
+                    uint2 x[2][P::KW];
+#pragma unroll
+                    for (int r = 0; r < 2; ++r) {
+                        const char* src = row(tok + g + 8 * r, true);
+                        uint32_t mx = 0;
+#pragma unroll
+                        for (int w = 0; w < P::KW; ++w) {
+                            x[r][w] = src ? *reinterpret_cast<const uint2*>(src + 2 * key_dim<D>(w, t)) : make_uint2(0u, 0u);
+                            mx = max(mx, mag(x[r][w]));
+                        }
+                        if (bf) {
+                            mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+                            mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+                            const float f = stage_scale(mx << 16);
+                            kn[r] = 1.f / f;
+#pragma unroll
+                            for (int w = 0; w < P::KW; ++w) half4(x[r][w], f);
+                        }
+                    }
+#pragma unroll
+                    for (int w = 0; w < P::KW; ++w) mma16816(s, x[0][w].x, x[1][w].x, x[0][w].y, x[1][w].y, bq[w][0], bq[w][1]);
+                }
+                uint2 x[4][P::VW];
+                float f[4] = {1.f, 1.f, 1.f, 1.f};
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const char* src = row(tok + 2 * t + (r & 1) + 8 * (r >> 1), false);
+                    uint32_t mx = 0;
+#pragma unroll
+                    for (int w = 0; w < P::VW; ++w) {
+                        x[r][w] = src ? *reinterpret_cast<const uint2*>(src + 2 * value_dim<D>(w, g)) : make_uint2(0u, 0u);
+                        mx = max(mx, mag(x[r][w]));
+                    }
+                    if (bf) {
+#pragma unroll
+                        for (int off = 4; off < 32; off <<= 1) mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, off));
+                        f[r] = stage_scale(mx << 16);
+#pragma unroll
+                        for (int w = 0; w < P::VW; ++w) half4(x[r][w], f[r]);
+                    }
+                }
+                float vn[2];                           // tokens g and g + 8 sit with the lane of t = g / 2
+#pragma unroll
+                for (int r = 0; r < 2; ++r) {
+                    const float a = __shfl_sync(0xffffffffu, f[2 * r], g >> 1), e = __shfl_sync(0xffffffffu, f[2 * r + 1], g >> 1);
+                    vn[r] = 1.f / ((g & 1) ? e : a);
+                }
+                uint32_t bp[2];
+                weights<D, true>(s, kn[0], kn[1], vn[0], vn[1], tok + g, c, p.window, p.sinks, st, bp);
+#pragma unroll
+                for (int w = 0; w < P::VW; ++w) {
+                    mma16816(st.o[2 * w], __byte_perm(x[0][w].x, x[1][w].x, 0x5410), __byte_perm(x[0][w].x, x[1][w].x, 0x7632), __byte_perm(x[2][w].x, x[3][w].x, 0x5410),
+                             __byte_perm(x[2][w].x, x[3][w].x, 0x7632), bp[0], bp[1]);
+                    mma16816(st.o[2 * w + 1], __byte_perm(x[0][w].y, x[1][w].y, 0x5410), __byte_perm(x[0][w].y, x[1][w].y, 0x7632), __byte_perm(x[2][w].y, x[3][w].y, 0x5410),
+                             __byte_perm(x[2][w].y, x[3][w].y, 0x7632), bp[0], bp[1]);
+                }
+            }
+        }
+        if (p.kn != nullptr && grp == 0 && u1 == z.n_units) {          // whoever has the lane's last unit stores the appended row
+            for (int i = tid; i < D / 4; i += AW * 32) {
+                const int side = i >= D / 8, ch = (i - side * (D / 8)) * 8;
+                const char* src = side ? static_cast<const char*>(p.vn) + 2 * (b * p.vn_sb + kv * p.vn_sh) : static_cast<const char*>(p.kn) + 2 * (b * p.kn_sb + kv * p.kn_sh);
+                char* dst = static_cast<char*>(side ? p.vt_w : p.kt_w) + 2 * (lane_c * p.block + (p.total - 1 - p.n8)) * D;
+                *reinterpret_cast<uint4*>(dst + 2 * ch) = *reinterpret_cast<const uint4*>(src + 2 * ch);
+            }
+        }
+        // ---- the warps' sums into one
+        st.finish();
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+#pragma unroll
+            for (int off = 4; off < 32; off <<= 1) st.l[i] += __shfl_xor_sync(0xffffffffu, st.l[i], off);
+            float* row = red[warp][2 * t + i];
+#pragma unroll
+            for (int w = 0; w < P::VW; ++w) {
+                const int d0 = value_dim<D>(w, g);
+                *reinterpret_cast<float4*>(row + d0) = make_float4(st.o[2 * w][i], st.o[2 * w][2 + i], st.o[2 * w + 1][i], st.o[2 * w + 1][2 + i]);
+            }
+            if (g == 0) { row[D] = st.m[i]; row[D + 1] = st.l[i]; }
+        }
+        __syncthreads();
+        const bool alone = u0 == 0 && u1 == z.n_units;
+        const int slot = int(blockIdx.x - job * z.n_units / z.per);
+        for (int i = tid; i < rows * (D / 4); i += AW * 32) {
+            const int r = i / (D / 4), d0 = (i - r * (D / 4)) * 4;
+            float top = -1e30f, l = 0.f, x[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int w = 0; w < AW; ++w) top = fmaxf(top, red[w][r][D]);
+#pragma unroll
+            for (int w = 0; w < AW; ++w) {
+                const float a = ex2(red[w][r][D] - top);
+                const float4 v = *reinterpret_cast<const float4*>(&red[w][r][d0]);
+                l += a * red[w][r][D + 1];
+                x[0] += a * v.x; x[1] += a * v.y; x[2] += a * v.z; x[3] += a * v.w;
+            }
+            if (alone) {
+                const int rr = r0 + r, ti = rr / p.G, h = kv * p.G + rr - ti * p.G;
+                const float il = 1.f / l;
+                char* dst = static_cast<char*>(p.out) + 2 * (((int64_t(b) * p.Hq + h) * p.Tq + ti) * D + d0);
+                *reinterpret_cast<uint2*>(dst) = bf ? make_uint2(pack_bf2(x[0] * il, x[1] * il), pack_bf2(x[2] * il, x[3] * il)) : make_uint2(pack_h2(x[0] * il, x[1] * il), pack_h2(x[2] * il, x[3] * il));
+            } else {
+                float* part = p.part + ((job * z.slots + slot) * HPG + r) * P::RS;
+                *reinterpret_cast<float4*>(part + d0) = make_float4(x[0], x[1], x[2], x[3]);
+                if (d0 == 0) *reinterpret_cast<float2*>(part + D) = make_float2(top, l);
+            }
+        }
+        __syncthreads();
+    }
+}
+
+// A warp per query row that more than one CTA worked on
+template <int D> __global__ void __launch_bounds__(128) blocks_merge_kernel(const __grid_constant__ BlockAttendParams p, const __grid_constant__ AttendGrid z) {
+    using P = AttendPlan<D>;
+    constexpr int NV = D / 32;
+    const int lane = threadIdx.x & 31;
+    const int64_t row = int64_t(blockIdx.x) * 4 + (threadIdx.x >> 5), job = row / HPG, lane_c = job / z.groups;
+    const int grp = int(job - lane_c * z.groups), rr = grp * HPG + int(row % HPG);
+    pdl_wait();
+    if (job >= z.jobs || rr >= p.Tq * p.G) return;
+    const int64_t c0 = job * z.n_units / z.per, c1 = ((job + 1) * z.n_units - 1) / z.per;
+    if (c0 == c1) return;
+    const int n = int(c1 - c0) + 1;
+    const float* part = p.part + (job * z.slots * HPG + row % HPG) * P::RS;
+    constexpr int STEP = HPG * P::RS;
+    float top = -1e30f, l = 0.f, x[NV];
+    for (int s = lane; s < n; s += 32) top = fmaxf(top, part[int64_t(s) * STEP + D]);
+#pragma unroll
+    for (int off = 16; off; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+#pragma unroll
+    for (int i = 0; i < NV; ++i) x[i] = 0.f;
+#pragma unroll 4
+    for (int s = 0; s < n; ++s) {
+        const float* q = part + int64_t(s) * STEP;
+        const float2 ml = *reinterpret_cast<const float2*>(q + D);
+        const float a = ex2(ml.x - top);
+        l += a * ml.y;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) x[i] += a * q[i * 32 + lane];
+    }
+    const int b = int(lane_c / p.Hkv), kv = int(lane_c - int64_t(b) * p.Hkv), ti = rr / p.G, h = kv * p.G + rr - ti * p.G;
+    const int64_t out = ((int64_t(b) * p.Hq + h) * p.Tq + ti) * D + lane;
+    const float il = 1.f / l;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) store_from_f32(p.out, p.dtype, out + i * 32, x[i] * il);
+}
+
+template <int D> AttendGrid grid_of(const BlockAttendParams& p) {
+    using P = AttendPlan<D>;
+    const Visible v = visible_of(p.total, p.Tq, p.window, p.sinks);
+    AttendGrid z{};
+    const int code_units = (p.n8 + P::UNIT - 1) / P::UNIT;
+    z.low_unit = std::min(v.low, p.n8) / P::UNIT;
+    z.n_win = v.low >= p.n8 ? 0 : code_units - z.low_unit;
+    z.n_sink = (std::min(v.sinks, p.n8) + P::UNIT - 1) / P::UNIT;
+    if (z.n_win > 0) z.n_sink = std::min(z.n_sink, z.low_unit);
+    z.tail_unit = v.sinks > p.n8 ? 0 : std::max(v.low - p.n8, 0) / P::UNIT;
+    z.n_units = z.n_sink + z.n_win + (p.total - p.n8 + P::UNIT - 1) / P::UNIT - z.tail_unit;
+    z.groups = int((int64_t(p.Tq) * p.G + HPG - 1) / HPG);
+    z.jobs = int64_t(p.B) * p.Hkv * z.groups;
+    const int64_t units = z.jobs * z.n_units, ctas = int64_t(blocks_sm_count()) * P::PER_SM;
+    z.per = std::max<int64_t>(AW, (units + ctas - 1) / ctas);
+    z.merge = z.per % z.n_units != 0;                  // (otherwise every row has one CTA)
+    z.slots = int(std::min<int64_t>((z.n_units - 2) / z.per + 2, z.n_units));
+    return z;
+}
+template <int D> size_t split_workspace(const BlockAttendParams& p) {
+    const AttendGrid z = grid_of<D>(p);
+    if (!z.merge) return 0;
+    return size_t(z.jobs) * z.slots * HPG * AttendPlan<D>::RS * sizeof(float);
+}
+
+template <int D> int launch_split(const BlockAttendParams& p, cudaStream_t s) {
+    using P = AttendPlan<D>;
+    const AttendGrid z = grid_of<D>(p);
+    const int64_t blocks = (z.jobs * z.n_units + z.per - 1) / z.per, merge = (z.jobs * HPG + 3) / 4;
+    if (blocks >= (int64_t(1) << 31) || merge >= (int64_t(1) << 31)) return fail(TQ_ERR_UNSUPPORTED, "tq_blocks_attend: too many query rows");
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(unsigned(blocks));
+    cfg.blockDim = dim3(AW * 32);
+    cfg.stream = s;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    if (p.e4m3) cudaLaunchKernelEx(&cfg, blocks_attend_kernel<D, true>, p, z);
+    else cudaLaunchKernelEx(&cfg, blocks_attend_kernel<D, false>, p, z);
+    if (int rc = check_launch("tq_blocks_attend")) return rc;
+    if (!z.merge) return TQ_OK;
+    cfg.gridDim = dim3(unsigned(merge));
+    cfg.blockDim = dim3(128);
+    cudaLaunchKernelEx(&cfg, blocks_merge_kernel<D>, p, z);
+    return check_launch("tq_blocks_attend");
+}
+
+bool split_takes(const BlockAttendParams& p) { return p.dtype != TQ_F32 && (p.D == 64 || p.D == 96 || p.D == 128 || p.D == 256); }
+
+// Arguments -> parameters; done: nothing to compute
+int prepare(const tq_blocks_attend_args* a, BlockAttendParams& p, bool& done) {
+    const char* what = "tq_blocks_attend";
+    if (!a) return fail(TQ_ERR_INVALID, "%s: null args", what);
+    const tq_block_store& s = a->store;
+    if (int rc = check_store(&s, what)) return rc;
+    const bool append = a->k_new.x != nullptr;
+    const int64_t total = s.length + (append ? 1 : 0);
+    if (a->n_q_heads < 0 || a->t_q < 0 || (s.n_kv_heads > 0 && a->n_q_heads % s.n_kv_heads)) return fail(TQ_ERR_INVALID, "%s: %d query heads on %d", what, a->n_q_heads, s.n_kv_heads);
+    if (a->window < 0 || a->sinks < 0) return fail(TQ_ERR_INVALID, "%s: window %lld, sinks %lld", what, (long long)a->window, (long long)a->sinks);
+    if (append != (a->v_new.x != nullptr)) return fail(TQ_ERR_INVALID, "%s: new keys without values", what);
+    if (append && (a->t_q != 1 || s.length % s.block + 1 >= s.block))
+        return fail(TQ_ERR_INVALID, "%s: one new token that does not complete a block can be appended (%lld query tokens, length %lld)", what, (long long)a->t_q, (long long)s.length);
+    if (a->t_q > total) return fail(TQ_ERR_INVALID, "%s: %lld query tokens over %lld in the cache", what, (long long)a->t_q, (long long)total);
+    done = s.batch == 0 || a->n_q_heads == 0 || a->t_q == 0;
+    if (done) return TQ_OK;
+    if (s.n_kv_heads == 0 || !a->q.x || !a->out) return fail(TQ_ERR_INVALID, "%s: null queries or result", what);
+    const int es = s.dtype == TQ_F32 ? 4 : 2;
+    auto rows_ok = [&](const tq_new_rows& r, bool tokens) { return aligned(r.x, 16) && (r.sb * es) % 16 == 0 && (r.sh * es) % 16 == 0 && (!tokens || (r.st * es) % 16 == 0); };
+    if (!rows_ok(a->q, true) || !aligned(a->out, 16) || (append && (!rows_ok(a->k_new, false) || !rows_ok(a->v_new, false))))
+        return fail(TQ_ERR_UNSUPPORTED, "%s: rows must be 16-byte aligned", what);
+    p = BlockAttendParams{};
+    p.kc = static_cast<const uint8_t*>(s.k_codes); p.vc = static_cast<const uint8_t*>(s.v_codes); p.ks = s.k_scales; p.vs = s.v_scales;
+    p.kt = p.kt_w = s.k_tail; p.vt = p.vt_w = s.v_tail;
+    if (append) {
+        p.kn = a->k_new.x; p.vn = a->v_new.x; p.kn_sb = a->k_new.sb; p.kn_sh = a->k_new.sh; p.vn_sb = a->v_new.sb; p.vn_sh = a->v_new.sh;
+    }
+    p.q = a->q.x; p.q_sb = a->q.sb; p.q_sh = a->q.sh; p.q_st = a->q.st;
+    p.out = a->out; p.dtype = s.dtype; p.e4m3 = s.code_type == TQ_CODE_E4M3;
+    p.B = s.batch; p.Hq = a->n_q_heads; p.Hkv = s.n_kv_heads; p.G = a->n_q_heads / s.n_kv_heads; p.D = s.d; p.Tq = int(a->t_q);
+    p.block = s.block; p.shift = log2_of(s.block); p.cap = s.capacity;
+    p.n8 = int(s.length / s.block * s.block); p.total = int(total);
+    p.window = a->window > 0 ? int(std::min<int64_t>(a->window, INT_MAX / 2)) : INT_MAX / 2;
+    p.sinks = int(std::min<int64_t>(a->sinks, INT_MAX / 2));
+    p.scale_log2 = a->scale * LOG2E;
+    p.part = static_cast<float*>(a->workspace);
+    return TQ_OK;
+}
+
+size_t workspace_of(const BlockAttendParams& p) {
+    if (!split_takes(p)) return 0;
+    return p.D == 64 ? split_workspace<64>(p) : p.D == 96 ? split_workspace<96>(p) : p.D == 128 ? split_workspace<128>(p) : split_workspace<256>(p);
+}
+
+}  // namespace
+
+int launch_blocks_plain(const BlockAttendParams& p, cudaStream_t s) {
+    const int64_t rows = int64_t(p.B) * p.Hq * p.Tq;
+    if (rows >= (int64_t(1) << 31)) return fail(TQ_ERR_UNSUPPORTED, "tq_blocks_attend: too many query rows");
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(unsigned(rows));
+    cfg.blockDim = dim3(PL_W * 32);
+    cfg.stream = s;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    cudaLaunchKernelEx(&cfg, blocks_plain_kernel, p);
+    return check_launch("tq_blocks_attend");
+}
+
+}  // namespace tq
+
+extern "C" size_t tq_blocks_attend_workspace(const tq_blocks_attend_args* a) {
+    tq::BlockAttendParams p;
+    bool done = false;
+    if (tq::prepare(a, p, done) != TQ_OK || done) return 0;
+    return tq::workspace_of(p);
+}
+
+extern "C" int tq_blocks_attend(const tq_blocks_attend_args* a, void* stream) {
+    using namespace tq;
+    BlockAttendParams p;
+    bool done = false;
+    if (int rc = prepare(a, p, done)) return rc;
+    if (done) return TQ_OK;
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    if (!split_takes(p)) return launch_blocks_plain(p, s);
+    const size_t need = workspace_of(p);
+    if (need > 0 && (!a->workspace || !aligned(a->workspace, 256) || a->workspace_bytes < need))
+        return fail(TQ_ERR_INVALID, "tq_blocks_attend: workspace %zu B < %zu B, or not 256-byte aligned", a->workspace_bytes, need);
+    if (p.D == 64) return launch_split<64>(p, s);
+    if (p.D == 96) return launch_split<96>(p, s);
+    if (p.D == 128) return launch_split<128>(p, s);
+    return launch_split<256>(p, s);
+}

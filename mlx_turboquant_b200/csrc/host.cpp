@@ -8,12 +8,14 @@
 #include <torch/csrc/python_headers.h>
 
 #include <ATen/ATen.h>
+#include <c10/core/GradMode.h>
 #include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/utils/object_ptr.h>
 
+#include <cmath>
 #include <cstring>
 
 #include "../../include/tq_abi.h"
@@ -298,8 +300,171 @@ PyObject* fetch(PyObject*, PyObject* const* a, Py_ssize_t n) {
     END_HANDLE_TH_ERRORS
 }
 
+// ---- rotary positions, 8-bit blocks ----------------------------------------------------------------------------------
+// Inference only: what asks for a gradient goes back to Python, which refuses it.
+bool plain(const at::Tensor& t, int device) { return here(t, device) && !(t.requires_grad() && c10::GradMode::is_enabled()); }
+// Rows (B, H, T, D) of contiguous coordinates that start on 16 bytes
+bool rows16(const at::Tensor& x, tq_new_rows& r) {
+    const int64_t n = 16 / int64_t(x.element_size());
+    if (x.stride(3) != 1 || reinterpret_cast<uintptr_t>(x.data_ptr()) % 16) return false;
+    int64_t st[3];
+    for (int i = 0; i < 3; ++i) {
+        st[i] = x.size(i) > 1 ? x.stride(i) : 0;
+        if (st[i] % n) return false;
+    }
+    r = tq_new_rows{x.data_ptr(), st[0], st[1], st[2]};
+    return true;
+}
+// rotary(q, k or None, freqs, offset, positions or None, interleaved, factor) -> (q, k or None)
+PyObject* rotary(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    if (n != 7 || !is_tensor(a[0]) || !is_tensor(a[2])) return none();
+    const int device = c10::cuda::current_device();
+    const at::Tensor &q = tensor(a[0]), &f = tensor(a[2]);
+    const int code = type_code(q.scalar_type());
+    if (code < 0 || !plain(q, device) || q.dim() != 4 || !here(f, device) || f.scalar_type() != at::kDouble || f.dim() != 1 || !f.is_contiguous() || f.numel() == 0 ||
+        2 * f.numel() > q.size(3) || !PyLong_Check(a[3]))
+        return none();
+    tq_rotary_args r;
+    std::memset(&r, 0, sizeof r);
+    r.dtype = code; r.batch = int(q.size(0)); r.length = q.size(2); r.d = int(q.size(3)); r.dims = int(2 * f.numel());
+    r.freqs = f.data_ptr<double>(); r.offset = integer(a[3]); r.interleaved = PyObject_IsTrue(a[5]) == 1;
+    r.factor = float(PyFloat_AsDouble(a[6]));
+    if (PyErr_Occurred()) { PyErr_Clear(); return none(); }
+    if (a[4] != Py_None) {
+        if (!is_tensor(a[4])) return none();
+        const at::Tensor& pos = tensor(a[4]);
+        const bool each = pos.dim() == 2;
+        if (!here(pos, device) || pos.scalar_type() != at::kLong || pos.dim() < 1 || pos.dim() > 2 || pos.size(-1) != r.length || (each && pos.size(0) != r.batch) ||
+            (r.length > 1 && pos.stride(-1) != 1))
+            return none();
+        r.positions = pos.data_ptr<int64_t>();
+        r.pos_sb = each && r.batch > 1 ? pos.stride(0) : 0;
+    }
+    at::Tensor out[2];
+    for (int i = 0; i < 2; ++i) {
+        if (i && a[1] == Py_None) continue;
+        if (!is_tensor(a[i])) return none();
+        const at::Tensor& x = tensor(a[i]);
+        if (!plain(x, device) || x.dim() != 4 || x.scalar_type() != q.scalar_type() || x.size(0) != r.batch || x.size(2) != r.length || x.size(3) != r.d || x.stride(3) != 1) return none();
+        out[i] = empty(x.sizes(), x.scalar_type(), device);
+        r.part[i] = tq_rotary_rows{x.data_ptr(), x.stride(0), x.stride(1), x.stride(2), out[i].data_ptr(), int(x.size(1))};
+    }
+    int rc;
+    {
+        Release gil;
+        rc = tq_rotary(&r, stream_of(device));
+    }
+    if (rc) return status(rc);
+    THPObjectPtr first(THPVariable_Wrap(out[0])), second(out[1].defined() ? THPVariable_Wrap(out[1]) : none());
+    return PyTuple_Pack(2, first.get(), second.get());
+    END_HANDLE_TH_ERRORS
+}
+// k_codes, k_scales, v_codes, v_scales, k_tail, v_tail
+bool store_of(PyObject* const* a, int64_t length, int device, tq_block_store& s) {
+    for (int i = 0; i < 6; ++i)
+        if (!is_tensor(a[i]) || !here(tensor(a[i]), device) || !tensor(a[i]).is_contiguous()) return false;
+    const at::Tensor &kc = tensor(a[0]), &ks = tensor(a[1]), &vc = tensor(a[2]), &vs = tensor(a[3]), &kt = tensor(a[4]), &vt = tensor(a[5]);
+    const auto type = kc.scalar_type();
+    const int code = type_code(kt.scalar_type());
+    if ((type != at::kChar && type != at::kFloat8_e4m3fn) || vc.scalar_type() != type || ks.scalar_type() != at::kFloat || vs.scalar_type() != at::kFloat || code < 0 ||
+        vt.scalar_type() != kt.scalar_type() || kc.dim() != 4 || ks.dim() != 3 || kt.dim() != 4)
+        return false;
+    const int64_t b = kc.size(0), h = kc.size(1), cap = kc.size(2), d = kc.size(3), block = kt.size(2);
+    if ((block != 16 && block != 32 && block != 64 && block != 128) || vc.sizes() != kc.sizes() || kt.size(0) != b || kt.size(1) != h || kt.size(3) != d || vt.sizes() != kt.sizes() ||
+        cap % block || ks.size(0) != b || ks.size(1) != h || ks.size(2) != cap / block || vs.sizes() != ks.sizes() || length < 0 || length / block * block > cap)
+        return false;
+    s = tq_block_store{int(b), int(h), int(d), int(block), type == at::kChar ? TQ_CODE_INT8 : TQ_CODE_E4M3, code, kc.data_ptr(), vc.data_ptr(), ks.data_ptr<float>(), vs.data_ptr<float>(),
+                       kt.data_ptr(), vt.data_ptr(), cap, length};
+    return true;
+}
+bool new_rows(PyObject* ko, PyObject* vo, const at::Tensor& tail, int device, tq_new_rows& k, tq_new_rows& v, int64_t& t) {
+    if (!is_tensor(ko) || !is_tensor(vo)) return false;
+    const at::Tensor &kn = tensor(ko), &vn = tensor(vo);
+    if (!plain(kn, device) || !plain(vn, device) || kn.dim() != 4 || kn.sizes() != vn.sizes() || kn.scalar_type() != tail.scalar_type() || vn.scalar_type() != tail.scalar_type() ||
+        kn.size(0) != tail.size(0) || kn.size(1) != tail.size(1) || kn.size(3) != tail.size(3) || !rows16(kn, k) || !rows16(vn, v))
+        return false;
+    t = kn.size(2);
+    return true;
+}
+// blocks_write(keys, values, storage x 6, length) -> the new length
+PyObject* blocks_write(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    if (n != 9 || !PyLong_Check(a[8])) return none();
+    const int device = c10::cuda::current_device();
+    const int64_t length = integer(a[8]);
+    tq_block_store s;
+    tq_new_rows k, v;
+    int64_t t = 0;
+    if (!store_of(a + 2, length, device, s) || !new_rows(a[0], a[1], tensor(a[6]), device, k, v, t) || (length + t) / s.block * s.block > s.capacity) return none();
+    int rc;
+    {
+        Release gil;
+        rc = tq_blocks_write(&s, &k, &v, t, stream_of(device));
+    }
+    return rc ? status(rc) : PyLong_FromLongLong(length + t);
+    END_HANDLE_TH_ERRORS
+}
+// blocks_read(storage x 6, length) -> dense keys and values of the tails' type
+PyObject* blocks_read(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    if (n != 7 || !PyLong_Check(a[6])) return none();
+    const int device = c10::cuda::current_device();
+    const int64_t length = integer(a[6]);
+    tq_block_store s;
+    if (!store_of(a, length, device, s)) return none();
+    const int64_t size[4] = {s.batch, s.n_kv_heads, length, s.d};
+    const auto type = tensor(a[4]).scalar_type();
+    at::Tensor k = empty(size, type, device), v = empty(size, type, device);
+    int rc;
+    {
+        Release gil;
+        rc = tq_blocks_read(&s, k.data_ptr(), v.data_ptr(), s.dtype, stream_of(device));
+    }
+    if (rc) return status(rc);
+    return PyTuple_Pack(2, THPObjectPtr(THPVariable_Wrap(k)).get(), THPObjectPtr(THPVariable_Wrap(v)).get());
+    END_HANDLE_TH_ERRORS
+}
+// blocks_attend(queries, storage x 6, length, window or 0, sinks, scale or None, new keys or None, new values or None) -> result
+PyObject* blocks_attend(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    if (n != 13 || !is_tensor(a[0]) || !PyLong_Check(a[7]) || !PyLong_Check(a[8]) || !PyLong_Check(a[9])) return none();
+    const int device = c10::cuda::current_device();
+    const at::Tensor& q = tensor(a[0]);
+    tq_blocks_attend_args r;
+    std::memset(&r, 0, sizeof r);
+    const int64_t length = integer(a[7]);
+    if (!store_of(a + 1, length, device, r.store)) return none();
+    const tq_block_store& s = r.store;
+    if (!plain(q, device) || q.dim() != 4 || q.scalar_type() != tensor(a[5]).scalar_type() || q.size(0) != s.batch || q.size(3) != s.d || s.n_kv_heads == 0 || q.size(1) % s.n_kv_heads ||
+        q.numel() == 0 || !rows16(q, r.q))
+        return none();
+    r.n_q_heads = int(q.size(1)); r.t_q = q.size(2);
+    r.window = integer(a[8]); r.sinks = integer(a[9]);
+    r.scale = a[10] == Py_None ? float(1.0 / std::sqrt(double(s.d))) : float(PyFloat_AsDouble(a[10]));
+    if (PyErr_Occurred()) { PyErr_Clear(); return none(); }
+    int64_t t = 0;
+    if (a[11] != Py_None && (r.t_q != 1 || length % s.block + 1 == s.block || !new_rows(a[11], a[12], tensor(a[5]), device, r.k_new, r.v_new, t) || t != 1)) return none();
+    if (r.window < 0 || r.sinks < 0 || r.t_q > length + t) return none();
+    at::Tensor out = empty(q.sizes(), q.scalar_type(), device), ws;
+    r.out = out.data_ptr();
+    r.workspace_bytes = tq_blocks_attend_workspace(&r);
+    if (r.workspace_bytes) {
+        ws = empty({int64_t(r.workspace_bytes)}, at::kByte, device);
+        r.workspace = ws.data_ptr();
+    }
+    int rc;
+    {
+        Release gil;
+        rc = tq_blocks_attend(&r, stream_of(device));
+    }
+    return rc ? status(rc) : THPVariable_Wrap(out);
+    END_HANDLE_TH_ERRORS
+}
+
 #define FAST(name) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(name)), METH_FASTCALL, nullptr}
-PyMethodDef methods[] = {FAST(codec_quantize), FAST(codec_dequantize), FAST(append), FAST(buffers), FAST(storage), FAST(quantize), FAST(fetch), {nullptr, nullptr, 0, nullptr}};
+PyMethodDef methods[] = {FAST(codec_quantize), FAST(codec_dequantize), FAST(append), FAST(buffers), FAST(storage), FAST(quantize), FAST(fetch), FAST(rotary), FAST(blocks_write), FAST(blocks_read), FAST(blocks_attend),
+                         {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_host", "Native host path; see csrc/host.cpp.", -1, methods};
 
 }  // namespace
