@@ -36,6 +36,9 @@ struct BlockAttendParams {
 };
 
 int launch_blocks_plain(const BlockAttendParams& p, cudaStream_t s);
+bool blocks_fa_takes(const BlockAttendParams& p);
+size_t blocks_fa_workspace(const BlockAttendParams& p);
+int launch_blocks_fa(const BlockAttendParams& p, cudaStream_t s);
 
 // The first token that some query sees through its window, and how many sink tokens lie before it
 struct Visible { int low, sinks; };
@@ -48,6 +51,25 @@ __device__ __forceinline__ float e4m3_to_f32(uint8_t c) {
     uint32_t h;
     asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"(uint16_t(c)));
     return __half2float(__ushort_as_half(uint16_t(h & 0xffffu)));
+}
+
+__device__ __forceinline__ void ld_codes(uint4& x, const uint8_t* p) {
+    asm volatile("ld.global.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(x.x), "=r"(x.y), "=r"(x.z), "=r"(x.w) : "l"(p) : "memory");
+}
+__device__ __forceinline__ void st_shared(uint32_t at, uint4 x) {
+    asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(at), "r"(x.x), "r"(x.y), "r"(x.z), "r"(x.w) : "memory");
+}
+// four codes as two pairs of fp16.  int8: biased by 128 they are the low bytes of 1024 + code + 128
+template <bool E4M3> __device__ __forceinline__ void halves(uint32_t w, uint32_t& lo, uint32_t& hi) {
+    if constexpr (E4M3) {
+        asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, a;\n\tcvt.rn.f16x2.e4m3x2 %1, b;\n\t}" : "=r"(lo), "=r"(hi) : "r"(w));
+    } else {
+        const uint32_t u = w ^ 0x80808080u;
+        const uint32_t k = 0x64806480u;
+        uint32_t a = __byte_perm(u, 0x64646464u, 0x4140), b = __byte_perm(u, 0x64646464u, 0x4342);
+        asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(lo) : "r"(a), "r"(k));
+        asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(hi) : "r"(b), "r"(k));
+    }
 }
 
 }  // namespace tq

@@ -20,10 +20,6 @@
 
 namespace tq {
 
-bool blocks_fa_takes(const BlockAttendParams& p);
-size_t blocks_fa_workspace(const BlockAttendParams& p);
-int launch_blocks_fa(const BlockAttendParams& p, cudaStream_t s);
-
 namespace {
 
 // ---------------------------------------------------------------------------------------------------- float32, any head_dim
@@ -133,19 +129,6 @@ template <int D> __device__ __forceinline__ int key_dim(int w, int t) {
 template <int D> __device__ __forceinline__ int value_dim(int w, int g) {
     const int i = w / (Pieces<D>::V / 32);
     return Pieces<D>::V * i + Pieces<D>::value_bytes(i) * g + 4 * (w - i * (Pieces<D>::V / 32));
-}
-
-// four codes as two pairs of fp16.  int8: biased by 128 they are the low bytes of 1024 + code + 128
-template <bool E4M3> __device__ __forceinline__ void halves(uint32_t w, uint32_t& lo, uint32_t& hi) {
-    if constexpr (E4M3) {
-        asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, a;\n\tcvt.rn.f16x2.e4m3x2 %1, b;\n\t}" : "=r"(lo), "=r"(hi) : "r"(w));
-    } else {
-        const uint32_t u = w ^ 0x80808080u;
-        const uint32_t k = 0x64806480u;
-        uint32_t a = __byte_perm(u, 0x64646464u, 0x4140), b = __byte_perm(u, 0x64646464u, 0x4342);
-        asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(lo) : "r"(a), "r"(k));
-        asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(hi) : "r"(b), "r"(k));
-    }
 }
 
 template <int D> struct Unit {                         // a unit's codes and scales in a lane's registers
@@ -378,12 +361,18 @@ template <int D, bool E4M3> __global__ void __launch_bounds__(AW * 32, AttendPla
                         x[r][w] = src ? *reinterpret_cast<const uint2*>(src + 2 * value_dim<D>(w, g)) : make_uint2(0u, 0u);
                         mx = max(mx, mag(x[r][w]));
                     }
-                    if (bf) {
 #pragma unroll
-                        for (int off = 4; off < 32; off <<= 1) mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, off));
+                    for (int off = 4; off < 32; off <<= 1) mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, off));
+                    if (bf) {
                         f[r] = stage_scale(mx << 16);
 #pragma unroll
                         for (int w = 0; w < P::VW; ++w) half4(x[r][w], f[r]);
+                    }
+                    // values that are not finite would reach queries that they are hidden from as 0 * inf: zeros, and a score of NaN
+                    if (mx >= (bf ? 0x7f80u : 0x7c00u)) {
+                        f[r] = __uint_as_float(0x7fffffffu);
+#pragma unroll
+                        for (int w = 0; w < P::VW; ++w) x[r][w] = make_uint2(0u, 0u);
                     }
                 }
                 float vn[2];                           // tokens g and g + 8 sit with the lane of t = g / 2
@@ -391,6 +380,7 @@ template <int D, bool E4M3> __global__ void __launch_bounds__(AW * 32, AttendPla
                 for (int r = 0; r < 2; ++r) {
                     const float a = __shfl_sync(0xffffffffu, f[2 * r], g >> 1), e = __shfl_sync(0xffffffffu, f[2 * r + 1], g >> 1);
                     vn[r] = 1.f / ((g & 1) ? e : a);
+                    if (vn[r] != vn[r]) { kn[r] = vn[r]; vn[r] = 0.f; }
                 }
                 uint32_t bp[2];
                 weights<D, true>(s, kn[0], kn[1], vn[0], vn[1], tok + g, c, p.window, p.sinks, st, bp);
@@ -583,6 +573,7 @@ int prepare(const tq_blocks_attend_args* a, BlockAttendParams& p, bool& done) {
 
 size_t workspace_of(const BlockAttendParams& p) {
     if (!split_takes(p)) return 0;
+    if (blocks_fa_takes(p)) return blocks_fa_workspace(p);
     return p.D == 64 ? split_workspace<64>(p) : p.D == 96 ? split_workspace<96>(p) : p.D == 128 ? split_workspace<128>(p) : split_workspace<256>(p);
 }
 
@@ -624,6 +615,7 @@ extern "C" int tq_blocks_attend(const tq_blocks_attend_args* a, void* stream) {
     const size_t need = workspace_of(p);
     if (need > 0 && (!a->workspace || !aligned(a->workspace, 256) || a->workspace_bytes < need))
         return fail(TQ_ERR_INVALID, "tq_blocks_attend: workspace %zu B < %zu B, or not 256-byte aligned", a->workspace_bytes, need);
+    if (blocks_fa_takes(p)) return launch_blocks_fa(p, s);
     if (p.D == 64) return launch_split<64>(p, s);
     if (p.D == 96) return launch_split<96>(p, s);
     if (p.D == 128) return launch_split<128>(p, s);

@@ -167,12 +167,14 @@ def test_windows_and_sinks(d, block, codes, dtype, total):
                                                  (256, 64, torch.int8, torch.float16), (128, 128, torch.int8, torch.float32)))
 def test_several_tokens(d, block, codes, dtype):
     from mlx_turboquant_b200 import blocks
-    for b, hq, h, total, t in ((1, 4, 1, 2, 2), (2, 8, 2, 77, 5), (1, 6, 2, 300, 130), (1, 3, 3, 200, 200), (2, 8, 8, 1100, 33)):
+    for b, hq, h, total, t in ((1, 4, 1, 2, 2), (2, 8, 2, 77, 5), (1, 6, 2, 300, 130), (1, 3, 3, 200, 200), (2, 8, 8, 1100, 33), (1, 8, 2, 2500, 700), (1, 12, 1, 1337, 150)):
         store = filled(b, h, total, d, block, codes, dtype, seed=t)
         q = rows(b, hq, t, d, dtype, 5, std=0)
         k, v = dense(store, total)
         for window, sinks in ((None, 0), (1, 0), (20, 3), (64, 70), (300, 4)):
             check_attention(blocks.attend_blocks(q, *store, total, window=window, sinks=sinks), q, k, v, d ** -0.5, window, sinks)
+    from mlx_turboquant_b200 import _lib
+    assert _lib.lib().tq_device_status() == 0
 
 
 @pytest.mark.parametrize("dtype", (torch.float16, torch.bfloat16, torch.float32))
@@ -216,6 +218,31 @@ def test_hidden_values_do_not_count():
                 assert bool(ref.isfinite().all())
             else:
                 assert torch.equal(blocks.attend_blocks(q, *store, total, window=window, sinks=2), ref)
+
+
+@pytest.mark.parametrize("t", (5, 90))
+@pytest.mark.parametrize("dtype", (torch.float16, torch.bfloat16, torch.float32))
+def test_what_is_not_finite_reaches_those_who_see_it(dtype, t):
+    """A NaN or an infinity in one token: NaN for the queries that see it, the same bits as without it for the others."""
+    from mlx_turboquant_b200 import blocks
+    for total, at, side, bad in ((250, 247, 0, float("nan")), (250, 248, 1, float("nan")), (250, 246, 1, float("inf")), (200, 199, 1, float("-inf"))):
+        k, v = rows(1, 2, total, 64, dtype, 1), rows(1, 2, total, 64, dtype, 2)
+        q = rows(1, 8, t, 64, dtype, 3, std=0)
+        store = storage(1, 2, total, 64, 128, torch.int8, dtype)
+        blocks.write_blocks(k, v, *store, 0)
+        for window in (None, 3):
+            clean = blocks.attend_blocks(q, *store, total, window=window).clone()
+            tail = store[4 + side]
+            kept = tail.clone()
+            tail[:, :, at - 128, 7] = bad
+            got = blocks.attend_blocks(q, *store, total, window=window)
+            tail.copy_(kept)
+            pos = torch.arange(total - t, total)
+            sees = (pos >= at) & ((pos - at < window) if window else True)
+            assert bool(sees.any())
+            assert torch.equal(got[:, :, ~sees], clean[:, :, ~sees])
+            hit = got[:, :, sees]
+            assert bool((~hit.isfinite()).any(-1).all())
 
 
 def test_extreme_scales():
