@@ -5,11 +5,11 @@
 // The integers are exact as fp16, and so are the 8-bit floats: scores are products of codes with the query as it came (a bfloat16 one under a
 // power of two), the scales follow in float32, the values' scale on the softmax weights.  Only those are rounded, to fp16.
 //
-// blocks_attend_kernel: bound by the codes' bytes.  Work is a flat sequence of units (16 or 32 tokens) of all (lane, group of 8 query rows); a CTA of four warps
-// takes an equal run of it, whatever lanes that touches, a warp every fourth unit of a lane.  A warp reads its next unit's codes straight into registers
-// (16 bytes a lane, whole sectors) while it computes on this one: mma.sync m16n8k16 with the tokens as M (scores) and the coordinates as M (values), so
-// that eight query rows share every converted code.  Which coordinate a fragment's row or column stands for is free as long as queries and results agree:
-// a lane's 16 bytes are four fragments.  (The products are tiny, N = 8: tcgen05 would want 64 rows of operands staged in shared memory as fp16.)
+// blocks_attend_kernel: bound by the codes' bytes.  Work is a flat sequence of tiles (16 tokens) of all (lane, group of 8 query rows); a CTA of eight warps
+// takes an equal run of it, whatever lanes that touches, a warp every eighth tile of a lane.  Codes go through a ring of each warp's own in shared memory
+// (cp.async, 16 bytes a lane); mma.sync m16n8k16 with the tokens as M (scores) and the coordinates as M (values), so that eight query rows share every
+// converted code.  Which coordinate a fragment's row or column stands for is free as long as queries and results agree: a lane's 16 bytes are four
+// fragments.  (The products are tiny, N = 8: tcgen05 would want 64 rows of operands staged in shared memory as fp16.)
 // blocks_merge_kernel: joins the partials of a row that several CTAs worked on, in their order: results do not depend on which one came first.
 // blocks_plain_kernel: a warp per token on CUDA cores, float32 throughout: float32 tokens, head dims without a layout above.
 #include <algorithm>
@@ -79,62 +79,70 @@ __global__ void __launch_bounds__(PL_W * 32) blocks_plain_kernel(const __grid_co
 }
 
 // ---------------------------------------------------------------------------------------------------- 16-bit tokens
-constexpr int AW = 4;                                  // warps of a CTA
+constexpr int AW = 8;                                  // warps of a CTA
 
-// A code row's bytes of a lane: pieces of the row, each shared evenly by the four (keys) or eight (values) lanes that hold parts of the row
-template <int D> struct Pieces {
-    static constexpr int K = 64, V = D >= 128 ? 128 : 64;      // bytes of a piece; the last one may be shorter (d = 96)
-    static __host__ __device__ constexpr int key_bytes(int i) { return D - K * i < K ? (D - K * i) / 4 : K / 4; }
-    static __host__ __device__ constexpr int value_bytes(int i) { return D - V * i < V ? (D - V * i) / 8 : V / 8; }
-};
-
+// A tile is 16 tokens.  Each warp has a ring of ST tiles of codes in shared memory, row by row in 16-byte pieces; piece `c` of row `r` sits at place c ^ swizzle(r),
+// which keeps the fragment reads below free of bank conflicts.
 template <int D> struct AttendPlan {
-    static constexpr int TILES = D == 256 ? 1 : 2;     // 16-token tiles of a unit
-    static constexpr int UNIT = 16 * TILES;
-    static constexpr int PER_SM = D == 64 ? 4 : D == 96 ? 3 : 2;
+    static constexpr int PER_SM = D == 256 ? 1 : 2;    // CTAs per SM
+    static constexpr int ST = D == 64 ? 6 : D == 96 ? 4 : 3;
+    static constexpr int CPR = D / 16;                 // 16-byte pieces of a row
+    static constexpr uint32_t SIDE = 16 * D, STAGE = 2 * SIDE + 16;          // keys, values, their scales
     static constexpr int KW = D / 16, VW = D / 32;     // words of a lane per key row (two a tile) and value row (four)
     static constexpr int RS = D + 4;                   // floats of a partial row: sums, maximum, sum of weights
+    static constexpr size_t RING = size_t(AW) * ST * STAGE, RED = size_t(AW) * HPG * RS * 4, SMEM = RING > RED ? RING : RED;
 };
 
 struct AttendGrid {
-    int n_units, n_sink, n_win, low_unit, tail_unit;   // units of a (lane, group): sink tokens, window tokens in blocks, the tail's from tail_unit on
+    int n_units, n_sink, n_win, low_unit, tail_unit;   // tiles of a (lane, group): sink tokens, window tokens in blocks, the tail's from tail_unit on
     int groups, slots;                                 // groups of 8 query rows per lane; partials of one
     int merge;                                         // the merge kernel follows
-    int64_t per;                                       // units of a CTA
-    int64_t jobs;                                      // lanes x groups
+    uint32_t per, jobs;                                // tiles of a CTA; lanes x groups
 };
 
-template <int BYTES> __device__ __forceinline__ void ld_bytes(const uint8_t* p, uint32_t* w) {
-    if constexpr (BYTES == 16) asm volatile("ld.global.L1::no_allocate.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "l"(p) : "memory");
-    else if constexpr (BYTES == 8) asm volatile("ld.global.L1::no_allocate.v2.b32 {%0,%1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "l"(p) : "memory");
-    else asm volatile("ld.global.L1::no_allocate.b32 %0, [%1];" : "=r"(w[0]) : "l"(p) : "memory");
-}
-template <int D, int I = 0> __device__ __forceinline__ void ld_key_row(const uint8_t* row, int t, uint32_t* w) {
-    if constexpr (Pieces<D>::K * I < D) {
-        ld_bytes<Pieces<D>::key_bytes(I)>(row + Pieces<D>::K * I + Pieces<D>::key_bytes(I) * t, w);
-        ld_key_row<D, I + 1>(row, t, w + Pieces<D>::key_bytes(I) / 4);
-    }
-}
-template <int D, int I = 0> __device__ __forceinline__ void ld_value_row(const uint8_t* row, int g, uint32_t* w) {
-    if constexpr (Pieces<D>::V * I < D) {
-        ld_bytes<Pieces<D>::value_bytes(I)>(row + Pieces<D>::V * I + Pieces<D>::value_bytes(I) * g, w);
-        ld_value_row<D, I + 1>(row, g, w + Pieces<D>::value_bytes(I) / 4);
-    }
-}
-// first of the four coordinates of word w of a lane's part of a key row / value row
+// Which coordinates a lane's words are: a lane of t (keys) or g (values) holds 16-byte pieces of a row where the row has enough of them for all lanes, else parts of one.
+//   keys, words of 4 codes:   d = 128 pieces 2 t, 2 t + 1;   256 pieces 4 t ... + 3;   64 piece t;   96 pieces t (0 ... 3), then half a piece of the last two
+//   values:                   d = 128 piece g;   256 pieces 2 g, + 1;   64 half of piece g / 2;   96 half of piece g / 2 (0 ... 3), then a quarter of the last two
 template <int D> __device__ __forceinline__ int key_dim(int w, int t) {
-    const int i = w / (Pieces<D>::K / 16);
-    return Pieces<D>::K * i + Pieces<D>::key_bytes(i) * t + 4 * (w - i * (Pieces<D>::K / 16));
+    if (D == 96) return w < 4 ? 16 * t + 4 * w : 64 + 8 * t + 4 * (w - 4);
+    return (D / 4) * t + 4 * w;
 }
 template <int D> __device__ __forceinline__ int value_dim(int w, int g) {
-    const int i = w / (Pieces<D>::V / 32);
-    return Pieces<D>::V * i + Pieces<D>::value_bytes(i) * g + 4 * (w - i * (Pieces<D>::V / 32));
+    if (D == 96) return w < 2 ? 8 * g + 4 * w : 64 + 4 * g;
+    return (D / 8) * g + 4 * w;
 }
-
-template <int D> struct Unit {                         // a unit's codes and scales in a lane's registers
-    uint32_t k[AttendPlan<D>::TILES][2][AttendPlan<D>::KW], v[AttendPlan<D>::TILES][4][AttendPlan<D>::VW];
-    float ks[AttendPlan<D>::TILES], vs[AttendPlan<D>::TILES];
-};
+// Place of piece c of row r.  A read of 16 bytes is eight lanes at a time.  Keys: two rows (g, g + 1) x four pieces; values: four rows (2 t) x two pieces; with 8 or 16
+// pieces a row, 128 or 256 bytes, a row's low bits over the piece's do for both.  d = 64: eight bytes a value lane, sixteen lanes at a time, four rows x two pieces.
+template <int D> __device__ __forceinline__ uint32_t place(int r, int c) {
+    if (D == 128) return uint32_t(r * 8 + (c ^ (r & 7)));
+    if (D == 256) return uint32_t(r * 16 + (c ^ ((c >> 3) * 2) ^ (((r ^ (r >> 1)) & 1) + ((r >> 2) & 1) * 4)));
+    if (D == 64 || c < 4) return uint32_t(r * 4 + (c ^ ((r >> 1) & 3)));
+    return uint32_t(64 + r * 2 + (c - 4));             // (d = 96: two regions)
+}
+template <int BYTES> __device__ __forceinline__ void ld_ring(uint32_t at, uint32_t* w) {
+    if constexpr (BYTES == 16) asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(at) : "memory");
+    else if constexpr (BYTES == 8) asm volatile("ld.shared.v2.b32 {%0,%1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "r"(at) : "memory");
+    else asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w[0]) : "r"(at) : "memory");
+}
+template <int D> __device__ __forceinline__ void key_row(uint32_t side, int r, int t, uint32_t* w) {
+    if constexpr (D == 96) {
+        ld_ring<16>(side + place<D>(r, t) * 16, w);
+        ld_ring<8>(side + place<D>(r, 4 + (t >> 1)) * 16 + (t & 1) * 8, w + 4);
+    } else {
+#pragma unroll
+        for (int i = 0; i < D / 64; ++i) ld_ring<16>(side + place<D>(r, (D / 64) * t + i) * 16, w + 4 * i);
+    }
+}
+template <int D> __device__ __forceinline__ void value_row(uint32_t side, int r, int g, uint32_t* w) {
+    if constexpr (D == 64) ld_ring<8>(side + place<D>(r, g >> 1) * 16 + (g & 1) * 8, w);
+    else if constexpr (D == 96) {
+        ld_ring<8>(side + place<D>(r, g >> 1) * 16 + (g & 1) * 8, w);
+        ld_ring<4>(side + place<D>(r, 4 + (g >> 2)) * 16 + (g & 3) * 4, w + 2);
+    } else {
+#pragma unroll
+        for (int i = 0; i < D / 128; ++i) ld_ring<16>(side + place<D>(r, (D / 128) * g + i) * 16, w + 4 * i);
+    }
+}
 
 // What a lane knows of the query columns 2 t and 2 t + 1 of its group
 struct Cols {
@@ -143,13 +151,15 @@ struct Cols {
     int pos_min, pos_max;                              // of the group
 };
 
-// Scores of 16 tokens (rows g, g + 8) times their scales -> running softmax -> the weights as the value products' operand.  tok: token of row g.
-template <int D, bool MASKED>
-__device__ __forceinline__ void weights(float (&s)[4], float kn0, float kn1, float vn0, float vn1, int tok, const Cols& c, int window, int sinks, WarpAcc<D, 0>& st, uint32_t (&bp)[2]) {
+// Scores of 16 tokens (rows g, g + 8) times their scales -> running softmax -> the weights as the value products' operand, as fp16 and what that leaves
+// (fp16 results: the weights' rounding, 2^-12 on average, would be as large as the result's own).  tok: token of row g.
+template <int D>
+__device__ __forceinline__ void weights(float (&s)[4], float kn0, float kn1, float vn0, float vn1, bool masked, int tok, const Cols& c, int window, int sinks, WarpAcc<D, 0>& st,
+                                        uint32_t (&bp)[2], uint32_t (&rest)[2], bool fine) {
     s[0] *= kn0 * c.scale[0]; s[1] *= kn0 * c.scale[1];
     s[2] *= kn1 * c.scale[0]; s[3] *= kn1 * c.scale[1];
     bool hide[4] = {false, false, false, false};
-    if (MASKED) {
+    if (masked) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const int j = tok + 8 * (i >> 1), pos = c.pos[i & 1];
@@ -165,61 +175,99 @@ __device__ __forceinline__ void weights(float (&s)[4], float kn0, float kn1, flo
     st.l[0] += p0 + p2;
     st.l[1] += p1 + p3;
     const float w0 = vn0 * st.vsc, w1 = vn1 * st.vsc;
-    float x0 = p0 * w0, x1 = p1 * w0, x2 = p2 * w1, x3 = p3 * w1;
-    if (MASKED) {                                      // (a hidden token's scale may be a NaN)
-        if (hide[0]) x0 = 0.f;
-        if (hide[1]) x1 = 0.f;
-        if (hide[2]) x2 = 0.f;
-        if (hide[3]) x3 = 0.f;
+    float x[4] = {p0 * w0, p1 * w0, p2 * w1, p3 * w1};
+    if (masked) {                                      // (a hidden token's scale may be a NaN)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (hide[i]) x[i] = 0.f;
     }
-    bp[0] = movm_t(pack_h2(x0, x1));
-    bp[1] = movm_t(pack_h2(x2, x3));
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const __half2 h = __floats2half2_rn(x[2 * i], x[2 * i + 1]);
+        bp[i] = movm_t(*reinterpret_cast<const uint32_t*>(&h));
+        if (fine) {
+            const float2 hf = __half22float2(h);
+            rest[i] = movm_t(pack_h2(x[2 * i] - hf.x, x[2 * i + 1] - hf.y));
+        }
+    }
 }
 
 template <int D, bool E4M3> __global__ void __launch_bounds__(AW * 32, AttendPlan<D>::PER_SM) blocks_attend_kernel(const __grid_constant__ BlockAttendParams p, const __grid_constant__ AttendGrid z) {
     using P = AttendPlan<D>;
-    __shared__ __align__(16) float red[AW][HPG][P::RS];
+    constexpr int ST = P::ST;
+    extern __shared__ __align__(16) unsigned char smem[];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
-    const int64_t u_first = int64_t(blockIdx.x) * z.per, u_last = min(u_first + z.per, z.jobs * z.n_units);
+    const uint32_t u_first = blockIdx.x * z.per, u_last = min(u_first + z.per, z.jobs * uint32_t(z.n_units));
     const bool bf = p.dtype == TQ_BF16;
+    const uint32_t ring = static_cast<uint32_t>(__cvta_generic_to_shared(smem)) + uint32_t(warp) * ST * P::STAGE;
+    const int n_code = z.n_sink + z.n_win;
     pdl_wait();
     if (z.merge) pdl_trigger();                        // (the grid is one wave: the merge's CTAs take nobody's place)
 
-    for (int64_t at = u_first; at < u_last;) {
-        const int64_t job = at / z.n_units, lane_c = job / z.groups;
-        const int u0 = int(at - job * z.n_units), u1 = int(min(int64_t(z.n_units), u0 + (u_last - at)));
-        at += u1 - u0;
-        const int grp = int(job - lane_c * z.groups), b = int(lane_c / p.Hkv), kv = int(lane_c - int64_t(b) * p.Hkv);
+    for (uint32_t at = u_first; at < u_last;) {
+        const uint32_t job = at / uint32_t(z.n_units), lane_u = job / uint32_t(z.groups);
+        const int u0 = int(at - job * uint32_t(z.n_units)), u1 = int(min(uint32_t(z.n_units), u0 + (u_last - at)));
+        at += uint32_t(u1 - u0);
+        const int grp = int(job - lane_u * uint32_t(z.groups)), b = int(lane_u / uint32_t(p.Hkv)), kv = int(lane_u) - b * p.Hkv;
+        const int64_t lane_c = lane_u;
+
+        // ---- this warp's tiles of codes are asked for first
+        const uint8_t* kc = p.kc + lane_c * p.cap * D;
+        const uint8_t* vc = p.vc + lane_c * p.cap * D;
+        const float* sc = (lane ? p.vs : p.ks) + lane_c * (p.cap >> p.shift);
+        auto base_of = [&](int u) { return (u < z.n_sink ? u : z.low_unit + u - z.n_sink) * 16; };
+        const int end = min(u1, n_code);
+        int next = u0 + warp, fill = 0, use = 0;       // the next tile to be asked for; ring places
+        auto ask = [&]() {
+            if (next < end) {
+                const int base = base_of(next);
+                const uint8_t* ks = kc + int64_t(base) * D;
+                const uint8_t* vs = vc + int64_t(base) * D;
+                const uint32_t dst = ring + fill * P::STAGE;
+#pragma unroll
+                for (int i = 0; i < (16 * P::CPR + 31) / 32; ++i) {
+                    const int x = lane + 32 * i, r = x / P::CPR;
+                    const uint32_t pl = place<D>(r, x - r * P::CPR) * 16;
+                    cp_async16(dst + pl, ks + x * 16, 16);
+                    cp_async16(dst + P::SIDE + pl, vs + x * 16, 16);
+                }
+                if (lane < 2) asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst + 2 * P::SIDE + 4 * lane), "l"(sc + (base >> p.shift)) : "memory");
+            }
+            cp_async_commit();
+            next += AW;
+            fill = fill + 1 == ST ? 0 : fill + 1;
+        };
+#pragma unroll
+        for (int i = 0; i < ST - 1; ++i) ask();
+
+        // ---- the group's queries as B operands (row g's coordinates in the order of the key codes), bfloat16 under a power of two
         const int rows = min(HPG, p.Tq * p.G - grp * HPG), r0 = grp * HPG;
         Cols c;
         uint32_t bq[D / 16][2];
         {
-            // ---- the group's queries as B operands (row g's coordinates in the order of the key codes), bfloat16 under a power of two
             const bool has = g < rows;
             const int r = r0 + g, ti = r / p.G, h = kv * p.G + r - ti * p.G;
             const char* q = static_cast<const char*>(p.q) + 2 * (b * p.q_sb + h * p.q_sh + ti * p.q_st);
-            uint2 x[D / 16];
             uint32_t mx = 0;
 #pragma unroll
             for (int w = 0; w < D / 16; ++w) {
-                x[w] = has ? *reinterpret_cast<const uint2*>(q + 2 * key_dim<D>(w, t)) : make_uint2(0u, 0u);
-                const uint32_t m = 0x7fff7fffu, y = __vmaxu2(x[w].x & m, x[w].y & m);
-                mx = max(mx, max(y & 0xffffu, y >> 16));
+                const uint2 x = has ? *reinterpret_cast<const uint2*>(q + 2 * key_dim<D>(w, t)) : make_uint2(0u, 0u);
+                bq[w][0] = x.x; bq[w][1] = x.y;
             }
             float f = 1.f;
             if (bf) {
+#pragma unroll
+                for (int w = 0; w < D / 16; ++w) {
+                    const uint32_t m = 0x7fff7fffu, y = __vmaxu2(bq[w][0] & m, bq[w][1] & m);
+                    mx = max(mx, max(y & 0xffffu, y >> 16));
+                }
                 mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
                 mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
                 f = stage_scale(mx << 16);
-            }
 #pragma unroll
-            for (int w = 0; w < D / 16; ++w) {
-                if (bf) {
-                    auto two = [&](uint32_t v) { return pack_h2(__uint_as_float(v << 16) * f, __uint_as_float(v & 0xffff0000u) * f); };
-                    bq[w][0] = two(x[w].x); bq[w][1] = two(x[w].y);
-                } else {
-                    bq[w][0] = x[w].x; bq[w][1] = x[w].y;
-                }
+                for (int w = 0; w < D / 16; ++w)
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) bq[w][i] = pack_h2(__uint_as_float(bq[w][i] << 16) * f, __uint_as_float(bq[w][i] & 0xffff0000u) * f);
             }
             const float inv = p.scale_log2 / f;
             const int first = p.total - p.Tq;
@@ -239,161 +287,145 @@ template <int D, bool E4M3> __global__ void __launch_bounds__(AW * 32, AttendPla
         auto whole = [&](int base) { return base + 15 <= c.pos_min && (base >= lo_max || base + 15 < p.sinks); };
 
         // ---- blocks
-        const int n_code = z.n_sink + z.n_win;
-        const uint8_t* kc = p.kc + lane_c * p.cap * D;
-        const uint8_t* vc = p.vc + lane_c * p.cap * D;
-        const float* ksc = p.ks + lane_c * (p.cap >> p.shift);
-        const float* vsc = p.vs + lane_c * (p.cap >> p.shift);
-        auto base_of = [&](int u) { return (u < z.n_sink ? u : z.low_unit + u - z.n_sink) * P::UNIT; };
-        auto load = [&](int u, Unit<D>& x) {
-            const int base = base_of(u);
-#pragma unroll
-            for (int i = 0; i < P::TILES; ++i) {
-                const int tok = min(base + 16 * i, p.n8 - 16);         // (a tile behind the last block: read again, not used)
-                const uint8_t* kr = kc + int64_t(tok + g) * D;
-                const uint8_t* vr = vc + int64_t(tok + 2 * t) * D;
-                ld_key_row<D>(kr, t, x.k[i][0]);
-                ld_key_row<D>(kr + 8 * D, t, x.k[i][1]);
-#pragma unroll
-                for (int r = 0; r < 4; ++r) ld_value_row<D>(vr + ((r & 1) + 8 * (r >> 1)) * D, g, x.v[i][r]);
-                x.ks[i] = ksc[tok >> p.shift];
-                x.vs[i] = vsc[tok >> p.shift];
-            }
-        };
-        auto compute = [&](int u, const Unit<D>& x) {
-            const int base = base_of(u);
-#pragma unroll
-            for (int i = 0; i < P::TILES; ++i) {
-                const int tok = base + 16 * i;
-                if (tok >= p.n8 || hidden(tok)) continue;
-                float s[4] = {0.f, 0.f, 0.f, 0.f}, s2[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 1
+        for (int u = u0 + warp; u < end; u += AW) {
+            cp_async_wait<ST - 2>();
+            __syncwarp();
+            ask();
+            const uint32_t src = ring + use * P::STAGE;
+            use = use + 1 == ST ? 0 : use + 1;
+            const int tok = base_of(u);
+            if (hidden(tok)) continue;
+            uint32_t scales[2];
+            ld_ring<8>(src + 2 * P::SIDE, scales);
+            float s[4] = {0.f, 0.f, 0.f, 0.f};
+            {
+                float s2[4] = {0.f, 0.f, 0.f, 0.f};
+                uint32_t k0[P::KW], k1[P::KW];
+                key_row<D>(src, g, t, k0);
+                key_row<D>(src, g + 8, t, k1);
 #pragma unroll
                 for (int w = 0; w < P::KW; ++w) {
                     uint32_t a[4];
-                    halves<E4M3>(x.k[i][0][w], a[0], a[2]);
-                    halves<E4M3>(x.k[i][1][w], a[1], a[3]);
+                    halves<E4M3>(k0[w], a[0], a[2]);
+                    halves<E4M3>(k1[w], a[1], a[3]);
                     mma16816((w & 1) ? s2 : s, a[0], a[1], a[2], a[3], bq[w][0], bq[w][1]);
                 }
 #pragma unroll
                 for (int k = 0; k < 4; ++k) s[k] += s2[k];
-                uint32_t bp[2];
-                if (whole(tok)) weights<D, false>(s, x.ks[i], x.ks[i], x.vs[i], x.vs[i], tok + g, c, p.window, p.sinks, st, bp);
-                else weights<D, true>(s, x.ks[i], x.ks[i], x.vs[i], x.vs[i], tok + g, c, p.window, p.sinks, st, bp);
-                // two tokens' bytes side by side are the pairs of the transposed operand: coordinates w, w + 1 and w + 2, w + 3
-#pragma unroll
-                for (int w = 0; w < P::VW; ++w) {
-                    uint32_t a[4], e[4];
-                    halves<E4M3>(__byte_perm(x.v[i][0][w], x.v[i][1][w], 0x5140), a[0], a[1]);
-                    halves<E4M3>(__byte_perm(x.v[i][2][w], x.v[i][3][w], 0x5140), a[2], a[3]);
-                    halves<E4M3>(__byte_perm(x.v[i][0][w], x.v[i][1][w], 0x7362), e[0], e[1]);
-                    halves<E4M3>(__byte_perm(x.v[i][2][w], x.v[i][3][w], 0x7362), e[2], e[3]);
-                    mma16816(st.o[2 * w], a[0], a[1], a[2], a[3], bp[0], bp[1]);
-                    mma16816(st.o[2 * w + 1], e[0], e[1], e[2], e[3], bp[0], bp[1]);
-                }
             }
-        };
-        {
-            int u = u0 + warp;
-            const int end = min(u1, n_code);
-            Unit<D> x, y;
-            if (u < end) load(u, x);
-            while (u < end) {
-                if (u + AW < end) load(u + AW, y);
-                compute(u, x);
-                u += AW;
-                if (u >= end) break;
-                if (u + AW < end) load(u + AW, x);
-                compute(u, y);
-                u += AW;
+            uint32_t v[4][P::VW];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) value_row<D>(src + P::SIDE, 2 * t + (r & 1) + 8 * (r >> 1), g, v[r]);
+            const float kn = __uint_as_float(scales[0]), vn = __uint_as_float(scales[1]);
+            uint32_t bp[2], rest[2];
+            weights<D>(s, kn, kn, vn, vn, !whole(tok), tok + g, c, p.window, p.sinks, st, bp, rest, !bf);
+            // two tokens' bytes side by side are the pairs of the transposed operand: coordinates w, w + 1 and w + 2, w + 3
+#pragma unroll
+            for (int w = 0; w < P::VW; ++w) {
+                uint32_t a[4], e[4];
+                halves<E4M3>(__byte_perm(v[0][w], v[1][w], 0x5140), a[0], a[1]);
+                halves<E4M3>(__byte_perm(v[2][w], v[3][w], 0x5140), a[2], a[3]);
+                halves<E4M3>(__byte_perm(v[0][w], v[1][w], 0x7362), e[0], e[1]);
+                halves<E4M3>(__byte_perm(v[2][w], v[3][w], 0x7362), e[2], e[3]);
+                mma16816(st.o[2 * w], a[0], a[1], a[2], a[3], bp[0], bp[1]);
+                mma16816(st.o[2 * w + 1], e[0], e[1], e[2], e[3], bp[0], bp[1]);
+                if (!bf) {
+                    mma16816(st.o[2 * w], a[0], a[1], a[2], a[3], rest[0], rest[1]);
+                    mma16816(st.o[2 * w + 1], e[0], e[1], e[2], e[3], rest[0], rest[1]);
+                }
             }
         }
+        cp_async_wait<0>();
         // ---- the tail: 16-bit rows, bfloat16 ones each under its power of two
-        for (int u = max(u0, n_code) + (warp + AW - (max(u0, n_code) - u0) % AW) % AW; u < u1; u += AW) {
+        const int t0 = max(u0, n_code);
 #pragma unroll 1
-            for (int i = 0; i < P::TILES; ++i) {
-                const int tok = p.n8 + (z.tail_unit + u - n_code) * P::UNIT + 16 * i;
-                if (tok >= p.total || hidden(tok)) continue;
-                // (rows that no query sees are not read: what they hold must not reach the sums)
-                auto row = [&](int j, bool keys) -> const char* {
-                    if (j >= p.total || (j < lo_min && j >= p.sinks)) return nullptr;
-                    if (p.kn != nullptr && j == p.total - 1)
-                        return keys ? static_cast<const char*>(p.kn) + 2 * (b * p.kn_sb + kv * p.kn_sh) : static_cast<const char*>(p.vn) + 2 * (b * p.vn_sb + kv * p.vn_sh);
-                    return static_cast<const char*>(keys ? p.kt : p.vt) + 2 * (lane_c * p.block + (j - p.n8)) * D;
-                };
-                auto mag = [](uint2 v) { const uint32_t m = 0x7fff7fffu, y = __vmaxu2(v.x & m, v.y & m); return max(y & 0xffffu, y >> 16); };
-                auto half4 = [&](uint2& v, float f) {
-                    if (!bf) return;
-                    v.x = pack_h2(__uint_as_float(v.x << 16) * f, __uint_as_float(v.x & 0xffff0000u) * f);
-                    v.y = pack_h2(__uint_as_float(v.y << 16) * f, __uint_as_float(v.y & 0xffff0000u) * f);
-                };
-                float kn[2] = {1.f, 1.f}, s[4] = {0.f, 0.f, 0.f, 0.f};
-                {
-                    uint2 x[2][P::KW];
+        for (int u = t0 + ((warp - (t0 - u0)) & (AW - 1)); u < u1; u += AW) {
+            const int tok = p.n8 + (z.tail_unit + u - n_code) * 16;
+            if (hidden(tok)) continue;
+            // (rows that no query sees are not read: what they hold must not reach the sums)
+            auto row = [&](int j, bool keys) -> const char* {
+                if (j >= p.total || (j < lo_min && j >= p.sinks)) return nullptr;
+                if (p.kn != nullptr && j == p.total - 1)
+                    return keys ? static_cast<const char*>(p.kn) + 2 * (b * p.kn_sb + kv * p.kn_sh) : static_cast<const char*>(p.vn) + 2 * (b * p.vn_sb + kv * p.vn_sh);
+                return static_cast<const char*>(keys ? p.kt : p.vt) + 2 * (lane_c * p.block + (j - p.n8)) * D;
+            };
+            auto mag = [](uint2 v) { const uint32_t m = 0x7fff7fffu, y = __vmaxu2(v.x & m, v.y & m); return max(y & 0xffffu, y >> 16); };
+            auto half4 = [&](uint2& v, float f) {
+                v.x = pack_h2(__uint_as_float(v.x << 16) * f, __uint_as_float(v.x & 0xffff0000u) * f);
+                v.y = pack_h2(__uint_as_float(v.y << 16) * f, __uint_as_float(v.y & 0xffff0000u) * f);
+            };
+            uint2 k[2][P::KW], v[4][P::VW];
 #pragma unroll
-                    for (int r = 0; r < 2; ++r) {
-                        const char* src = row(tok + g + 8 * r, true);
-                        uint32_t mx = 0;
+            for (int r = 0; r < 2; ++r) {
+                const char* src = row(tok + g + 8 * r, true);
 #pragma unroll
-                        for (int w = 0; w < P::KW; ++w) {
-                            x[r][w] = src ? *reinterpret_cast<const uint2*>(src + 2 * key_dim<D>(w, t)) : make_uint2(0u, 0u);
-                            mx = max(mx, mag(x[r][w]));
-                        }
-                        if (bf) {
-                            mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-                            mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-                            const float f = stage_scale(mx << 16);
-                            kn[r] = 1.f / f;
+                for (int w = 0; w < P::KW; ++w) k[r][w] = src ? *reinterpret_cast<const uint2*>(src + 2 * key_dim<D>(w, t)) : make_uint2(0u, 0u);
+            }
 #pragma unroll
-                            for (int w = 0; w < P::KW; ++w) half4(x[r][w], f);
-                        }
-                    }
+            for (int r = 0; r < 4; ++r) {
+                const char* src = row(tok + 2 * t + (r & 1) + 8 * (r >> 1), false);
 #pragma unroll
-                    for (int w = 0; w < P::KW; ++w) mma16816(s, x[0][w].x, x[1][w].x, x[0][w].y, x[1][w].y, bq[w][0], bq[w][1]);
-                }
-                uint2 x[4][P::VW];
-                float f[4] = {1.f, 1.f, 1.f, 1.f};
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const char* src = row(tok + 2 * t + (r & 1) + 8 * (r >> 1), false);
-                    uint32_t mx = 0;
-#pragma unroll
-                    for (int w = 0; w < P::VW; ++w) {
-                        x[r][w] = src ? *reinterpret_cast<const uint2*>(src + 2 * value_dim<D>(w, g)) : make_uint2(0u, 0u);
-                        mx = max(mx, mag(x[r][w]));
-                    }
-#pragma unroll
-                    for (int off = 4; off < 32; off <<= 1) mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, off));
-                    if (bf) {
-                        f[r] = stage_scale(mx << 16);
-#pragma unroll
-                        for (int w = 0; w < P::VW; ++w) half4(x[r][w], f[r]);
-                    }
-                    // values that are not finite would reach queries that they are hidden from as 0 * inf: zeros, and a score of NaN
-                    if (mx >= (bf ? 0x7f80u : 0x7c00u)) {
-                        f[r] = __uint_as_float(0x7fffffffu);
-#pragma unroll
-                        for (int w = 0; w < P::VW; ++w) x[r][w] = make_uint2(0u, 0u);
-                    }
-                }
-                float vn[2];                           // tokens g and g + 8 sit with the lane of t = g / 2
+                for (int w = 0; w < P::VW; ++w) v[r][w] = src ? *reinterpret_cast<const uint2*>(src + 2 * value_dim<D>(w, g)) : make_uint2(0u, 0u);
+            }
+            float kn[2] = {1.f, 1.f}, s[4] = {0.f, 0.f, 0.f, 0.f};
+            if (bf) {
 #pragma unroll
                 for (int r = 0; r < 2; ++r) {
-                    const float a = __shfl_sync(0xffffffffu, f[2 * r], g >> 1), e = __shfl_sync(0xffffffffu, f[2 * r + 1], g >> 1);
-                    vn[r] = 1.f / ((g & 1) ? e : a);
-                    if (vn[r] != vn[r]) { kn[r] = vn[r]; vn[r] = 0.f; }
-                }
-                uint32_t bp[2];
-                weights<D, true>(s, kn[0], kn[1], vn[0], vn[1], tok + g, c, p.window, p.sinks, st, bp);
+                    uint32_t mx = 0;
 #pragma unroll
-                for (int w = 0; w < P::VW; ++w) {
-                    mma16816(st.o[2 * w], __byte_perm(x[0][w].x, x[1][w].x, 0x5410), __byte_perm(x[0][w].x, x[1][w].x, 0x7632), __byte_perm(x[2][w].x, x[3][w].x, 0x5410),
-                             __byte_perm(x[2][w].x, x[3][w].x, 0x7632), bp[0], bp[1]);
-                    mma16816(st.o[2 * w + 1], __byte_perm(x[0][w].y, x[1][w].y, 0x5410), __byte_perm(x[0][w].y, x[1][w].y, 0x7632), __byte_perm(x[2][w].y, x[3][w].y, 0x5410),
-                             __byte_perm(x[2][w].y, x[3][w].y, 0x7632), bp[0], bp[1]);
+                    for (int w = 0; w < P::KW; ++w) mx = max(mx, mag(k[r][w]));
+                    mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+                    mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+                    const float f = stage_scale(mx << 16);
+                    kn[r] = 1.f / f;
+#pragma unroll
+                    for (int w = 0; w < P::KW; ++w) half4(k[r][w], f);
+                }
+            }
+#pragma unroll
+            for (int w = 0; w < P::KW; ++w) mma16816(s, k[0][w].x, k[1][w].x, k[0][w].y, k[1][w].y, bq[w][0], bq[w][1]);
+            float f[4] = {1.f, 1.f, 1.f, 1.f};
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                uint32_t mx = 0;
+#pragma unroll
+                for (int w = 0; w < P::VW; ++w) mx = max(mx, mag(v[r][w]));
+#pragma unroll
+                for (int off = 4; off < 32; off <<= 1) mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, off));
+                if (bf) {
+                    f[r] = stage_scale(mx << 16);
+#pragma unroll
+                    for (int w = 0; w < P::VW; ++w) half4(v[r][w], f[r]);
+                }
+                // values that are not finite would reach queries that they are hidden from as 0 * inf: zeros, and a score of NaN
+                if (mx >= (bf ? 0x7f80u : 0x7c00u)) {
+                    f[r] = __uint_as_float(0x7fffffffu);
+#pragma unroll
+                    for (int w = 0; w < P::VW; ++w) v[r][w] = make_uint2(0u, 0u);
+                }
+            }
+            float vn[2];                               // tokens g and g + 8 sit with the lane of t = g / 2
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+                const float a = __shfl_sync(0xffffffffu, f[2 * r], g >> 1), e = __shfl_sync(0xffffffffu, f[2 * r + 1], g >> 1);
+                vn[r] = 1.f / ((g & 1) ? e : a);
+                if (vn[r] != vn[r]) { kn[r] = vn[r]; vn[r] = 0.f; }
+            }
+            uint32_t bp[2], rest[2];
+            weights<D>(s, kn[0], kn[1], vn[0], vn[1], true, tok + g, c, p.window, p.sinks, st, bp, rest, !bf);
+#pragma unroll
+            for (int w = 0; w < P::VW; ++w) {
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const uint32_t x0 = i ? v[0][w].y : v[0][w].x, x1 = i ? v[1][w].y : v[1][w].x, x2 = i ? v[2][w].y : v[2][w].x, x3 = i ? v[3][w].y : v[3][w].x;
+                    const uint32_t a0 = __byte_perm(x0, x1, 0x5410), a1 = __byte_perm(x0, x1, 0x7632), a2 = __byte_perm(x2, x3, 0x5410), a3 = __byte_perm(x2, x3, 0x7632);
+                    mma16816(st.o[2 * w + i], a0, a1, a2, a3, bp[0], bp[1]);
+                    if (!bf) mma16816(st.o[2 * w + i], a0, a1, a2, a3, rest[0], rest[1]);
                 }
             }
         }
-        if (p.kn != nullptr && grp == 0 && u1 == z.n_units) {          // whoever has the lane's last unit stores the appended row
+        if (p.kn != nullptr && grp == 0 && u1 == z.n_units) {          // whoever has the lane's last tile stores the appended row
             for (int i = tid; i < D / 4; i += AW * 32) {
                 const int side = i >= D / 8, ch = (i - side * (D / 8)) * 8;
                 const char* src = side ? static_cast<const char*>(p.vn) + 2 * (b * p.vn_sb + kv * p.vn_sh) : static_cast<const char*>(p.kn) + 2 * (b * p.kn_sb + kv * p.kn_sh);
@@ -401,33 +433,35 @@ template <int D, bool E4M3> __global__ void __launch_bounds__(AW * 32, AttendPla
                 *reinterpret_cast<uint4*>(dst + 2 * ch) = *reinterpret_cast<const uint4*>(src + 2 * ch);
             }
         }
-        // ---- the warps' sums into one
+        // ---- the warps' sums into one, where the rings were
+        __syncthreads();
+        float* red = reinterpret_cast<float*>(smem);
         st.finish();
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
 #pragma unroll
             for (int off = 4; off < 32; off <<= 1) st.l[i] += __shfl_xor_sync(0xffffffffu, st.l[i], off);
-            float* row = red[warp][2 * t + i];
+            float* row = red + (warp * HPG + 2 * t + i) * P::RS;
 #pragma unroll
-            for (int w = 0; w < P::VW; ++w) {
-                const int d0 = value_dim<D>(w, g);
-                *reinterpret_cast<float4*>(row + d0) = make_float4(st.o[2 * w][i], st.o[2 * w][2 + i], st.o[2 * w + 1][i], st.o[2 * w + 1][2 + i]);
-            }
-            if (g == 0) { row[D] = st.m[i]; row[D + 1] = st.l[i]; }
+            for (int w = 0; w < P::VW; ++w)
+                *reinterpret_cast<float4*>(row + value_dim<D>(w, g)) = make_float4(st.o[2 * w][i], st.o[2 * w][2 + i], st.o[2 * w + 1][i], st.o[2 * w + 1][2 + i]);
+            if (g == 0) *reinterpret_cast<float2*>(row + D) = make_float2(st.m[i], st.l[i]);
         }
         __syncthreads();
         const bool alone = u0 == 0 && u1 == z.n_units;
-        const int slot = int(blockIdx.x - job * z.n_units / z.per);
+        const uint32_t slot = blockIdx.x - job * uint32_t(z.n_units) / z.per;
         for (int i = tid; i < rows * (D / 4); i += AW * 32) {
             const int r = i / (D / 4), d0 = (i - r * (D / 4)) * 4;
+            const float* row = red + r * P::RS;
             float top = -1e30f, l = 0.f, x[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int w = 0; w < AW; ++w) top = fmaxf(top, red[w][r][D]);
+            for (int w = 0; w < AW; ++w) top = fmaxf(top, row[w * HPG * P::RS + D]);
 #pragma unroll
             for (int w = 0; w < AW; ++w) {
-                const float a = ex2(red[w][r][D] - top);
-                const float4 v = *reinterpret_cast<const float4*>(&red[w][r][d0]);
-                l += a * red[w][r][D + 1];
+                const float2 ml = *reinterpret_cast<const float2*>(row + w * HPG * P::RS + D);
+                const float a = ex2(ml.x - top);
+                const float4 v = *reinterpret_cast<const float4*>(row + w * HPG * P::RS + d0);
+                l += a * ml.y;
                 x[0] += a * v.x; x[1] += a * v.y; x[2] += a * v.z; x[3] += a * v.w;
             }
             if (alone) {
@@ -436,7 +470,7 @@ template <int D, bool E4M3> __global__ void __launch_bounds__(AW * 32, AttendPla
                 char* dst = static_cast<char*>(p.out) + 2 * (((int64_t(b) * p.Hq + h) * p.Tq + ti) * D + d0);
                 *reinterpret_cast<uint2*>(dst) = bf ? make_uint2(pack_bf2(x[0] * il, x[1] * il), pack_bf2(x[2] * il, x[3] * il)) : make_uint2(pack_h2(x[0] * il, x[1] * il), pack_h2(x[2] * il, x[3] * il));
             } else {
-                float* part = p.part + ((job * z.slots + slot) * HPG + r) * P::RS;
+                float* part = p.part + ((int64_t(job) * z.slots + slot) * HPG + r) * P::RS;
                 *reinterpret_cast<float4*>(part + d0) = make_float4(x[0], x[1], x[2], x[3]);
                 if (d0 == 0) *reinterpret_cast<float2*>(part + D) = make_float2(top, l);
             }
@@ -445,59 +479,90 @@ template <int D, bool E4M3> __global__ void __launch_bounds__(AW * 32, AttendPla
     }
 }
 
-// A warp per query row that more than one CTA worked on
-template <int D> __global__ void __launch_bounds__(128) blocks_merge_kernel(const __grid_constant__ BlockAttendParams p, const __grid_constant__ AttendGrid z) {
+// A CTA per query row that more than one CTA worked on: a thread has four coordinates and every n-th partial, so that all loads are under way at once
+constexpr int MG_T = 128;
+template <int D> __global__ void __launch_bounds__(MG_T) blocks_merge_kernel(const __grid_constant__ BlockAttendParams p, const __grid_constant__ AttendGrid z) {
     using P = AttendPlan<D>;
-    constexpr int NV = D / 32;
-    const int lane = threadIdx.x & 31;
-    const int64_t row = int64_t(blockIdx.x) * 4 + (threadIdx.x >> 5), job = row / HPG, lane_c = job / z.groups;
-    const int grp = int(job - lane_c * z.groups), rr = grp * HPG + int(row % HPG);
-    pdl_wait();
-    if (job >= z.jobs || rr >= p.Tq * p.G) return;
-    const int64_t c0 = job * z.n_units / z.per, c1 = ((job + 1) * z.n_units - 1) / z.per;
+    constexpr int Q = D / 4, N = MG_T / Q;             // threads of a partial row; partials at a time
+    __shared__ float4 sx[N][Q];
+    __shared__ float2 sm[N];
+    const uint32_t job = blockIdx.x / HPG, lane_u = job / uint32_t(z.groups);
+    const int r = blockIdx.x % HPG, grp = int(job - lane_u * uint32_t(z.groups)), rr = grp * HPG + r;
+    const int set = threadIdx.x / Q, d0 = threadIdx.x - set * Q;
+    if (rr >= p.Tq * p.G) return;
+    const uint32_t c0 = job * uint32_t(z.n_units) / z.per, c1 = ((job + 1) * uint32_t(z.n_units) - 1) / z.per;
     if (c0 == c1) return;
     const int n = int(c1 - c0) + 1;
-    const float* part = p.part + (job * z.slots * HPG + row % HPG) * P::RS;
+    const float* part = p.part + (int64_t(job) * z.slots * HPG + r) * P::RS;
     constexpr int STEP = HPG * P::RS;
-    float top = -1e30f, l = 0.f, x[NV];
-    for (int s = lane; s < n; s += 32) top = fmaxf(top, part[int64_t(s) * STEP + D]);
+    pdl_wait();
+    float m = -1e30f, l = 0.f;
+    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (set < N) {
+        for (int s = set; s < n; s += 8 * N) {
+            float2 ml[8];
+            float4 v[8];
 #pragma unroll
-    for (int off = 16; off; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+            for (int i = 0; i < 8; ++i) {
+                const float* q = part + int64_t(s + i * N < n ? s + i * N : s) * STEP;
+                ml[i] = *reinterpret_cast<const float2*>(q + D);
+                v[i] = *reinterpret_cast<const float4*>(q + 4 * d0);
+                if (s + i * N >= n) { ml[i] = make_float2(-1e30f, 0.f); v[i] = make_float4(0.f, 0.f, 0.f, 0.f); }
+            }
+            float top = m;
 #pragma unroll
-    for (int i = 0; i < NV; ++i) x[i] = 0.f;
-#pragma unroll 4
-    for (int s = 0; s < n; ++s) {
-        const float* q = part + int64_t(s) * STEP;
-        const float2 ml = *reinterpret_cast<const float2*>(q + D);
-        const float a = ex2(ml.x - top);
-        l += a * ml.y;
+            for (int i = 0; i < 8; ++i) top = fmaxf(top, ml[i].x);
+            const float a0 = ex2(m - top);
+            l *= a0; x.x *= a0; x.y *= a0; x.z *= a0; x.w *= a0;
+            m = top;
 #pragma unroll
-        for (int i = 0; i < NV; ++i) x[i] += a * q[i * 32 + lane];
+            for (int i = 0; i < 8; ++i) {
+                const float a = ex2(ml[i].x - top);
+                l += a * ml[i].y;
+                x.x += a * v[i].x; x.y += a * v[i].y; x.z += a * v[i].z; x.w += a * v[i].w;
+            }
+        }
+        sx[set][d0] = x;
+        if (d0 == 0) sm[set] = make_float2(m, l);
     }
-    const int b = int(lane_c / p.Hkv), kv = int(lane_c - int64_t(b) * p.Hkv), ti = rr / p.G, h = kv * p.G + rr - ti * p.G;
-    const int64_t out = ((int64_t(b) * p.Hq + h) * p.Tq + ti) * D + lane;
-    const float il = 1.f / l;
+    __syncthreads();
+    if (threadIdx.x >= Q) return;
+    float top = -1e30f;
 #pragma unroll
-    for (int i = 0; i < NV; ++i) store_from_f32(p.out, p.dtype, out + i * 32, x[i] * il);
+    for (int i = 0; i < N; ++i) top = fmaxf(top, sm[i].x);
+    l = 0.f;
+    x = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const float a = ex2(sm[i].x - top);
+        const float4 v = sx[i][d0];
+        l += a * sm[i].y;
+        x.x += a * v.x; x.y += a * v.y; x.z += a * v.z; x.w += a * v.w;
+    }
+    const int b = int(lane_u / uint32_t(p.Hkv)), kv = int(lane_u) - b * p.Hkv, ti = rr / p.G, h = kv * p.G + rr - ti * p.G;
+    const float il = 1.f / l;
+    char* dst = static_cast<char*>(p.out) + 2 * (((int64_t(b) * p.Hq + h) * p.Tq + ti) * D + 4 * d0);
+    *reinterpret_cast<uint2*>(dst) = p.dtype == TQ_BF16 ? make_uint2(pack_bf2(x.x * il, x.y * il), pack_bf2(x.z * il, x.w * il)) : make_uint2(pack_h2(x.x * il, x.y * il), pack_h2(x.z * il, x.w * il));
 }
 
 template <int D> AttendGrid grid_of(const BlockAttendParams& p) {
     using P = AttendPlan<D>;
     const Visible v = visible_of(p.total, p.Tq, p.window, p.sinks);
     AttendGrid z{};
-    const int code_units = (p.n8 + P::UNIT - 1) / P::UNIT;
-    z.low_unit = std::min(v.low, p.n8) / P::UNIT;
+    const int code_units = p.n8 / 16;
+    z.low_unit = std::min(v.low, p.n8) / 16;
     z.n_win = v.low >= p.n8 ? 0 : code_units - z.low_unit;
-    z.n_sink = (std::min(v.sinks, p.n8) + P::UNIT - 1) / P::UNIT;
+    z.n_sink = (std::min(v.sinks, p.n8) + 15) / 16;
     if (z.n_win > 0) z.n_sink = std::min(z.n_sink, z.low_unit);
-    z.tail_unit = v.sinks > p.n8 ? 0 : std::max(v.low - p.n8, 0) / P::UNIT;
-    z.n_units = z.n_sink + z.n_win + (p.total - p.n8 + P::UNIT - 1) / P::UNIT - z.tail_unit;
+    z.tail_unit = v.sinks > p.n8 ? 0 : std::max(v.low - p.n8, 0) / 16;
+    z.n_units = z.n_sink + z.n_win + (p.total - p.n8 + 15) / 16 - z.tail_unit;
     z.groups = int((int64_t(p.Tq) * p.G + HPG - 1) / HPG);
-    z.jobs = int64_t(p.B) * p.Hkv * z.groups;
-    const int64_t units = z.jobs * z.n_units, ctas = int64_t(blocks_sm_count()) * P::PER_SM;
-    z.per = std::max<int64_t>(AW, (units + ctas - 1) / ctas);
-    z.merge = z.per % z.n_units != 0;                  // (otherwise every row has one CTA)
-    z.slots = int(std::min<int64_t>((z.n_units - 2) / z.per + 2, z.n_units));
+    const int64_t jobs = int64_t(p.B) * p.Hkv * z.groups, units = jobs * z.n_units, ctas = int64_t(blocks_sm_count()) * P::PER_SM;
+    if (units >= (int64_t(1) << 31) || jobs >= (int64_t(1) << 28)) { z.jobs = 0; return z; }
+    z.jobs = uint32_t(jobs);
+    z.per = uint32_t(std::max<int64_t>(AW, (units + ctas - 1) / ctas));
+    z.merge = z.per % uint32_t(z.n_units) != 0;        // (otherwise every row has one CTA)
+    z.slots = std::min((z.n_units - 2) / int(z.per) + 2, z.n_units);
     return z;
 }
 template <int D> size_t split_workspace(const BlockAttendParams& p) {
@@ -509,14 +574,23 @@ template <int D> size_t split_workspace(const BlockAttendParams& p) {
 template <int D> int launch_split(const BlockAttendParams& p, cudaStream_t s) {
     using P = AttendPlan<D>;
     const AttendGrid z = grid_of<D>(p);
-    const int64_t blocks = (z.jobs * z.n_units + z.per - 1) / z.per, merge = (z.jobs * HPG + 3) / 4;
-    if (blocks >= (int64_t(1) << 31) || merge >= (int64_t(1) << 31)) return fail(TQ_ERR_UNSUPPORTED, "tq_blocks_attend: too many query rows");
+    if (z.jobs == 0) return fail(TQ_ERR_UNSUPPORTED, "tq_blocks_attend: too many query rows");
+    static std::atomic<bool> set[64];
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess) dev = -1;
+    if (dev < 0 || dev >= 64 || !set[dev].load()) {
+        cudaError_t e = cudaFuncSetAttribute(blocks_attend_kernel<D, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, int(P::SMEM));
+        if (e == cudaSuccess) e = cudaFuncSetAttribute(blocks_attend_kernel<D, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, int(P::SMEM));
+        if (e != cudaSuccess) return fail(TQ_ERR_LAUNCH, "tq_blocks_attend: shared memory %zu B: %s", P::SMEM, cudaGetErrorString(e));
+        if (dev >= 0 && dev < 64) set[dev].store(true);
+    }
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(unsigned(blocks));
+    cfg.gridDim = dim3((z.jobs * uint32_t(z.n_units) + z.per - 1) / z.per);
     cfg.blockDim = dim3(AW * 32);
+    cfg.dynamicSmemBytes = P::SMEM;
     cfg.stream = s;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
@@ -524,8 +598,9 @@ template <int D> int launch_split(const BlockAttendParams& p, cudaStream_t s) {
     else cudaLaunchKernelEx(&cfg, blocks_attend_kernel<D, false>, p, z);
     if (int rc = check_launch("tq_blocks_attend")) return rc;
     if (!z.merge) return TQ_OK;
-    cfg.gridDim = dim3(unsigned(merge));
-    cfg.blockDim = dim3(128);
+    cfg.gridDim = dim3(z.jobs * HPG);
+    cfg.blockDim = dim3(MG_T);
+    cfg.dynamicSmemBytes = 0;
     cudaLaunchKernelEx(&cfg, blocks_merge_kernel<D>, p, z);
     return check_launch("tq_blocks_attend");
 }
