@@ -68,12 +68,6 @@ template <typename E> __device__ __forceinline__ Eight8<E> load8(const E* p) { r
 template <typename E> __device__ __forceinline__ void store8(E* p, const Eight8<E>& v) { *reinterpret_cast<Eight8<E>*>(p) = v; }
 template <typename E> __device__ __forceinline__ float at8(const Eight8<E>& v, int i) { return to_f32<E>(reinterpret_cast<const E*>(&v)[i]); }
 
-__device__ __forceinline__ uint32_t e4m3x2_of(float lo, float hi) {
-    uint16_t r;
-    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
-    return r;
-}
-
 constexpr int WR_U = 4;                      // vectors of eight values per thread: a CTA has block * d / 32 threads (32 to 1024)
 
 // One CTA per (lane, keys or values, block).  The CTA of the first block is the only one that reads the tail, and the one that leaves the rest there

@@ -47,6 +47,11 @@ inline __host__ __device__ Visible visible_of(int total, int t_q, int window, in
     return Visible{low, sinks < low ? sinks : low};
 }
 
+__device__ __forceinline__ uint32_t e4m3x2_of(float lo, float hi) {
+    uint16_t r;
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
+    return r;
+}
 __device__ __forceinline__ float e4m3_to_f32(uint8_t c) {
     uint32_t h;
     asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"(uint16_t(c)));

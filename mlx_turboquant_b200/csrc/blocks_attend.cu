@@ -2,14 +2,18 @@
 //
 //   out = sum_j softmax_j(scale q.k_j) v_j,   k_j = kc_j ks, v_j = vc_j vs with one ks, vs for each block of tokens, tokens of the tail as they are
 //
-// The integers are exact as fp16, and so are the 8-bit floats: scores are products of codes with the query as it came (a bfloat16 one under a
-// power of two), the scales follow in float32, the values' scale on the softmax weights.  Only those are rounded, to fp16.
-//
 // blocks_attend_kernel: bound by the codes' bytes.  Work is a flat sequence of tiles (16 tokens) of all (lane, group of 8 query rows); a CTA of eight warps
 // takes an equal run of it, whatever lanes that touches, a warp every eighth tile of a lane.  Codes go through a ring of each warp's own in shared memory
-// (cp.async, 16 bytes a lane); mma.sync m16n8k16 with the tokens as M (scores) and the coordinates as M (values), so that eight query rows share every
-// converted code.  Which coordinate a fragment's row or column stands for is free as long as queries and results agree: a lane's 16 bytes are four
-// fragments.  (The products are tiny, N = 8: tcgen05 would want 64 rows of operands staged in shared memory as fp16.)
+// (cp.async, 16 bytes a lane).  mma.sync with the tokens as M (scores) and the coordinates as M (values): eight query rows share every code.  (The products
+// are tiny, N = 8: tcgen05 would want 64 rows of operands staged in shared memory.)  Which coordinate a fragment's row or column stands for is free as long
+// as queries and results agree.
+//   scores, int8: integer products m16n8k32 on the codes as they are; the query in fixed point, 15 bits of its largest element for bfloat16 tokens, 22 for
+//     fp16 ones, in digits of 7 bits; the sums are exact.  (As fp16 operands the key codes cost 80 of 476 instructions per tile of 16 tokens at d = 128; the
+//     card runs this kernel at its power limit, so that instructions count beside bytes.)
+//   scores, e4m3: fp16 operands (codes are exact in them, and queries, bfloat16 ones under a power of two).  (mma.sync on e4m3 operands costs more than the
+//     conversions here: 404 instructions per tile against 376.)
+//   values: fp16, exact for both kinds of codes, times the softmax weights under their block's scale as fp16 - for fp16 tokens with a second part: the
+//     weights' rounding would be as large as the result's own.  (8-bit weights would lose the sum of many small ones.)
 // blocks_merge_kernel: joins the partials of a row that several CTAs worked on, in their order: results do not depend on which one came first.
 // blocks_plain_kernel: a warp per token on CUDA cores, float32 throughout: float32 tokens, head dims without a layout above.
 #include <algorithm>
@@ -151,11 +155,11 @@ struct Cols {
     int pos_min, pos_max;                              // of the group
 };
 
-// Scores of 16 tokens (rows g, g + 8) times their scales -> running softmax -> the weights as the value products' operand, as fp16 and what that leaves
-// (fp16 results: the weights' rounding, 2^-12 on average, would be as large as the result's own).  tok: token of row g.
-template <int D>
+// Scores of 16 tokens (rows g, g + 8) times their scales -> running softmax -> the weights as the value products' operand, as fp16 and (FINE) what that
+// leaves.  tok: token of row g.
+template <int D, bool FINE>
 __device__ __forceinline__ void weights(float (&s)[4], float kn0, float kn1, float vn0, float vn1, bool masked, int tok, const Cols& c, int window, int sinks, WarpAcc<D, 0>& st,
-                                        uint32_t (&bp)[2], uint32_t (&rest)[2], bool fine) {
+                                        uint32_t (&bp)[2], uint32_t (&rest)[2]) {
     s[0] *= kn0 * c.scale[0]; s[1] *= kn0 * c.scale[1];
     s[2] *= kn1 * c.scale[0]; s[3] *= kn1 * c.scale[1];
     bool hide[4] = {false, false, false, false};
@@ -185,20 +189,41 @@ __device__ __forceinline__ void weights(float (&s)[4], float kn0, float kn1, flo
     for (int i = 0; i < 2; ++i) {
         const __half2 h = __floats2half2_rn(x[2 * i], x[2 * i + 1]);
         bp[i] = movm_t(*reinterpret_cast<const uint32_t*>(&h));
-        if (fine) {
+        if (FINE) {
             const float2 hf = __half22float2(h);
             rest[i] = movm_t(pack_h2(x[2 * i] - hf.x, x[2 * i + 1] - hf.y));
         }
     }
 }
 
-template <int D, bool E4M3> __global__ void __launch_bounds__(AW * 32, AttendPlan<D>::PER_SM) blocks_attend_kernel(const __grid_constant__ BlockAttendParams p, const __grid_constant__ AttendGrid z) {
+// Integer products, 16 tokens x 8 queries x 32 coordinates
+__device__ __forceinline__ void mma_codes(int (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// A query's four coordinates in N digits of 7 bits, the largest first: a word of four for each
+template <int N> __device__ __forceinline__ void digits_of(const float (&x)[4], uint32_t (&w)[N]) {
+#pragma unroll
+    for (int n = 0; n < N; ++n) w[n] = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        int r = __float2int_rn(x[i]);
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+            const int sh = 7 * (N - 1 - n), d = sh ? (r + (1 << (sh - 1))) >> sh : r;
+            r -= d << sh;
+            w[n] |= uint32_t(d & 255) << (8 * i);
+        }
+    }
+}
+
+template <int D, bool E4M3, bool FINE> __global__ void __launch_bounds__(AW * 32, AttendPlan<D>::PER_SM) blocks_attend_kernel(const __grid_constant__ BlockAttendParams p, const __grid_constant__ AttendGrid z) {
     using P = AttendPlan<D>;
-    constexpr int ST = P::ST;
+    constexpr int ST = P::ST, N = FINE && !E4M3 ? 3 : 2;       // words of a query's four coordinates: digits, or fp16 pairs
+    constexpr bool bf = !FINE;
     extern __shared__ __align__(16) unsigned char smem[];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
     const uint32_t u_first = blockIdx.x * z.per, u_last = min(u_first + z.per, z.jobs * uint32_t(z.n_units));
-    const bool bf = p.dtype == TQ_BF16;
     const uint32_t ring = static_cast<uint32_t>(__cvta_generic_to_shared(smem)) + uint32_t(warp) * ST * P::STAGE;
     const int n_code = z.n_sink + z.n_win;
     pdl_wait();
@@ -212,62 +237,81 @@ template <int D, bool E4M3> __global__ void __launch_bounds__(AW * 32, AttendPla
         const int64_t lane_c = lane_u;
 
         // ---- this warp's tiles of codes are asked for first
-        const uint8_t* kc = p.kc + lane_c * p.cap * D;
-        const uint8_t* vc = p.vc + lane_c * p.cap * D;
+        const uint8_t* kc = p.kc + lane_c * p.cap * D + lane * 16;
+        const uint8_t* vc = p.vc + lane_c * p.cap * D + lane * 16;
         const float* sc = (lane ? p.vs : p.ks) + lane_c * (p.cap >> p.shift);
-        auto base_of = [&](int u) { return (u < z.n_sink ? u : z.low_unit + u - z.n_sink) * 16; };
+        const int jump = (z.low_unit - z.n_sink) * 16;
+        auto base_of = [&](int u) { return u * 16 + (u < z.n_sink ? 0 : jump); };
         const int end = min(u1, n_code);
-        int next = u0 + warp, fill = 0, use = 0;       // the next tile to be asked for; ring places
+        int next = u0 + warp;                          // the next tile to be asked for
+        uint32_t fill = ring, use = ring;              // its place in the ring; the place of the tile at hand
         auto ask = [&]() {
             if (next < end) {
                 const int base = base_of(next);
                 const uint8_t* ks = kc + int64_t(base) * D;
                 const uint8_t* vs = vc + int64_t(base) * D;
-                const uint32_t dst = ring + fill * P::STAGE;
 #pragma unroll
                 for (int i = 0; i < (16 * P::CPR + 31) / 32; ++i) {
+                    // (rows are 16 pieces or fewer: a lane's i-th piece is 32 / CPR rows further down)
                     const int x = lane + 32 * i, r = x / P::CPR;
-                    const uint32_t pl = place<D>(r, x - r * P::CPR) * 16;
-                    cp_async16(dst + pl, ks + x * 16, 16);
-                    cp_async16(dst + P::SIDE + pl, vs + x * 16, 16);
+                    const uint32_t dst = fill + place<D>(r, x - r * P::CPR) * 16;
+                    cp_async16(dst, ks + 512 * i, 16);
+                    cp_async16(dst + P::SIDE, vs + 512 * i, 16);
                 }
-                if (lane < 2) asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst + 2 * P::SIDE + 4 * lane), "l"(sc + (base >> p.shift)) : "memory");
+                if (lane < 2) asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(fill + 2 * P::SIDE + 4 * lane), "l"(sc + (base >> p.shift)) : "memory");
             }
             cp_async_commit();
             next += AW;
-            fill = fill + 1 == ST ? 0 : fill + 1;
+            fill = fill == ring + (ST - 1) * P::STAGE ? ring : fill + P::STAGE;
         };
 #pragma unroll
         for (int i = 0; i < ST - 1; ++i) ask();
 
-        // ---- the group's queries as B operands (row g's coordinates in the order of the key codes), bfloat16 under a power of two
+        // ---- the group's queries as B operands (row g's coordinates in the order of the key codes)
         const int rows = min(HPG, p.Tq * p.G - grp * HPG), r0 = grp * HPG;
         Cols c;
-        uint32_t bq[D / 16][2];
-        {
-            const bool has = g < rows;
+        uint32_t bq[N][P::KW];
+        auto query = [&](int w) -> uint2 {             // coordinates key_dim(w, t) ... + 3 of row g
             const int r = r0 + g, ti = r / p.G, h = kv * p.G + r - ti * p.G;
-            const char* q = static_cast<const char*>(p.q) + 2 * (b * p.q_sb + h * p.q_sh + ti * p.q_st);
+            if (g >= rows) return make_uint2(0u, 0u);
+            return *reinterpret_cast<const uint2*>(static_cast<const char*>(p.q) + 2 * (b * p.q_sb + h * p.q_sh + ti * p.q_st + key_dim<D>(w, t)));
+        };
+        auto f4 = [&](uint2 v, float (&x)[4], float f) {
+            if (bf) {
+                x[0] = __uint_as_float(v.x << 16) * f; x[1] = __uint_as_float(v.x & 0xffff0000u) * f; x[2] = __uint_as_float(v.y << 16) * f; x[3] = __uint_as_float(v.y & 0xffff0000u) * f;
+            } else {
+                const float2 lo = __half22float2(*reinterpret_cast<const __half2*>(&v.x)), hi = __half22float2(*reinterpret_cast<const __half2*>(&v.y));
+                x[0] = lo.x * f; x[1] = lo.y * f; x[2] = hi.x * f; x[3] = hi.y * f;
+            }
+        };
+        auto mag = [](uint2 v) { const uint32_t m = 0x7fff7fffu, y = __vmaxu2(v.x & m, v.y & m); return max(y & 0xffffu, y >> 16); };
+        float q_max;
+        {
+            uint2 x[P::KW];
             uint32_t mx = 0;
 #pragma unroll
-            for (int w = 0; w < D / 16; ++w) {
-                const uint2 x = has ? *reinterpret_cast<const uint2*>(q + 2 * key_dim<D>(w, t)) : make_uint2(0u, 0u);
-                bq[w][0] = x.x; bq[w][1] = x.y;
-            }
-            float f = 1.f;
-            if (bf) {
+            for (int w = 0; w < P::KW; ++w) x[w] = query(w);
 #pragma unroll
-                for (int w = 0; w < D / 16; ++w) {
-                    const uint32_t m = 0x7fff7fffu, y = __vmaxu2(bq[w][0] & m, bq[w][1] & m);
-                    mx = max(mx, max(y & 0xffffu, y >> 16));
+            for (int w = 0; w < P::KW; ++w) mx = max(mx, mag(x[w]));
+            mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+            mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+            q_max = bf ? __uint_as_float(mx << 16) : __half2float(__ushort_as_half(uint16_t(mx)));
+            // e4m3: bfloat16 queries under the power of two that takes the largest element to [2^7, 2^8); int8: the largest element in N digits of 7 bits
+            float f = E4M3 ? (bf ? stage_scale(__float_as_uint(q_max)) : 1.f) : q_max > 0.f ? fminf((FINE ? 2080000.f : 16250.f) / q_max, 3.4028235e38f) : 1.f;
+            if (!E4M3 && !(q_max <= 3.4028235e38f)) f = __uint_as_float(0x7fffffffu);       // (integers know no NaN: the scale is one)
+#pragma unroll
+            for (int w = 0; w < P::KW; ++w) {
+                float y[4];
+                uint32_t part[N];
+                f4(x[w], y, f);
+                if constexpr (E4M3) {
+                    part[0] = bf ? pack_h2(y[0], y[1]) : x[w].x;
+                    part[1] = bf ? pack_h2(y[2], y[3]) : x[w].y;
+                } else {
+                    digits_of<N>(y, part);
                 }
-                mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-                mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-                f = stage_scale(mx << 16);
 #pragma unroll
-                for (int w = 0; w < D / 16; ++w)
-#pragma unroll
-                    for (int i = 0; i < 2; ++i) bq[w][i] = pack_h2(__uint_as_float(bq[w][i] << 16) * f, __uint_as_float(bq[w][i] & 0xffff0000u) * f);
+                for (int n = 0; n < N; ++n) bq[n][w] = part[n];
             }
             const float inv = p.scale_log2 / f;
             const int first = p.total - p.Tq;
@@ -292,34 +336,47 @@ template <int D, bool E4M3> __global__ void __launch_bounds__(AW * 32, AttendPla
             cp_async_wait<ST - 2>();
             __syncwarp();
             ask();
-            const uint32_t src = ring + use * P::STAGE;
-            use = use + 1 == ST ? 0 : use + 1;
+            const uint32_t src = use;
+            use = use == ring + (ST - 1) * P::STAGE ? ring : use + P::STAGE;
             const int tok = base_of(u);
             if (hidden(tok)) continue;
             uint32_t scales[2];
             ld_ring<8>(src + 2 * P::SIDE, scales);
-            float s[4] = {0.f, 0.f, 0.f, 0.f};
+            float s[4];
             {
-                float s2[4] = {0.f, 0.f, 0.f, 0.f};
                 uint32_t k0[P::KW], k1[P::KW];
                 key_row<D>(src, g, t, k0);
                 key_row<D>(src, g + 8, t, k1);
+                if constexpr (E4M3) {
+                    float s2[4] = {0.f, 0.f, 0.f, 0.f};
+                    s[0] = s[1] = s[2] = s[3] = 0.f;
 #pragma unroll
-                for (int w = 0; w < P::KW; ++w) {
-                    uint32_t a[4];
-                    halves<E4M3>(k0[w], a[0], a[2]);
-                    halves<E4M3>(k1[w], a[1], a[3]);
-                    mma16816((w & 1) ? s2 : s, a[0], a[1], a[2], a[3], bq[w][0], bq[w][1]);
+                    for (int w = 0; w < P::KW; ++w) {
+                        uint32_t a[4];
+                        halves<true>(k0[w], a[0], a[2]);
+                        halves<true>(k1[w], a[1], a[3]);
+                        mma16816((w & 1) ? s2 : s, a[0], a[1], a[2], a[3], bq[0][w], bq[1][w]);
+                    }
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) s[k] += s2[k];
+                } else {
+                    int acc[N][4];
+#pragma unroll
+                    for (int n = 0; n < N; ++n) {
+                        acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0;
+#pragma unroll
+                        for (int w = 0; w < P::KW; w += 2) mma_codes(acc[n], k0[w], k1[w], k0[w + 1], k1[w + 1], bq[n][w], bq[n][w + 1]);
+                    }
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) s[k] = N == 3 ? float(acc[0][k]) * 16384.f + float(acc[1][k] * 128 + acc[N - 1][k]) : float(acc[0][k] * 128 + acc[1][k]);
                 }
-#pragma unroll
-                for (int k = 0; k < 4; ++k) s[k] += s2[k];
             }
+            const float kn = __uint_as_float(scales[0]), vn = __uint_as_float(scales[1]);
+            uint32_t bp[2], rest[2];
+            weights<D, FINE>(s, kn, kn, vn, vn, !whole(tok), tok + g, c, p.window, p.sinks, st, bp, rest);
             uint32_t v[4][P::VW];
 #pragma unroll
             for (int r = 0; r < 4; ++r) value_row<D>(src + P::SIDE, 2 * t + (r & 1) + 8 * (r >> 1), g, v[r]);
-            const float kn = __uint_as_float(scales[0]), vn = __uint_as_float(scales[1]);
-            uint32_t bp[2], rest[2];
-            weights<D>(s, kn, kn, vn, vn, !whole(tok), tok + g, c, p.window, p.sinks, st, bp, rest, !bf);
             // two tokens' bytes side by side are the pairs of the transposed operand: coordinates w, w + 1 and w + 2, w + 3
 #pragma unroll
             for (int w = 0; w < P::VW; ++w) {
@@ -330,7 +387,7 @@ template <int D, bool E4M3> __global__ void __launch_bounds__(AW * 32, AttendPla
                 halves<E4M3>(__byte_perm(v[2][w], v[3][w], 0x7362), e[2], e[3]);
                 mma16816(st.o[2 * w], a[0], a[1], a[2], a[3], bp[0], bp[1]);
                 mma16816(st.o[2 * w + 1], e[0], e[1], e[2], e[3], bp[0], bp[1]);
-                if (!bf) {
+                if (FINE) {
                     mma16816(st.o[2 * w], a[0], a[1], a[2], a[3], rest[0], rest[1]);
                     mma16816(st.o[2 * w + 1], e[0], e[1], e[2], e[3], rest[0], rest[1]);
                 }
@@ -350,7 +407,6 @@ template <int D, bool E4M3> __global__ void __launch_bounds__(AW * 32, AttendPla
                     return keys ? static_cast<const char*>(p.kn) + 2 * (b * p.kn_sb + kv * p.kn_sh) : static_cast<const char*>(p.vn) + 2 * (b * p.vn_sb + kv * p.vn_sh);
                 return static_cast<const char*>(keys ? p.kt : p.vt) + 2 * (lane_c * p.block + (j - p.n8)) * D;
             };
-            auto mag = [](uint2 v) { const uint32_t m = 0x7fff7fffu, y = __vmaxu2(v.x & m, v.y & m); return max(y & 0xffffu, y >> 16); };
             auto half4 = [&](uint2& v, float f) {
                 v.x = pack_h2(__uint_as_float(v.x << 16) * f, __uint_as_float(v.x & 0xffff0000u) * f);
                 v.y = pack_h2(__uint_as_float(v.y << 16) * f, __uint_as_float(v.y & 0xffff0000u) * f);
@@ -369,6 +425,7 @@ template <int D, bool E4M3> __global__ void __launch_bounds__(AW * 32, AttendPla
                 for (int w = 0; w < P::VW; ++w) v[r][w] = src ? *reinterpret_cast<const uint2*>(src + 2 * value_dim<D>(w, g)) : make_uint2(0u, 0u);
             }
             float kn[2] = {1.f, 1.f}, s[4] = {0.f, 0.f, 0.f, 0.f};
+            Cols ct = c;
             if (bf) {
 #pragma unroll
                 for (int r = 0; r < 2; ++r) {
@@ -383,8 +440,18 @@ template <int D, bool E4M3> __global__ void __launch_bounds__(AW * 32, AttendPla
                     for (int w = 0; w < P::KW; ++w) half4(k[r][w], f);
                 }
             }
+            {
+                // the queries as fp16, bfloat16 ones under a power of two; c.scale is for the parts' scale
+                const float qf = bf ? stage_scale(__float_as_uint(q_max)) : 1.f, inv = p.scale_log2 / qf;
 #pragma unroll
-            for (int w = 0; w < P::KW; ++w) mma16816(s, k[0][w].x, k[1][w].x, k[0][w].y, k[1][w].y, bq[w][0], bq[w][1]);
+                for (int w = 0; w < P::KW; ++w) {
+                    uint2 x = query(w);
+                    if (bf) half4(x, qf);
+                    mma16816(s, k[0][w].x, k[1][w].x, k[0][w].y, k[1][w].y, x.x, x.y);
+                }
+#pragma unroll
+                for (int i = 0; i < 2; ++i) ct.scale[i] = __shfl_sync(0xffffffffu, inv, 4 * (2 * t + i));
+            }
             float f[4] = {1.f, 1.f, 1.f, 1.f};
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
@@ -413,7 +480,7 @@ template <int D, bool E4M3> __global__ void __launch_bounds__(AW * 32, AttendPla
                 if (vn[r] != vn[r]) { kn[r] = vn[r]; vn[r] = 0.f; }
             }
             uint32_t bp[2], rest[2];
-            weights<D>(s, kn[0], kn[1], vn[0], vn[1], true, tok + g, c, p.window, p.sinks, st, bp, rest, !bf);
+            weights<D, FINE>(s, kn[0], kn[1], vn[0], vn[1], true, tok + g, ct, p.window, p.sinks, st, bp, rest);
 #pragma unroll
             for (int w = 0; w < P::VW; ++w) {
 #pragma unroll
@@ -421,7 +488,7 @@ template <int D, bool E4M3> __global__ void __launch_bounds__(AW * 32, AttendPla
                     const uint32_t x0 = i ? v[0][w].y : v[0][w].x, x1 = i ? v[1][w].y : v[1][w].x, x2 = i ? v[2][w].y : v[2][w].x, x3 = i ? v[3][w].y : v[3][w].x;
                     const uint32_t a0 = __byte_perm(x0, x1, 0x5410), a1 = __byte_perm(x0, x1, 0x7632), a2 = __byte_perm(x2, x3, 0x5410), a3 = __byte_perm(x2, x3, 0x7632);
                     mma16816(st.o[2 * w + i], a0, a1, a2, a3, bp[0], bp[1]);
-                    if (!bf) mma16816(st.o[2 * w + i], a0, a1, a2, a3, rest[0], rest[1]);
+                    if (FINE) mma16816(st.o[2 * w + i], a0, a1, a2, a3, rest[0], rest[1]);
                 }
             }
         }
@@ -579,8 +646,9 @@ template <int D> int launch_split(const BlockAttendParams& p, cudaStream_t s) {
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess) dev = -1;
     if (dev < 0 || dev >= 64 || !set[dev].load()) {
-        cudaError_t e = cudaFuncSetAttribute(blocks_attend_kernel<D, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, int(P::SMEM));
-        if (e == cudaSuccess) e = cudaFuncSetAttribute(blocks_attend_kernel<D, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, int(P::SMEM));
+        cudaError_t e = cudaSuccess;
+        for (auto* k : {blocks_attend_kernel<D, true, true>, blocks_attend_kernel<D, true, false>, blocks_attend_kernel<D, false, true>, blocks_attend_kernel<D, false, false>})
+            if (e == cudaSuccess) e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, int(P::SMEM));
         if (e != cudaSuccess) return fail(TQ_ERR_LAUNCH, "tq_blocks_attend: shared memory %zu B: %s", P::SMEM, cudaGetErrorString(e));
         if (dev >= 0 && dev < 64) set[dev].store(true);
     }
@@ -594,8 +662,9 @@ template <int D> int launch_split(const BlockAttendParams& p, cudaStream_t s) {
     cfg.stream = s;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    if (p.e4m3) cudaLaunchKernelEx(&cfg, blocks_attend_kernel<D, true>, p, z);
-    else cudaLaunchKernelEx(&cfg, blocks_attend_kernel<D, false>, p, z);
+    const bool fine = p.dtype == TQ_F16;
+    cudaLaunchKernelEx(&cfg, p.e4m3 ? (fine ? blocks_attend_kernel<D, true, true> : blocks_attend_kernel<D, true, false>)
+                                    : (fine ? blocks_attend_kernel<D, false, true> : blocks_attend_kernel<D, false, false>), p, z);
     if (int rc = check_launch("tq_blocks_attend")) return rc;
     if (!z.merge) return TQ_OK;
     cfg.gridDim = dim3(z.jobs * HPG);
