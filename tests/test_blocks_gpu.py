@@ -177,6 +177,32 @@ def test_several_tokens(d, block, codes, dtype):
     assert _lib.lib().tq_device_status() == 0
 
 
+@pytest.mark.parametrize("d,codes,dtype", ((128, torch.int8, torch.bfloat16), (64, torch.float8_e4m3fn, torch.float16), (96, torch.int8, torch.float16), (256, torch.float8_e4m3fn, torch.bfloat16)))
+def test_pieces_of_a_prompt(d, codes, dtype):
+    """Many row blocks: runs of key tiles that end inside them, whole ones in between, rows of several lanes and head groups."""
+    from mlx_turboquant_b200 import _lib, blocks
+    for b, hq, h, total, t in ((3, 8, 2, 1500, 600), (1, 20, 1, 900, 333), (2, 5, 5, 700, 700), (1, 1, 1, 4500, 4100), (9, 32, 8, 130, 40)):
+        store = filled(b, h, total, d, 64, codes, dtype, seed=t)
+        q = rows(b, hq, t, d, dtype, 5, std=0)
+        k, v = dense(store, total)
+        for window, sinks in ((None, 0), (100, 0), (333, 70)):
+            check_attention(blocks.attend_blocks(q, *store, total, window=window, sinks=sinks), q, k, v, d ** -0.5, window, sinks)
+    assert _lib.lib().tq_device_status() == 0
+
+
+def test_query_magnitudes():
+    """bfloat16 queries of very different rows, outside the fp16 range."""
+    from mlx_turboquant_b200 import blocks
+    store = filled(1, 1, 500, 128, 64, torch.int8, torch.bfloat16)
+    store[1].mul_(2.0 ** -60)
+    tail = store[4]
+    tail.mul_(2.0 ** -60)
+    k, v = dense(store, 500)
+    for t in (1, 20, 200):
+        q = (rows(1, 4, t, 128, torch.float32, 2, std=0) * torch.exp2(60 - 30 * torch.rand(1, 4, t, 1).cuda())).bfloat16()
+        check_attention(blocks.attend_blocks(q, *store, 500), q, k, v, 128 ** -0.5)
+
+
 @pytest.mark.parametrize("dtype", (torch.float16, torch.bfloat16, torch.float32))
 @pytest.mark.parametrize("length", (0, 5, 62, 63, 64, 200, 1000))
 def test_the_new_token_joins(length, dtype):
@@ -220,18 +246,19 @@ def test_hidden_values_do_not_count():
                 assert torch.equal(blocks.attend_blocks(q, *store, total, window=window, sinks=2), ref)
 
 
-@pytest.mark.parametrize("t", (5, 90))
+@pytest.mark.parametrize("t", (5, 40, 190))
 @pytest.mark.parametrize("dtype", (torch.float16, torch.bfloat16, torch.float32))
 def test_what_is_not_finite_reaches_those_who_see_it(dtype, t):
-    """A NaN or an infinity in one token: NaN for the queries that see it, the same bits as without it for the others."""
+    """A NaN or an infinity in one token: not finite for the queries that see it, the others' results as without it.  (Not the same bits: the rows of a warp
+    move their reference maxima together, which a NaN does not ask for, and weights are rounded to fp16 from another reference.  Each is within the bound.)"""
     from mlx_turboquant_b200 import blocks
     for total, at, side, bad in ((250, 247, 0, float("nan")), (250, 248, 1, float("nan")), (250, 246, 1, float("inf")), (200, 199, 1, float("-inf"))):
         k, v = rows(1, 2, total, 64, dtype, 1), rows(1, 2, total, 64, dtype, 2)
         q = rows(1, 8, t, 64, dtype, 3, std=0)
         store = storage(1, 2, total, 64, 128, torch.int8, dtype)
         blocks.write_blocks(k, v, *store, 0)
+        kd, vd = dense(store, total)
         for window in (None, 3):
-            clean = blocks.attend_blocks(q, *store, total, window=window).clone()
             tail = store[4 + side]
             kept = tail.clone()
             tail[:, :, at - 128, 7] = bad
@@ -240,7 +267,12 @@ def test_what_is_not_finite_reaches_those_who_see_it(dtype, t):
             pos = torch.arange(total - t, total)
             sees = (pos >= at) & ((pos - at < window) if window else True)
             assert bool(sees.any())
-            assert torch.equal(got[:, :, ~sees], clean[:, :, ~sees])
+            first = int(sees.nonzero()[0])
+            if first > 0:
+                check_attention(got[:, :, :first], q[:, :, :first], kd[:, :, :total - t + first], vd[:, :, :total - t + first], 0.125, window)
+            last = int(sees.nonzero()[-1]) + 1
+            if last < t:
+                check_attention(got[:, :, last:], q[:, :, last:], kd, vd, 0.125, window)
             hit = got[:, :, sees]
             assert bool((~hit.isfinite()).any(-1).all())
 
