@@ -36,6 +36,7 @@ constexpr int ERR_WAIT = 114;
 constexpr int NSC = 8;                                 // tiles' scales in flight
 constexpr int MAX_CTAS = 160;                          // CTAs of a launch (one per SM)
 constexpr int TN = 64;                                 // tokens per key tile
+constexpr int TILE_INFO = 2 * TN + 4;                  // words that go with a tile: scales, first token, end of its region
 
 template <int D, bool FUSED> struct Plan {
     static constexpr int NQ = FUSED || D == 256 ? 1 : 2;       // query tiles per CTA
@@ -48,7 +49,7 @@ template <int D, bool FUSED> struct Plan {
     static constexpr uint32_t QBLK = TM * 128u, KBLK = TN * 128u;            // bytes of a 64-column block
     static constexpr uint32_t Q_TILE = NBLK * QBLK, K_TILE = NBLK * KBLK;
     static constexpr uint32_t OFF_Q = 0, OFF_K = NQ * Q_TILE, OFF_V = OFF_K + ST * K_TILE;
-    static constexpr uint32_t SC = 2 * TN * 4, OFF_SC = OFF_V + ST * K_TILE; // per tile float keys[TN], values[TN]
+    static constexpr uint32_t SC = TILE_INFO * 4, OFF_SC = OFF_V + ST * K_TILE;       // per tile float keys[TN], values[TN], int its first token, the end of its region
     static constexpr uint32_t OFF_BAR = OFF_SC + NSC * SC;
     static constexpr uint32_t OFF_SLOT = OFF_BAR + 8 * 48;                   // [0] tensor-memory base, [1] abort
     static constexpr size_t NEED = OFF_SLOT + 16 + 1024, SMEM = NEED > 116 * 1024 ? NEED : 116 * 1024;      // one CTA per SM: it takes all of the tensor memory
@@ -85,7 +86,7 @@ struct Params {
     struct Start { int job, tile; } start[MAX_CTAS + 1];       // where each CTA's run begins: (lane x head group, row block) and its key tile
     float* part;                                       // two partials per CTA: NQ * 128 rows of D + 4 floats (sums, maximum, sum of weights)
     const unsigned char* tiles;                        // expanded: per lane and key tile of the call the keys', the values'
-    const float* scales;                               // ... and their scales, 2 x 64
+    const float* scales;                               // ... and what goes with each
     Tiles all;                                         // the key tiles of the call
     int* status;
 };
@@ -149,12 +150,12 @@ __global__ void __launch_bounds__(Plan<D, FUSED>::NT, 1) blocks_fa_kernel(const 
 
     // This CTA's run: row blocks `job` from key tile `tile` on, up to the next CTA's start
     const Params::Start from = p.start[blockIdx.x], to = p.start[blockIdx.x + 1];
-    struct Segment { int y, blk, lane_c, hg, tq0, t_lo, n; bool whole; Tiles tiles; };
+    struct Segment { int lane_c, hg, tq0, t_lo, n; Tiles tiles; };
     auto segment = [&](int job) -> Segment {
         const int y = job / p.n_blk, blk = job - y * p.n_blk, tq0 = blk * NQ * p.QT;
         const Tiles t(c, q_pos0 + tq0, q_pos0 + min(tq0 + NQ * p.QT, c.Tq) - 1);
         const int lo = job == from.job ? from.tile : 0, hi = job == to.job ? to.tile : t.n;
-        return Segment{y, blk, y / p.HG, y - y / p.HG * p.HG, tq0, lo, hi - lo, lo == 0 && hi == t.n, t};
+        return Segment{y / p.HG, y - y / p.HG * p.HG, tq0, lo, hi - lo, t};
     };
     const int last_job = to.tile > 0 ? to.job : to.job - 1;
 
@@ -198,7 +199,7 @@ __global__ void __launch_bounds__(Plan<D, FUSED>::NT, 1) blocks_fa_kernel(const 
                     if (side) continue;
                     if (j >= NSC && !(ok = wait_bar(SC_FREE + s, j / NSC - 1))) break;
                     mbar_expect_tx(bar(SC_FULL + s), P::SC);
-                    bulk_g2s(sbase + P::OFF_SC + s * P::SC, p.scales + at * 2 * TN, P::SC, bar(SC_FULL + s));
+                    bulk_g2s(sbase + P::OFF_SC + s * P::SC, p.scales + at * TILE_INFO, P::SC, bar(SC_FULL + s));
                     asked_sc = j + 1;
                 }
             }
@@ -286,6 +287,7 @@ __global__ void __launch_bounds__(Plan<D, FUSED>::NT, 1) blocks_fa_kernel(const 
                     v = !in ? 0.f : side ? (fine ? 1.f / f : 0.f) : (fine ? c.scale_log2 / f : __uint_as_float(0x7fffffffu));
                 }
                 if (ct < TN) reinterpret_cast<float*>(smem + P::OFF_SC + s * P::SC)[side * TN + ct] = v;
+                if (side && ct == 0) *reinterpret_cast<int2*>(smem + P::OFF_SC + s * P::SC + 2 * TN * 4) = make_int2(base_of(i), sg.tiles.is_tail(sg.t_lo + i) ? c.total : c.n8);
                 fence_proxy_async();
                 mbar_arrive(bar(full + st));
                 mbar_arrive(bar(SC_FULL + s));
@@ -402,12 +404,16 @@ __global__ void __launch_bounds__(Plan<D, FUSED>::NT, 1) blocks_fa_kernel(const 
             mbar_arrive(bar(Q_FULL + q));
             return some;
         };
-        Segment sg = segment(from.job);
-        bool some = lay_out(sg);
+        int n = 0, tile_tok = 0;                                   // key tiles of the row block; the tile's first query token
+        bool some = false;
+        auto enter = [&](int job) {
+            const Segment sg = segment(job);
+            n = __shfl_sync(0xffffffffu, sg.n, 0);
+            tile_tok = __shfl_sync(0xffffffffu, sg.tq0 + q * p.QT, 0);
+            some = lay_out(sg);
+        };
+        enter(from.job);
         for (int job = from.job; job <= last_job && ok; ++job, ++seg) {
-            const int n = sg.n, heads_here = min(HPG, c.G - sg.hg * HPG), tile_tok = sg.tq0 + q * p.QT;
-            auto row_token = [&](int m) { return tile_tok + ((m & 127) >> gp_bits); };
-            auto row_valid = [&](int m) { return (m & (p.GP - 1)) < heads_here && row_token(m) < c.Tq; };
             if (!some) {
                 // a warp without a row: the others' exponentials have the pipe to themselves.  (What it leaves in tensor memory meets rows that nobody reads.  A
                 // score buffer is full again only behind the products that every warp of the query tile has arrived for, so that no arrival is a phase early.)
@@ -417,24 +423,31 @@ __global__ void __launch_bounds__(Plan<D, FUSED>::NT, 1) blocks_fa_kernel(const 
                     mbar_arrive(bar(P_FULL + sbuf(q, j)));
                     mbar_arrive(bar(SC_FREE + j % NSC));
                 }
-                if (job < last_job && ok) { sg = segment(job + 1); some = lay_out(sg); }
+                if (job < last_job && ok) enter(job + 1);
                 continue;
             }
             const int tile_first = q_pos0 + tile_tok, tile_lo = tile_first + p.QT - c.window;      // position of the tile's first row; the first token that its last row's window holds
             int pos[2];
+            {
+                const int hg = job / p.n_blk % p.HG, heads_here = min(HPG, c.G - hg * HPG);
 #pragma unroll
-            for (int k = 0; k < 2; ++k) pos[k] = row_valid(mf + 8 * k) ? q_pos0 + row_token(mf + 8 * k) : -1;
+                for (int k = 0; k < 2; ++k) {
+                    const int m = m0 + (lane >> 2) + 8 * k, tok = tile_tok + (m >> gp_bits);
+                    pos[k] = (m & (p.GP - 1)) < heads_here && tok < c.Tq ? q_pos0 + tok : -1;
+                }
+            }
             // A row that has seen no token yet keeps m_ref = -1e30, has lvsc for a bias and asks for a reference at its first one.
             float vsc = 1.f, vthr = 0.f, lvsc = 0.f;               // (vthr 0: the first tile with a non-zero value scale picks the scale); log2(vsc)
             float m_ref[2] = {-1e30f, -1e30f};
             u64 l2[2] = {pk(0.f, 0.f), pk(0.f, 0.f)};              // this thread's share of the rows' sums
             auto bias_of = [&](int k) { return m_ref[k] > -1e30f ? lvsc - m_ref[k] : lvsc; };
             for (int i = 0; i < n; ++i, ++j) {
-                const bool in_tail = sg.tiles.is_tail(sg.t_lo + i);
-                const int s = j % NSC, base = (in_tail ? c.n8 : 0) + sg.tiles.tile_of(sg.t_lo + i) * TN, end = in_tail ? c.total : c.n8;      // (a tile's tokens lie before `end`)
+                const int s = j % NSC;
                 ok = wait_bar(SC_FULL + s, j / NSC) && wait_bar(S_FULL + sbuf(q, j), sph(j));
                 if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
                 tc_fence_after();
+                const int2 at_end = *reinterpret_cast<const int2*>(smem + P::OFF_SC + s * P::SC + 2 * TN * 4);
+                const int base = at_end.x, end = at_end.y;         // (the tile's tokens lie before `end`)
                 const float* kn = reinterpret_cast<const float*>(smem + P::OFF_SC + s * P::SC) + t2;
                 const float* vn = kn + TN;
                 const uint32_t s_col = t_frag + sbuf(q, j) * TN;
@@ -566,8 +579,8 @@ __global__ void __launch_bounds__(Plan<D, FUSED>::NT, 1) blocks_fa_kernel(const 
             }
             if (!ok) break;
             // ---- the next row block's queries, then this one's results, still as fragments: 32 bytes of a row from four lanes
-            const Segment now = sg;
-            if (job < last_job) { sg = segment(job + 1); some = lay_out(sg); }
+            const int now_tok = tile_tok;
+            if (job < last_job) enter(job + 1);
             float l_sum[2];
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
@@ -580,7 +593,8 @@ __global__ void __launch_bounds__(Plan<D, FUSED>::NT, 1) blocks_fa_kernel(const 
             ok = __all_sync(0xffffffffu, wait_bar(ALL_DONE + q, seg));
             if (!ok) break;
             tc_fence_after();
-            const bool parts = !now.whole;
+            const int y = job / p.n_blk, lane_c = y / p.HG, gl = p.lane0 + lane_c, b = gl / c.Hkv, h0 = (gl - b * c.Hkv) * c.G + (y - lane_c * p.HG) * HPG;
+            const bool parts = (job == from.job && from.tile > 0) || job == to.job;      // (a run that ends inside this row block, or began there)
             float* const part = p.part + (int64_t(blockIdx.x) * 2 + (seg > 0 ? 1 : 0)) * (P::ROWS * (D + 4)) + int64_t(mf) * (D + 4);
             if (parts && t2 == 0) {
 #pragma unroll
@@ -590,14 +604,13 @@ __global__ void __launch_bounds__(Plan<D, FUSED>::NT, 1) blocks_fa_kernel(const 
             float il[2];
             bool store[2];
             char* dst[2];
-            const int gl = p.lane0 + now.lane_c, b = gl / c.Hkv, h0 = (gl - b * c.Hkv) * c.G + now.hg * HPG;
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
-                const int m = mf + 8 * k;
+                const int m = m0 + (lane >> 2) + 8 * k;
                 il[k] = parts ? 1.f : 1.f / l_sum[k];
-                store[k] = parts || row_valid(m);
+                store[k] = parts || pos[k] >= 0;
                 dst[k] = parts ? reinterpret_cast<char*>(part + k * 8 * (D + 4) + t2)
-                               : static_cast<char*>(c.out) + 2 * (((int64_t(b) * c.Hq + h0 + (m & (p.GP - 1))) * c.Tq + row_token(m)) * D + (t2 & 4) + (odd ? 8 : 0));
+                               : static_cast<char*>(c.out) + 2 * (((int64_t(b) * c.Hq + h0 + (m & (p.GP - 1))) * c.Tq + now_tok + (m >> gp_bits)) * D + (t2 & 4) + (odd ? 8 : 0));
             }
             auto rows = [&](int c0, uint32_t (&o)[16]) {           // of eight columns: two of row g, two of row g + 8
                 tmem_ld_frag32(t_frag + P::COL_O + q * DP + c0, o);
@@ -653,7 +666,8 @@ template <int D> __global__ void __launch_bounds__(EX_T) blocks_fa_expand_kernel
     const int64_t lane = p.lane0 + lane_c, at = int64_t(lane_c) * p.all.n + ord;
     const int base = (p.all.is_tail(ord) ? c.n8 : 0) + p.all.tile_of(ord) * TN;
     unsigned char* tiles = const_cast<unsigned char*>(p.tiles) + at * 2 * K_TILE;
-    float* scales = const_cast<float*>(p.scales) + at * 2 * TN;
+    float* scales = const_cast<float*>(p.scales) + at * TILE_INFO;
+    if (tid == 0) *reinterpret_cast<int2*>(scales + 2 * TN) = make_int2(base, p.all.is_tail(ord) ? c.total : c.n8);
     pdl_wait();
     if (!p.all.is_tail(ord)) {
         constexpr int U = 2 * PIECES / EX_T;               // (1024 / 16 = 64 tokens x D / 16 pieces x 2: a multiple of 256 for every D)
@@ -771,7 +785,10 @@ template <int D, bool FUSED> Layout layout_of(const BlockAttendParams& p) {
     return l;
 }
 
-// Equal runs of key tiles for the CTAs: where each one starts in the sequence of row blocks.  The row blocks of every (lane, head group) have the same tiles.
+// Runs of key tiles for the CTAs: where each one starts in the sequence of row blocks.  The row blocks of every (lane, head group) have the same tiles.  Either equal
+// runs, wherever that cuts a row block, or runs of whole row blocks.  A cut costs partials and their merge, 18 us and more where every CTA has one, or some
+// CUT tiles; whole row blocks cost what the longest run has more than the others.
+constexpr int CUT = 20;
 template <int D, bool FUSED> void divide(Params& p, int lanes) {
     const BlockAttendParams& a = p.a;
     const int rows = Plan<D, FUSED>::NQ * p.QT, q0 = a.total - a.Tq;
@@ -780,15 +797,32 @@ template <int D, bool FUSED> void divide(Params& p, int lanes) {
     for (int i = 0; i < p.n_blk; ++i) per_y += tiles_of(i);
     const int64_t total = per_y * lanes * p.HG;
     // at least four tiles a CTA: its set-up, and a partial more to join, cost about as much
-    p.ctas = int(std::max<int64_t>(1, std::min<int64_t>(p.ctas, total / 4)));
-    int blk = 0;
-    int64_t y = 0, before = 0;                             // tiles in front of row block `blk` of y
-    for (int i = 0; i <= p.ctas; ++i) {
-        const int64_t at = total * i / p.ctas, ny = at / per_y, off = at - ny * per_y;
-        if (ny != y) { y = ny; blk = 0; before = 0; }
-        while (blk < p.n_blk && before + tiles_of(blk) <= off) before += tiles_of(blk++);
-        p.start[i] = Params::Start{int(y * p.n_blk + blk), int(off - before)};
-    }
+    const int most = int(std::max<int64_t>(1, std::min<int64_t>(p.ctas, total / 4)));
+    auto fill = [&](bool whole) -> int64_t {               // -> tiles of the longest run
+        int blk = 0, n = 0;
+        int64_t y = 0, before = 0, longest = 0, last = 0;  // tiles in front of row block `blk` of y
+        p.start[0] = Params::Start{0, 0};
+        for (int i = 1; i <= most; ++i) {
+            int64_t at = total * i / most;
+            const int64_t ny = i == most ? int64_t(lanes) * p.HG : at / per_y, off = at - ny * per_y;
+            if (ny != y) { y = ny; blk = 0; before = 0; }
+            while (blk < p.n_blk && before + tiles_of(blk) <= off) before += tiles_of(blk++);
+            Params::Start s{int(y * p.n_blk + blk), int(off - before)};
+            if (whole && s.tile > 0) {                     // to the nearer end of the row block
+                const bool next = 2 * s.tile > tiles_of(blk);
+                at += (next ? tiles_of(blk) : 0) - s.tile;
+                s = Params::Start{s.job + (next ? 1 : 0), 0};
+            }
+            if (s.job == p.start[n].job && s.tile == p.start[n].tile) continue;        // (no run is empty)
+            longest = std::max(longest, at - last);
+            last = at;
+            p.start[++n] = s;
+        }
+        p.ctas = n;
+        return longest;
+    };
+    const int64_t whole = fill(true);
+    if (whole > (total + most - 1) / most + CUT) fill(false);
 }
 
 template <int D, bool FUSED> int launch(const BlockAttendParams& a, unsigned char* ws, cudaStream_t st) {
