@@ -8,7 +8,7 @@
 //   * 8 NQ softmax warps, two rows' shares per thread: tcgen05.ld of the scores as fragments, one packed multiply-add each, ex2, P (fp16) back into tensor
 //     memory; a row's reference maximum is looked at through its sum.  They also lay out their rows of the queries, the next row block's before they write
 //     this one's results;
-//   * one warp issues S = Q K^T and O += P V, the query tiles alternating, scores two key tiles ahead;
+//   * a warp per query tile issues S = Q K^T and O += P V, scores two key tiles ahead;
 //   * keys and values as fp16 operands, by one of two ways:
 //     - expanded (NQ = 2; 1 at d = 256): blocks_fa_expand_kernel has written the tiles to workspace memory once, as they have to lie in shared memory, and two
 //       threads keep four tiles of each in flight (bulk copies).  What many row blocks share is converted once;
@@ -44,7 +44,7 @@ template <int D, bool FUSED> struct Plan {
     static constexpr int ST = D == 256 ? 2 : 4;        // key tiles (and value tiles) in shared memory
     static constexpr int NBLK = (D + 63) / 64;         // 64-column blocks of a row
     static constexpr int DP = NBLK * 64;               // columns of O (d = 96: nobody reads the last 32)
-    static constexpr int SW = NQ * 8, XW = FUSED ? 8 : 2, NT = (SW + 1 + XW) * 32;     // softmax warps; the MMA warp; warps that bring keys and values
+    static constexpr int SW = NQ * 8, XW = FUSED ? 8 : 2, NT = (SW + NQ + XW) * 32;    // softmax warps; MMA warps; warps that bring keys and values
     static constexpr int CH = D / 32;                  // 16-byte pieces of a tile per expanding thread (128 a side)
     static constexpr uint32_t QBLK = TM * 128u, KBLK = TN * 128u;            // bytes of a 64-column block
     static constexpr uint32_t Q_TILE = NBLK * QBLK, K_TILE = NBLK * KBLK;
@@ -58,7 +58,7 @@ template <int D, bool FUSED> struct Plan {
     static_assert(COL_O + NQ * DP <= 512, "tensor memory");
     static_assert(SMEM <= 227 * 1024, "shared memory");
 };
-enum Bars { K_FULL = 0, K_FREE = 4, V_FULL = 8, V_FREE = 12, SC_FULL = 16, SC_FREE = 24, S_FULL = 32, P_FULL = 36, O_DONE = 40, ALL_DONE = 42, Q_FULL = 44, DRAIN = 46 };       // (47 of 8 bytes)
+enum Bars { K_FULL = 0, K_FREE = 4, V_FULL = 8, V_FREE = 12, SC_FULL = 16, SC_FREE = 24, S_FULL = 32, P_FULL = 36, O_DONE = 40, ALL_DONE = 42, Q_FULL = 44, DRAIN = 46 };       // (48 of 8 bytes)
 
 // The key tiles of a range of query positions, in their order: sinks, the window's in blocks, the tail's
 struct Tiles {
@@ -129,11 +129,10 @@ __global__ void __launch_bounds__(Plan<D, FUSED>::NT, 1) blocks_fa_kernel(const 
 
     if (tid == 0) {
         for (int i = 0; i < 4; ++i) {
-            mbar_init(bar(K_FULL + i), FUSED ? 128 : 1); mbar_init(bar(K_FREE + i), 1); mbar_init(bar(V_FULL + i), FUSED ? 128 : 1); mbar_init(bar(V_FREE + i), 1);
+            mbar_init(bar(K_FULL + i), FUSED ? 128 : 1); mbar_init(bar(K_FREE + i), NQ); mbar_init(bar(V_FULL + i), FUSED ? 128 : 1); mbar_init(bar(V_FREE + i), NQ);
             mbar_init(bar(S_FULL + i), 1); mbar_init(bar(P_FULL + i), 256);
         }
-        for (int i = 0; i < 2; ++i) { mbar_init(bar(O_DONE + i), 1); mbar_init(bar(ALL_DONE + i), 1); mbar_init(bar(Q_FULL + i), 256); }
-        mbar_init(bar(DRAIN), 1);
+        for (int i = 0; i < 2; ++i) { mbar_init(bar(O_DONE + i), 1); mbar_init(bar(ALL_DONE + i), 1); mbar_init(bar(Q_FULL + i), 256); mbar_init(bar(DRAIN + i), 1); }
         for (int i = 0; i < NSC; ++i) { mbar_init(bar(SC_FULL + i), FUSED ? 256 : 1); mbar_init(bar(SC_FREE + i), NQ * 256); }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         slot[1] = 0u;
@@ -149,7 +148,9 @@ __global__ void __launch_bounds__(Plan<D, FUSED>::NT, 1) blocks_fa_kernel(const 
     const uint32_t tmem = __shfl_sync(0xffffffffu, slot[0], 0);
 
     // This CTA's run: row blocks `job` from key tile `tile` on, up to the next CTA's start
-    const Params::Start from = p.start[blockIdx.x], to = p.start[blockIdx.x + 1];
+    // (a value that a lane hands round is uniform for the compiler: loops and operands in uniform registers)
+    auto uniform = [](int v) { return __shfl_sync(0xffffffffu, v, 0); };
+    const Params::Start from{uniform(p.start[blockIdx.x].job), uniform(p.start[blockIdx.x].tile)}, to{uniform(p.start[blockIdx.x + 1].job), uniform(p.start[blockIdx.x + 1].tile)};
     struct Segment { int lane_c, hg, tq0, t_lo, n; Tiles tiles; };
     auto segment = [&](int job) -> Segment {
         const int y = job / p.n_blk, blk = job - y * p.n_blk, tq0 = blk * NQ * p.QT;
@@ -177,10 +178,10 @@ __global__ void __launch_bounds__(Plan<D, FUSED>::NT, 1) blocks_fa_kernel(const 
     auto sbuf = [](int q, int j) { return q * SB + j % SB; };
     auto sph = [](int j) { return j / SB; };
 
-    if (!FUSED && warp > P::SW) {
+    if (!FUSED && warp >= P::SW + NQ) {
         // ======================= expanded tiles: one thread the keys and scales, one the values =======================
         if (lane == 0) {
-            const int side = warp - P::SW - 1, full = side ? V_FULL : K_FULL, free_ = side ? V_FREE : K_FREE;
+            const int side = warp - P::SW - NQ, full = side ? V_FULL : K_FULL, free_ = side ? V_FREE : K_FREE;
             const uint32_t ring = sbase + (side ? P::OFF_V : P::OFF_K);
             int j = 0, asked = 0, asked_sc = 0;
             bool ok = true;
@@ -207,9 +208,9 @@ __global__ void __launch_bounds__(Plan<D, FUSED>::NT, 1) blocks_fa_kernel(const 
             for (int i = max(0, asked_sc - NSC); i < asked_sc; ++i) drain(SC_FULL + i % NSC, i / NSC);
         }
         __syncwarp();
-    } else if (FUSED && warp > P::SW) {
+    } else if (FUSED && warp >= P::SW + NQ) {
         // ======================= codes to operands: four warps the keys, four the values =======================
-        const int side = (warp - P::SW - 1) >> 2, ct = tid - (P::SW + 1 + 4 * side) * 32;                  // 0 ... 127
+        const int side = (warp - P::SW - NQ) >> 2, ct = tid - (P::SW + NQ + 4 * side) * 32;                  // 0 ... 127
         const uint32_t ring = sbase + (side ? P::OFF_V : P::OFF_K);
         const int full = side ? V_FULL : K_FULL, free_ = side ? V_FREE : K_FREE;
         int j = 0;
@@ -294,60 +295,68 @@ __global__ void __launch_bounds__(Plan<D, FUSED>::NT, 1) blocks_fa_kernel(const 
             }
         }
         __syncwarp();
-    } else if (warp == P::SW) {
-        // ======================= MMA issue: one warp, uniform =======================
-        auto wait_all = [&](int which, int phase) -> bool { return __all_sync(0xffffffffu, wait_bar(which, phase)); };
+    } else if (warp >= P::SW) {
+        // ======================= MMA issue: one warp per query tile, uniform =======================
+        // (With one warp for both query tiles its waits and the products' issue, one after the other, were what the softmax warps waited for: 1.3 us a key tile
+        // at d = 128, of 0.7 us of products.)
+        const int q = warp - P::SW;
+        // up to three barriers at once, a lane each
+        auto wait_all = [&](int w0, int p0, int w1, int p1, int w2, int p2) -> bool {
+            const uint32_t addr = bar(lane == 0 ? w0 : lane == 1 ? w1 : w2), parity = uint32_t(lane == 0 ? p0 : lane == 1 ? p1 : p2) & 1u;
+            bool done = false;
+            for (uint32_t i = 0; i < WAIT_LIMIT; ++i) {
+                done = done || mbar_try(addr, parity);
+                if (__all_sync(0xffffffffu, done)) { __syncwarp(); return true; }
+                if ((i & 1023u) == 1023u && __any_sync(0xffffffffu, slot[1] != 0u)) return false;
+            }
+            slot[1] = 1u;
+            if (lane == 0) atomicCAS(p.status, 0, ERR_WAIT);
+            return false;
+        };
+        auto wait_one = [&](int which, int phase) { return wait_all(which, phase, which, phase, which, phase); };
         bool ok = true, any = false;
         int j0 = 0, seg = 0;
         for (int job = from.job; job <= last_job && ok; ++job, ++seg) {
-            const int n = segment(job).n;
-            auto issue_qk = [&](int q, int j) {                    // S = Q K^T of key tile j
+            const int n = uniform(segment(job).n);
+            auto issue_qk = [&](int j) {                           // S = Q K^T of key tile j
                 const uint32_t s = tmem + sbuf(q, j) * TN;
 #pragma unroll
                 for (int ks = 0; ks < D / 16; ++ks)
                     umma_ss(s, desc_k(sbase + P::OFF_Q + q * P::Q_TILE, P::QBLK, ks), desc_k(sbase + P::OFF_K + (j % ST) * P::K_TILE, P::KBLK, ks),
                             idesc_of(TN, false), ks > 0 ? 1u : 0u);
                 umma_commit(bar(S_FULL + sbuf(q, j)));
+                umma_commit(bar(K_FREE + j % ST));
             };
-            auto issue_pv = [&](int q, int j) {                    // O += P V
+            auto issue_pv = [&](int j) {                           // O += P V
                 const uint32_t a = tmem + sbuf(q, j) * TN;
 #pragma unroll
                 for (int ks = 0; ks < TN / 16; ++ks)
                     umma_ts(tmem + P::COL_O + q * DP, a + ks * 8, desc_mn(sbase + P::OFF_V + (j % ST) * P::K_TILE, P::KBLK, ks), idesc_of(DP, true),
                             (j > j0 || ks > 0) ? 1u : 0u);
                 umma_commit(bar(O_DONE + q));
+                umma_commit(bar(V_FREE + j % ST));
                 if (j == j0 + n - 1) umma_commit(bar(ALL_DONE + q));       // (a barrier of its own: a parity wait on O_DONE could be two phases early or one late)
             };
-            for (int q = 0; q < NQ && ok; ++q) ok = wait_all(Q_FULL + q, seg);
+            ok = wait_one(Q_FULL + q, seg);
             for (int j = j0; j < j0 + min(n, SB) && ok; ++j) {
-                ok = wait_all(K_FULL + j % ST, j / ST);
+                ok = wait_one(K_FULL + j % ST, j / ST);
                 if (!ok) break;
                 tc_fence_after();
                 any = true;
-                for (int q = 0; q < NQ; ++q) issue_qk(q, j);
-                umma_commit(bar(K_FREE + j % ST));
+                issue_qk(j);
             }
             for (int j = j0; j < j0 + n && ok; ++j) {
-                ok = wait_all(V_FULL + j % ST, j / ST);
                 const int jn = j + SB;                             // the key tile whose scores go where P of tile j sits now
-                for (int q = 0; q < NQ && ok; ++q) {
-                    ok = wait_all(P_FULL + sbuf(q, j), sph(j));
-                    if (!ok) break;
-                    tc_fence_after();
-                    issue_pv(q, j);
-                    if (q == NQ - 1) umma_commit(bar(V_FREE + j % ST));
-                    if (jn < j0 + n) {                             // (the tensor core takes one thread's products in order)
-                        if (q == 0) ok = wait_all(K_FULL + jn % ST, jn / ST);
-                        if (!ok) break;
-                        tc_fence_after();
-                        issue_qk(q, jn);
-                        if (q == NQ - 1) umma_commit(bar(K_FREE + jn % ST));
-                    }
-                }
+                const bool more = jn < j0 + n;
+                ok = wait_all(P_FULL + sbuf(q, j), sph(j), V_FULL + j % ST, j / ST, more ? K_FULL + jn % ST : P_FULL + sbuf(q, j), more ? jn / ST : sph(j));
+                if (!ok) break;
+                tc_fence_after();
+                issue_pv(j);
+                if (more) issue_qk(jn);                            // (the tensor core takes one thread's products in order)
             }
             j0 += n;
         }
-        if (any) { umma_commit(bar(DRAIN)); drain(DRAIN, 0); }     // (nobody waits for the last products of a query tile without a row)
+        if (any) { umma_commit(bar(DRAIN + q)); drain(DRAIN + q, 0); }     // (nobody waits for the last products of a query tile without a row)
         __syncwarp();
     } else {
         // ======================= softmax: two rows per thread, sixteen columns of each =======================
@@ -408,8 +417,8 @@ __global__ void __launch_bounds__(Plan<D, FUSED>::NT, 1) blocks_fa_kernel(const 
         bool some = false;
         auto enter = [&](int job) {
             const Segment sg = segment(job);
-            n = __shfl_sync(0xffffffffu, sg.n, 0);
-            tile_tok = __shfl_sync(0xffffffffu, sg.tq0 + q * p.QT, 0);
+            n = uniform(sg.n);
+            tile_tok = uniform(sg.tq0 + q * p.QT);
             some = lay_out(sg);
         };
         enter(from.job);
