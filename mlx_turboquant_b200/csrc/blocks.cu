@@ -68,78 +68,153 @@ template <typename E> __device__ __forceinline__ Eight8<E> load8(const E* p) { r
 template <typename E> __device__ __forceinline__ void store8(E* p, const Eight8<E>& v) { *reinterpret_cast<Eight8<E>*>(p) = v; }
 template <typename E> __device__ __forceinline__ float at8(const Eight8<E>& v, int i) { return to_f32<E>(reinterpret_cast<const E*>(&v)[i]); }
 
+// the largest magnitude of eight values, as the bits of the type, and as those of a float32
+__device__ __forceinline__ uint32_t largest8(const uint4& v) {
+    const uint32_t k = 0x7fff7fffu, z = __vmaxu2(__vmaxu2(v.x & k, v.y & k), __vmaxu2(v.z & k, v.w & k));
+    return max(z & 0xffffu, z >> 16);
+}
+__device__ __forceinline__ uint32_t largest8(const Eight8<__half>& e) { return largest8(e.v); }
+__device__ __forceinline__ uint32_t largest8(const Eight8<__nv_bfloat16>& e) { return largest8(e.v); }
+__device__ __forceinline__ uint32_t largest8(const Eight8<float>& e) {
+    const uint32_t k = 0x7fffffffu;
+    return max(max(max(e.v[0].x & k, e.v[0].y & k), max(e.v[0].z & k, e.v[0].w & k)), max(max(e.v[1].x & k, e.v[1].y & k), max(e.v[1].z & k, e.v[1].w & k)));
+}
+template <typename E> __device__ __forceinline__ uint32_t bits32(uint32_t b) {
+    return std::is_same<E, float>::value ? b : std::is_same<E, __half>::value ? __float_as_uint(__half2float(__ushort_as_half(uint16_t(b)))) : b << 16;
+}
+
 constexpr int WR_U = 4;                      // vectors of eight values per thread: a CTA has block * d / 32 threads (32 to 1024)
 
-// One CTA per (lane, keys or values, block).  The CTA of the first block is the only one that reads the tail, and the one that leaves the rest there
-// (behind its own reads).
-template <typename E> __global__ void __launch_bounds__(1024) blocks_write_kernel(const __grid_constant__ WriteParams p) {
-    __shared__ uint32_t top[32];
-    const int unit = blockIdx.x % p.units, ls = blockIdx.x / p.units, side = ls & 1, lane = ls >> 1;
-    const WriteSide& w = p.side[side];
-    const int b = lane / p.Hkv, h = lane - b * p.Hkv, per_row = p.d / 8, tid = threadIdx.x;
-    const E* src = static_cast<const E*>(w.x) + b * w.sb + h * w.sh;
-    E* tail = static_cast<E*>(w.tail) + int64_t(lane) * p.block * p.d;
-    pdl_wait();
-    if (p.whole > 0) {
-        const int n = p.block * per_row;                                   // vectors of the block
-        const int64_t first = int64_t(unit) * p.block - p.old;             // new token of the block's row 0 (negative: in the tail)
-        Eight8<E> x[WR_U];
-        uint32_t mx = 0;
+// two float32 at once
+__device__ __forceinline__ uint64_t two(float a, float b) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ uint64_t add_two(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ uint2 halves_of(uint64_t v) {
+    uint2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=r"(r.x), "=r"(r.y) : "l"(v));
+    return r;
+}
+
+// A CTA works on blocks of (lane, keys or values), gridDim.x apart, the next one's rows on their way in registers while this one is quantised.  Bound by instructions
+// as much as by memory: the places of a thread's vectors in a block are the same for all blocks, the maximum is taken on the types' own bits, sums are packed
+// (us for 8 x 65,519 tokens a side at d = 128, 402 MB: a CTA per block 110; one after the other with divisions inside 115; so 90, then FIGURE).
+// The first block of a lane is the only one that reads the tail, and whoever works on it leaves the rest there, behind its own reads.
+template <typename E, bool E4M3> __global__ void __launch_bounds__(1024) blocks_write_kernel(const __grid_constant__ WriteParams p) {
+    __shared__ uint32_t top[2][32];
+    const int per_row = p.d / 8, tid = threadIdx.x, n = p.block * per_row, units = p.units;          // (n: vectors of a block)
+    int row[WR_U], at[WR_U];                               // this thread's vectors of a block: row, value
 #pragma unroll
-        for (int u = 0; u < WR_U; ++u) {
-            const int i = tid + u * blockDim.x;
-            if (i < n) {
-                const int row = i / per_row, c = (i - row * per_row) * 8;
-                const int64_t t = first + row;
-                x[u] = load8<E>(t < 0 ? tail + int64_t(row) * p.d + c : src + t * w.st + c);
-            }
+    for (int u = 0; u < WR_U; ++u) {
+        const int i = tid + u * blockDim.x;
+        row[u] = i < n ? i / per_row : -1;
+        at[u] = (i - i / per_row * per_row) * 8;
+    }
+    // units i = (lane, side, block): the next one without a division
+    const uint32_t step_ls = gridDim.x / uint32_t(units), step_unit = gridDim.x - step_ls * uint32_t(units);
+    uint32_t ls = blockIdx.x / uint32_t(units), unit = blockIdx.x - ls * uint32_t(units);
+    const E *src = nullptr;
+    E* tail = nullptr;
+    int64_t st = 0;
+    auto enter = [&]() {
+        const uint32_t lane = ls >> 1;
+        const bool v = ls & 1;
+        const int64_t sb = v ? p.side[1].sb : p.side[0].sb, sh = v ? p.side[1].sh : p.side[0].sh;
+        st = v ? p.side[1].st : p.side[0].st;
+        int64_t off = int64_t(lane) * sh;
+        if (sb != int64_t(p.Hkv) * sh) {                   // (lanes that are not evenly spaced)
+            const uint32_t b = lane / uint32_t(p.Hkv);
+            off = b * sb + (lane - b * uint32_t(p.Hkv)) * sh;
         }
+        src = static_cast<const E*>(v ? p.side[1].x : p.side[0].x) + off;
+        tail = static_cast<E*>(v ? p.side[1].tail : p.side[0].tail) + int64_t(lane) * p.block * p.d;
+    };
+    pdl_wait();
+    pdl_trigger();
+    Eight8<E> next[WR_U];
+    auto load = [&]() {
+        const int first = int(unit) * p.block - p.old;     // new token of the block's row 0 (negative: in the tail)
 #pragma unroll
         for (int u = 0; u < WR_U; ++u)
-            if (tid + u * int(blockDim.x) < n)
+            if (row[u] >= 0) next[u] = load8<E>((first + row[u] < 0 ? tail + row[u] * p.d : src + (first + row[u]) * st) + at[u]);
+    };
+    enter();
+    if (p.whole > 0) load();
+    for (int turn = 0;; turn ^= 1) {
+        const uint32_t ls0 = ls, unit0 = unit;
+        const E* const src0 = src;
+        E* const tail0 = tail;
+        const int64_t st0 = st;
+        ls += step_ls;
+        unit += step_unit;
+        if (unit >= uint32_t(units)) { unit -= uint32_t(units); ++ls; }
+        const bool more = ls < uint32_t(p.lanes) * 2u;
+        if (p.whole > 0) {
+            Eight8<E> x[WR_U];
+            uint32_t mx = 0;
 #pragma unroll
-                for (int i = 0; i < 8; ++i) mx = max(mx, __float_as_uint(at8<E>(x[u], i)) & 0x7fffffffu);      // (magnitudes order like integers, NaN above infinity)
-        mx = __reduce_max_sync(0xffffffffu, mx);
-        if ((tid & 31) == 0) top[tid >> 5] = mx;
-        __syncthreads();
-        mx = (tid & 31) < int(blockDim.x >> 5) ? top[tid & 31] : 0u;
-        mx = __reduce_max_sync(0xffffffffu, mx);
-        const float a = __uint_as_float(mx), largest = p.e4m3 ? 448.f : 127.f;
-        const bool finite = mx < 0x7f800000u;
-        // (127 / A overflows below 4e-37: values that small lose digits, and zeros stay zeros)
-        const float inv = !finite || mx == 0u ? 0.f : fminf(__fdiv_rn(largest, a), 3.4028235e38f);
-        const int64_t blk = int64_t(lane) * p.blocks_cap + p.at + unit;
-        uint2* out = reinterpret_cast<uint2*>(static_cast<uint8_t*>(w.codes) + blk * p.block * p.d);
-#pragma unroll
-        for (int u = 0; u < WR_U; ++u) {
-            const int i = tid + u * blockDim.x;
-            if (i >= n) continue;
-            uint32_t c[2];
-#pragma unroll
-            for (int k = 0; k < 2; ++k) {
-                float y[4];
-#pragma unroll
-                for (int j = 0; j < 4; ++j) y[j] = __fmul_rn(at8<E>(x[u], 4 * k + j), inv);
-                if (p.e4m3) {
-                    c[k] = e4m3x2_of(y[0], y[1]) | (e4m3x2_of(y[2], y[3]) << 16);
-                } else {
-                    c[k] = 0;
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) c[k] |= uint32_t(__float2int_rn(y[j]) & 255) << (8 * j);
-                }
+            for (int u = 0; u < WR_U; ++u) {
+                x[u] = next[u];
+                if (row[u] >= 0) mx = max(mx, largest8(x[u]));         // (magnitudes order like integers, NaN above infinity)
             }
-            out[i] = finite ? make_uint2(c[0], c[1]) : make_uint2(0u, 0u);
+            if (more) {
+                enter();
+                load();
+            }
+            mx = __reduce_max_sync(0xffffffffu, mx);
+            if ((tid & 31) == 0) top[turn][tid >> 5] = mx;
+            __syncthreads();                               // (the maxima of two blocks take turns: nobody writes what another still reads)
+            mx = (tid & 31) < int(blockDim.x >> 5) ? top[turn][tid & 31] : 0u;
+            mx = bits32<E>(__reduce_max_sync(0xffffffffu, mx));
+            const float a = __uint_as_float(mx);
+            constexpr float largest = E4M3 ? 448.f : 127.f;
+            const bool finite = mx < 0x7f800000u;
+            // (127 / A overflows below 4e-37: values that small lose digits, and zeros stay zeros)
+            const float inv = !finite || mx == 0u ? 0.f : fminf(__fdiv_rn(largest, a), 3.4028235e38f);
+            const int64_t blk = int64_t(ls0 >> 1) * p.blocks_cap + p.at + unit0;
+            uint2* out = reinterpret_cast<uint2*>(static_cast<uint8_t*>((ls0 & 1) ? p.side[1].codes : p.side[0].codes) + blk * p.block * p.d) + tid;
+            const uint64_t magic2 = two(12582912.f, 12582912.f);
+#pragma unroll
+            for (int u = 0; u < WR_U; ++u) {
+                if (row[u] < 0) continue;
+                uint32_t c[2];
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                    // (products one by one: packed ones are contracted with the sums behind them, and a product next to a tie is then rounded once, not twice)
+                    float y[4];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) y[j] = __fmul_rn(at8<E>(x[u], 4 * k + j), inv);
+                    if (E4M3) {
+                        c[k] = e4m3x2_of(y[0], y[1]) | (e4m3x2_of(y[2], y[3]) << 16);
+                        if (!finite) c[k] = 0u;            // (a code of its own that is NaN would reach queries that the token is hidden from)
+                    } else {
+                        // to the nearest integer by adding 1.5 * 2^23 (|y| < 2^22): the low byte of the sum; bytes of two words at a time
+                        const uint2 q0 = halves_of(add_two(two(y[0], y[1]), magic2)), q1 = halves_of(add_two(two(y[2], y[3]), magic2));
+                        c[k] = __byte_perm(__byte_perm(q0.x, q0.y, 0x0040), __byte_perm(q1.x, q1.y, 0x0040), 0x5410);
+                    }
+                }
+                out[u * blockDim.x] = make_uint2(c[0], c[1]);
+            }
+            if (tid == 0) ((ls0 & 1) ? p.side[1].scales : p.side[0].scales)[blk] = finite ? __fdiv_rn(a, largest) : __uint_as_float(0x7fffffffu);
+        } else if (more) {
+            enter();
         }
-        if (tid == 0) w.scales[blk] = finite ? __fdiv_rn(a, largest) : __uint_as_float(0x7fffffffu);
-    }
-    if (unit == 0) {
-        // the rest: behind the whole blocks from row 0 on, or behind what the tail holds
-        const int row0 = p.whole > 0 ? 0 : p.old, rows = p.rest - row0;
-        const int64_t t0 = p.whole > 0 ? p.n_new - p.rest : 0;
-        for (int i = tid; i < rows * per_row; i += blockDim.x) {
-            const int row = i / per_row, c = (i - row * per_row) * 8;
-            store8<E>(tail + int64_t(row0 + row) * p.d + c, load8<E>(src + (t0 + row) * w.st + c));
+        if (unit0 == 0) {
+            // the rest: behind the whole blocks from row 0 on, or behind what the tail holds
+            const int row0 = p.whole > 0 ? 0 : p.old, rows = p.rest - row0;
+            const int64_t t0 = p.whole > 0 ? p.n_new - p.rest : 0;
+            for (int i = tid; i < rows * per_row; i += blockDim.x) {
+                const int r = i / per_row, c = (i - r * per_row) * 8;
+                store8<E>(tail0 + int64_t(row0 + r) * p.d + c, load8<E>(src0 + (t0 + r) * st0 + c));
+            }
         }
+        if (!more) break;
     }
 }
 
@@ -181,6 +256,7 @@ template <typename O> __global__ void __launch_bounds__(RD_T) blocks_read_kernel
     const float* scales = p.scales[side] + lane * (p.cap >> p.shift);
     O* out = static_cast<O*>(p.out[side]) + lane * p.length * p.d;
     pdl_wait();
+    pdl_trigger();
     uint4 c[RD_U];
     float s[RD_U];
 #pragma unroll
@@ -242,14 +318,17 @@ extern "C" int tq_blocks_write(const tq_block_store* s, const tq_new_rows* k_new
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(unsigned(blocks));
-    cfg.blockDim = dim3(unsigned((s->block * s->d / (8 * WR_U) + 31) / 32 * 32));
+    const int threads = (s->block * s->d / (8 * WR_U) + 31) / 32 * 32;
+    // as many CTAs as the SMs hold (64 registers a thread)
+    const int64_t room = int64_t(blocks_sm_count()) * std::min(32, 1024 / threads);
+    cfg.gridDim = dim3(unsigned(std::min(blocks, room)));
+    cfg.blockDim = dim3(unsigned(threads));
     cfg.stream = static_cast<cudaStream_t>(stream);
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    if (s->dtype == TQ_F16) cudaLaunchKernelEx(&cfg, blocks_write_kernel<__half>, p);
-    else if (s->dtype == TQ_BF16) cudaLaunchKernelEx(&cfg, blocks_write_kernel<__nv_bfloat16>, p);
-    else cudaLaunchKernelEx(&cfg, blocks_write_kernel<float>, p);
+    if (s->dtype == TQ_F16) cudaLaunchKernelEx(&cfg, p.e4m3 ? blocks_write_kernel<__half, true> : blocks_write_kernel<__half, false>, p);
+    else if (s->dtype == TQ_BF16) cudaLaunchKernelEx(&cfg, p.e4m3 ? blocks_write_kernel<__nv_bfloat16, true> : blocks_write_kernel<__nv_bfloat16, false>, p);
+    else cudaLaunchKernelEx(&cfg, p.e4m3 ? blocks_write_kernel<float, true> : blocks_write_kernel<float, false>, p);
     return check_launch("tq_blocks_write");
 }
 

@@ -14,6 +14,7 @@
 //     conversions here: 404 instructions per tile against 376.)
 //   values: fp16, exact for both kinds of codes, times the softmax weights under their block's scale as fp16 - for fp16 tokens with a second part: the
 //     weights' rounding would be as large as the result's own.  (8-bit weights would lose the sum of many small ones.)
+// Where few (lane, group)s have few tiles each, a cluster of CTAs shares one and joins its sums over distributed shared memory: one launch.
 // blocks_merge_kernel: joins the partials of a row that several CTAs worked on, in their order: results do not depend on which one came first.
 // blocks_plain_kernel: a warp per token on CUDA cores, float32 throughout: float32 tokens, head dims without a layout above.
 #include <algorithm>
@@ -94,14 +95,15 @@ template <int D> struct AttendPlan {
     static constexpr uint32_t SIDE = 16 * D, STAGE = 2 * SIDE + 16;          // keys, values, their scales
     static constexpr int KW = D / 16, VW = D / 32;     // words of a lane per key row (two a tile) and value row (four)
     static constexpr int RS = D + 4;                   // floats of a partial row: sums, maximum, sum of weights
-    static constexpr size_t RING = size_t(AW) * ST * STAGE, RED = size_t(AW) * HPG * RS * 4, SMEM = RING > RED ? RING : RED;
+    static constexpr size_t RING = size_t(AW) * ST * STAGE, RED = size_t(AW) * HPG * RS * 4, OWN = size_t(HPG) * RS * 4, QB = size_t(3) * KW * 32 * 4, SMEM = (RING > RED + OWN ? RING : RED + OWN) + QB;
 };
 
 struct AttendGrid {
     int n_units, n_sink, n_win, low_unit, tail_unit;   // tiles of a (lane, group): sink tokens, window tokens in blocks, the tail's from tail_unit on
     int groups, slots;                                 // groups of 8 query rows per lane; partials of one
+    int cluster;                                       // CTAs of a (lane, group) that join their sums over distributed shared memory; 0: runs of tiles
     int merge;                                         // the merge kernel follows
-    uint32_t per, jobs;                                // tiles of a CTA; lanes x groups
+    uint32_t per, jobs;                                // tiles of a CTA's run; lanes x groups
 };
 
 // Which coordinates a lane's words are: a lane of t (keys) or g (values) holds 16-byte pieces of a row where the row has enough of them for all lanes, else parts of one.
@@ -223,11 +225,17 @@ template <int D, bool E4M3, bool FINE> __global__ void __launch_bounds__(AW * 32
     constexpr bool bf = !FINE;
     extern __shared__ __align__(16) unsigned char smem[];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
-    const uint32_t u_first = blockIdx.x * z.per, u_last = min(u_first + z.per, z.jobs * uint32_t(z.n_units));
+    // a run of tiles, or the rank's share of a (lane, group)
+    uint32_t u_first = blockIdx.x * z.per, u_last = min(u_first + z.per, z.jobs * uint32_t(z.n_units));
+    if (z.cluster) {
+        const uint32_t job = blockIdx.x / uint32_t(z.cluster), rank = blockIdx.x - job * uint32_t(z.cluster), n = uint32_t(z.n_units);
+        u_first = job * n + n * rank / uint32_t(z.cluster);
+        u_last = job * n + n * (rank + 1) / uint32_t(z.cluster);
+    }
     const uint32_t ring = static_cast<uint32_t>(__cvta_generic_to_shared(smem)) + uint32_t(warp) * ST * P::STAGE;
     const int n_code = z.n_sink + z.n_win;
     pdl_wait();
-    if (z.merge) pdl_trigger();                        // (the grid is one wave: the merge's CTAs take nobody's place)
+    pdl_trigger();
 
     for (uint32_t at = u_first; at < u_last;) {
         const uint32_t job = at / uint32_t(z.n_units), lane_u = job / uint32_t(z.groups);
@@ -287,6 +295,8 @@ template <int D, bool E4M3, bool FINE> __global__ void __launch_bounds__(AW * 32
         auto mag = [](uint2 v) { const uint32_t m = 0x7fff7fffu, y = __vmaxu2(v.x & m, v.y & m); return max(y & 0xffffu, y >> 16); };
         float q_max;
         {
+            // every warp looks at the whole query (its scale), and turns a word in eight of it into operands for all
+            uint32_t* sq = reinterpret_cast<uint32_t*>(smem + P::SMEM - P::QB);
             uint2 x[P::KW];
             uint32_t mx = 0;
 #pragma unroll
@@ -301,6 +311,7 @@ template <int D, bool E4M3, bool FINE> __global__ void __launch_bounds__(AW * 32
             if (!E4M3 && !(q_max <= 3.4028235e38f)) f = __uint_as_float(0x7fffffffu);       // (integers know no NaN: the scale is one)
 #pragma unroll
             for (int w = 0; w < P::KW; ++w) {
+                if ((w & (AW - 1)) != warp) continue;
                 float y[4];
                 uint32_t part[N];
                 f4(x[w], y, f);
@@ -311,8 +322,13 @@ template <int D, bool E4M3, bool FINE> __global__ void __launch_bounds__(AW * 32
                     digits_of<N>(y, part);
                 }
 #pragma unroll
-                for (int n = 0; n < N; ++n) bq[n][w] = part[n];
+                for (int n = 0; n < N; ++n) sq[(n * P::KW + w) * 32 + lane] = part[n];
             }
+            __syncthreads();
+#pragma unroll
+            for (int w = 0; w < P::KW; ++w)
+#pragma unroll
+                for (int n = 0; n < N; ++n) bq[n][w] = sq[(n * P::KW + w) * 32 + lane];
             const float inv = p.scale_log2 / f;
             const int first = p.total - p.Tq;
 #pragma unroll
@@ -517,6 +533,13 @@ template <int D, bool E4M3, bool FINE> __global__ void __launch_bounds__(AW * 32
         __syncthreads();
         const bool alone = u0 == 0 && u1 == z.n_units;
         const uint32_t slot = blockIdx.x - job * uint32_t(z.n_units) / z.per;
+        auto store = [&](int r, int d0, const float (&x)[4], float l) {
+            const int rr = r0 + r, ti = rr / p.G, h = kv * p.G + rr - ti * p.G;
+            const float il = 1.f / l;
+            char* dst = static_cast<char*>(p.out) + 2 * (((int64_t(b) * p.Hq + h) * p.Tq + ti) * D + d0);
+            *reinterpret_cast<uint2*>(dst) = bf ? make_uint2(pack_bf2(x[0] * il, x[1] * il), pack_bf2(x[2] * il, x[3] * il)) : make_uint2(pack_h2(x[0] * il, x[1] * il), pack_h2(x[2] * il, x[3] * il));
+        };
+        float* own = red + AW * HPG * P::RS;           // (cluster)
         for (int i = tid; i < rows * (D / 4); i += AW * 32) {
             const int r = i / (D / 4), d0 = (i - r * (D / 4)) * 4;
             const float* row = red + r * P::RS;
@@ -532,15 +555,43 @@ template <int D, bool E4M3, bool FINE> __global__ void __launch_bounds__(AW * 32
                 x[0] += a * v.x; x[1] += a * v.y; x[2] += a * v.z; x[3] += a * v.w;
             }
             if (alone) {
-                const int rr = r0 + r, ti = rr / p.G, h = kv * p.G + rr - ti * p.G;
-                const float il = 1.f / l;
-                char* dst = static_cast<char*>(p.out) + 2 * (((int64_t(b) * p.Hq + h) * p.Tq + ti) * D + d0);
-                *reinterpret_cast<uint2*>(dst) = bf ? make_uint2(pack_bf2(x[0] * il, x[1] * il), pack_bf2(x[2] * il, x[3] * il)) : make_uint2(pack_h2(x[0] * il, x[1] * il), pack_h2(x[2] * il, x[3] * il));
+                store(r, d0, x, l);
             } else {
-                float* part = p.part + ((int64_t(job) * z.slots + slot) * HPG + r) * P::RS;
+                float* part = z.cluster ? own + r * P::RS : p.part + ((int64_t(job) * z.slots + slot) * HPG + r) * P::RS;
                 *reinterpret_cast<float4*>(part + d0) = make_float4(x[0], x[1], x[2], x[3]);
                 if (d0 == 0) *reinterpret_cast<float2*>(part + D) = make_float2(top, l);
             }
+        }
+        if (z.cluster > 1) {
+            // the ranks' sums, each rank its share of the group's coordinates, in the ranks' order
+            const uint32_t rank = blockIdx.x % uint32_t(z.cluster), here = static_cast<uint32_t>(__cvta_generic_to_shared(own));
+            asm volatile("barrier.cluster.arrive.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
+            for (int i = tid + int(rank) * AW * 32; i < rows * (D / 4); i += z.cluster * AW * 32) {
+                const int r = i / (D / 4), d0 = (i - r * (D / 4)) * 4;
+                float4 v[8];
+                float2 ml[8];
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                    ml[k] = make_float2(-1e30f, 0.f);
+                    v[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+                    if (k >= z.cluster) continue;
+                    uint32_t at;
+                    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(here + uint32_t(r * P::RS * 4)), "r"(k));
+                    asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(v[k].x), "=f"(v[k].y), "=f"(v[k].z), "=f"(v[k].w) : "r"(at + 4 * d0) : "memory");
+                    asm volatile("ld.shared::cluster.v2.f32 {%0,%1}, [%2];" : "=f"(ml[k].x), "=f"(ml[k].y) : "r"(at + 4 * D) : "memory");
+                }
+                float top = -1e30f, l = 0.f, x[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int k = 0; k < 8; ++k) top = fmaxf(top, ml[k].x);
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                    const float a = ex2(ml[k].x - top);
+                    l += a * ml[k].y;
+                    x[0] += a * v[k].x; x[1] += a * v[k].y; x[2] += a * v[k].z; x[3] += a * v[k].w;
+                }
+                store(r, d0, x, l);
+            }
+            asm volatile("barrier.cluster.arrive.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");      // (a rank's memory stays until all have read it)
         }
         __syncthreads();
     }
@@ -563,6 +614,7 @@ template <int D> __global__ void __launch_bounds__(MG_T) blocks_merge_kernel(con
     const float* part = p.part + (int64_t(job) * z.slots * HPG + r) * P::RS;
     constexpr int STEP = HPG * P::RS;
     pdl_wait();
+    pdl_trigger();
     float m = -1e30f, l = 0.f;
     float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
     if (set < N) {
@@ -628,7 +680,16 @@ template <int D> AttendGrid grid_of(const BlockAttendParams& p) {
     if (units >= (int64_t(1) << 31) || jobs >= (int64_t(1) << 28)) { z.jobs = 0; return z; }
     z.jobs = uint32_t(jobs);
     z.per = uint32_t(std::max<int64_t>(AW, (units + ctas - 1) / ctas));
-    z.merge = z.per % uint32_t(z.n_units) != 0;        // (otherwise every row has one CTA)
+    // A (lane, group) in one launch, by a cluster of up to eight CTAs, or runs of tiles over the whole card and a merge.  In us, from what calls of 8 to 512 lanes
+    // measured: a tile 0.05 with one CTA on an SM and 0.1 with two, a cluster's joining 1, the merge 4.
+    auto tile_us = [&](int64_t n) { return n * 2 > ctas ? 0.1 : 0.05; };
+    double best = double(z.per) * tile_us((units + z.per - 1) / z.per) + (z.per % uint32_t(z.n_units) ? 4.0 : 0.0);
+    for (int c = 1; c <= 8 && (c == 1 || c * AW <= z.n_units + AW - 1); ++c) {
+        const int64_t n = jobs * c;
+        const double us = double((n + ctas - 1) / ctas) * double((z.n_units + c - 1) / c) * tile_us(n) + (c > 1 ? 1.0 : 0.0);
+        if (us < best) { best = us; z.cluster = c; }
+    }
+    z.merge = !z.cluster && z.per % uint32_t(z.n_units) != 0;        // (otherwise every row has one CTA)
     z.slots = std::min((z.n_units - 2) / int(z.per) + 2, z.n_units);
     return z;
 }
@@ -652,21 +713,25 @@ template <int D> int launch_split(const BlockAttendParams& p, cudaStream_t s) {
         if (e != cudaSuccess) return fail(TQ_ERR_LAUNCH, "tq_blocks_attend: shared memory %zu B: %s", P::SMEM, cudaGetErrorString(e));
         if (dev >= 0 && dev < 64) set[dev].store(true);
     }
-    cudaLaunchAttribute attr[1];
+    cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = unsigned(std::max(z.cluster, 1));
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3((z.jobs * uint32_t(z.n_units) + z.per - 1) / z.per);
+    cfg.gridDim = dim3(z.cluster ? z.jobs * uint32_t(z.cluster) : (z.jobs * uint32_t(z.n_units) + z.per - 1) / z.per);
     cfg.blockDim = dim3(AW * 32);
     cfg.dynamicSmemBytes = P::SMEM;
     cfg.stream = s;
     cfg.attrs = attr;
-    cfg.numAttrs = 1;
+    cfg.numAttrs = z.cluster > 1 ? 2 : 1;
     const bool fine = p.dtype == TQ_F16;
     cudaLaunchKernelEx(&cfg, p.e4m3 ? (fine ? blocks_attend_kernel<D, true, true> : blocks_attend_kernel<D, true, false>)
                                     : (fine ? blocks_attend_kernel<D, false, true> : blocks_attend_kernel<D, false, false>), p, z);
     if (int rc = check_launch("tq_blocks_attend")) return rc;
     if (!z.merge) return TQ_OK;
+    cfg.numAttrs = 1;
     cfg.gridDim = dim3(z.jobs * HPG);
     cfg.blockDim = dim3(MG_T);
     cfg.dynamicSmemBytes = 0;

@@ -3,8 +3,7 @@
 //   a' = m (a cos(p f) - b sin(p f)),  b' = m (b cos(p f) + a sin(p f))     for the pairs of the first `dims` coordinates; the rest is copied.
 //
 // Bound by memory: two bytes in and two out per coordinate.  A CTA owns a few tokens: it forms their cosines and sines once in shared memory,
-// dims / 2 per token (angle and turns in float64, the fraction of a turn in float32), and all heads of the tokens use them; a thread moves a vector of VEC
-// coordinates and its partner.
+// dims / 2 per token (angle and turns in float64, the fraction of a turn in float32), and all heads of the tokens use them.
 #include <algorithm>
 
 #include "decode_dev.cuh"
@@ -18,6 +17,7 @@ constexpr int RT_ANGLES = 1024;                        // (cos, sin) pairs that 
 struct RotaryParams {
     tq_rotary_rows part[2];
     int dtype, d, half, interleaved;                   // half: pairs per row
+    int one_batch;
     int per_cta, groups;                               // tokens of a CTA; CTAs that share the heads of the same tokens
     int64_t tokens, length;                            // batch x length
     const double* freqs;
@@ -62,58 +62,96 @@ __device__ __forceinline__ void angles(const RotaryParams& p, float2* cs, int64_
     }
 }
 
-// 16-bit types, vectors of VEC coordinates: dims / 2 (half layout) or dims (interleaved), d, strides and addresses are multiples of VEC
+// 16-bit types, vectors of VEC coordinates: dims / 2 (half layout) or dims (interleaved), d, strides and addresses are multiples of VEC.
+// A thread keeps one vector of the row (and its partner) and walks a run of the CTA's rows (token, head), ROWS loads under way at a time; the first ones are asked for
+// before the angles are formed, and a token's cosines and sines stay in registers over its heads.
 template <typename E, int VEC, bool INTERLEAVED> __global__ void __launch_bounds__(RT) rotary_kernel(const __grid_constant__ RotaryParams p) {
     using V = typename Vec<VEC>::T;
+    constexpr int ROWS = 4, W = INTERLEAVED ? VEC / 2 : VEC;       // angles of a vector
     __shared__ __align__(16) float2 cs[RT_ANGLES];
     const int64_t grp = blockIdx.x / p.groups, tok0 = grp * p.per_cta;
     const int share = int(blockIdx.x - grp * p.groups), n_tok = int(min(int64_t(p.per_cta), p.tokens - tok0));
-    pdl_wait();
-    angles(p, cs, tok0, n_tok);
-    __syncthreads();
     const int heads = p.part[0].heads + p.part[1].heads;
-    // items of a head's row: vectors with their partners (half layout) or on their own (interleaved), then the vectors that are copied
+    // vectors of a row: with their partners (half layout) or on their own (interleaved), then those that are copied
     const int turned = INTERLEAVED ? 2 * p.half / VEC : p.half / VEC, per_row = turned + (p.d - 2 * p.half) / VEC;
-    const int h0 = heads * share / p.groups, h1 = heads * (share + 1) / p.groups, n = n_tok * (h1 - h0) * per_row;
-    for (int i = threadIdx.x; i < n; i += RT) {
-        const int row = i / per_row, c = i - row * per_row, t = row / (h1 - h0);
-        int h = h0 + row - t * (h1 - h0);
-        const int64_t tok = tok0 + t, b = tok / p.length, l = tok - b * p.length;
-        const bool second = h >= p.part[0].heads;
-        const tq_rotary_rows& q = p.part[second];
-        if (second) h -= p.part[0].heads;
-        const E* src = static_cast<const E*>(q.x) + b * q.sb + h * q.sh + l * q.st;
-        E* dst = static_cast<E*>(q.out) + ((b * q.heads + h) * p.length + l) * p.d;
-        if (c >= turned) {
-            const int at = 2 * p.half + (c - turned) * VEC;
-            *reinterpret_cast<V*>(dst + at) = *reinterpret_cast<const V*>(src + at);
-        } else if (INTERLEAVED) {
-            float x[VEC];
-            unpack<E, VEC>(*reinterpret_cast<const V*>(src + c * VEC), x);
-            const float2* w = cs + t * p.half + c * (VEC / 2);
+    const int h0 = heads * share / p.groups, nh = heads * (share + 1) / p.groups - h0, rows = n_tok * nh;
+    const int sets = max(1, RT / per_row), set = threadIdx.x / per_row;
+    const int run = (rows + sets - 1) / sets, r0 = set * run, r1 = set < sets ? min(r0 + run, rows) : 0;
+    pdl_wait();
+    pdl_trigger();
+    auto walk = [&](int c, bool first_pass) {
+        const bool copied = c >= turned;
+        const int at = copied ? 2 * p.half + (c - turned) * VEC : c * VEC;
+        int t = r0 / nh, h = h0 + r0 - t * nh, seen = -1;
+        float2 w[W];
+        V x[ROWS], y[ROWS];
+        E* dst[ROWS];
+        bool angles_there = !first_pass;
+        for (int r = r0; r < r1 || !angles_there; r += ROWS) {
+            int tt = t, hh = h, tok_of[ROWS];
 #pragma unroll
-            for (int j = 0; j < VEC / 2; ++j) {
-                const float2 u = w[j];
-                const float a = x[2 * j], z = x[2 * j + 1];
-                x[2 * j] = a * u.x - z * u.y;
-                x[2 * j + 1] = z * u.x + a * u.y;
+            for (int u = 0; u < ROWS; ++u) {
+                if (r + u < r1) {
+                    const int64_t tok = tok0 + tt, b = p.one_batch ? 0 : tok / p.length, l = tok - b * p.length;
+                    const bool second = hh >= p.part[0].heads;
+                    const tq_rotary_rows& q = p.part[second];
+                    const int hq = second ? hh - p.part[0].heads : hh;
+                    const E* src = static_cast<const E*>(q.x) + b * q.sb + hq * q.sh + l * q.st + at;
+                    dst[u] = static_cast<E*>(q.out) + ((b * q.heads + hq) * p.length + l) * p.d + at;
+                    x[u] = *reinterpret_cast<const V*>(src);
+                    if (!INTERLEAVED && !copied) y[u] = *reinterpret_cast<const V*>(src + p.half);
+                    tok_of[u] = tt;
+                    if (++hh == h0 + nh) { hh = h0; ++tt; }
+                }
             }
-            *reinterpret_cast<V*>(dst + c * VEC) = pack<E, VEC>(x);
-        } else {
-            float x[VEC], y[VEC];
-            unpack<E, VEC>(*reinterpret_cast<const V*>(src + c * VEC), x);
-            unpack<E, VEC>(*reinterpret_cast<const V*>(src + p.half + c * VEC), y);
-            const float2* w = cs + t * p.half + c * VEC;
+            t = tt; h = hh;
+            if (!angles_there) {
+                angles(p, cs, tok0, n_tok);
+                __syncthreads();
+                angles_there = true;
+            }
 #pragma unroll
-            for (int j = 0; j < VEC; ++j) {
-                const float2 u = w[j];
-                const float a = x[j], z = y[j];
-                x[j] = a * u.x - z * u.y;
-                y[j] = z * u.x + a * u.y;
+            for (int u = 0; u < ROWS; ++u) {
+                if (r + u >= r1) continue;
+                if (copied) {
+                    *reinterpret_cast<V*>(dst[u]) = x[u];
+                    continue;
+                }
+                if (tok_of[u] != seen) {
+                    seen = tok_of[u];
+#pragma unroll
+                    for (int j = 0; j < W; ++j) w[j] = cs[seen * p.half + c * W + j];
+                }
+                float a[VEC];
+                unpack<E, VEC>(x[u], a);
+                if (INTERLEAVED) {
+#pragma unroll
+                    for (int j = 0; j < W; ++j) {
+                        const float e = a[2 * j], z = a[2 * j + 1];
+                        a[2 * j] = e * w[j].x - z * w[j].y;
+                        a[2 * j + 1] = z * w[j].x + e * w[j].y;
+                    }
+                } else {
+                    float z[VEC];
+                    unpack<E, VEC>(y[u], z);
+#pragma unroll
+                    for (int j = 0; j < VEC; ++j) {
+                        const float e = a[j], f = z[j];
+                        a[j] = e * w[j % W].x - f * w[j % W].y;
+                        z[j] = f * w[j % W].x + e * w[j % W].y;
+                    }
+                    *reinterpret_cast<V*>(dst[u] + p.half) = pack<E, VEC>(z);
+                }
+                *reinterpret_cast<V*>(dst[u]) = pack<E, VEC>(a);
             }
-            *reinterpret_cast<V*>(dst + c * VEC) = pack<E, VEC>(x);
-            *reinterpret_cast<V*>(dst + p.half + c * VEC) = pack<E, VEC>(y);
         }
+    };
+    if (per_row <= RT) {
+        walk(threadIdx.x - set * per_row, true);
+    } else {
+        // rows of more vectors than there are threads: one row at a time, a thread every 256th of its vectors
+        walk(threadIdx.x, true);
+        for (int c = threadIdx.x + RT; c < per_row; c += RT) walk(c, false);
     }
 }
 
@@ -123,6 +161,7 @@ __global__ void __launch_bounds__(RT) rotary_any_kernel(const __grid_constant__ 
     const int64_t grp = blockIdx.x / p.groups, tok0 = grp * p.per_cta;
     const int share = int(blockIdx.x - grp * p.groups), n_tok = int(min(int64_t(p.per_cta), p.tokens - tok0));
     pdl_wait();
+    pdl_trigger();
     angles(p, cs, tok0, n_tok);
     __syncthreads();
     const int heads = p.part[0].heads + p.part[1].heads, per_row = p.d - p.half;
@@ -175,6 +214,7 @@ extern "C" int tq_rotary(const tq_rotary_args* a, void* stream) {
     if (p.tokens == 0 || heads == 0) return TQ_OK;
     if (!a->freqs) return fail(TQ_ERR_INVALID, "tq_rotary: no frequencies");
     p.dtype = a->dtype; p.d = a->d; p.half = a->dims / 2; p.interleaved = a->interleaved != 0; p.length = a->length;
+    p.one_batch = a->batch == 1;
     p.freqs = a->freqs; p.factor = a->factor; p.offset = a->offset; p.positions = a->positions; p.pos_sb = a->pos_sb;
     int vec = a->dtype == TQ_F32 ? 1 : 8;
     for (int i = 0; i < 2; ++i) {
@@ -185,10 +225,10 @@ extern "C" int tq_rotary(const tq_rotary_args* a, void* stream) {
         while (vec > 1 && (!aligned(r.x, 2 * vec) || !aligned(r.out, 2 * vec) || r.sb % vec || r.sh % vec || r.st % vec)) vec /= 2;
     }
     while (vec > 1 && (a->d % vec || (a->interleaved ? a->dims : a->dims / 2) % vec)) vec /= 2;
-    // Tokens per CTA: about four vectors a thread, so that the angles cost little, unless that leaves SMs without a CTA; heads shared between
-    // CTAs where there are fewer tokens than that.
+    // Tokens per CTA: eight vectors a thread, so that the angles cost little, unless that leaves SMs without CTAs; heads shared between CTAs where there are
+    // fewer tokens than that.
     const int items = heads * std::max(1, (a->d - (a->interleaved ? 0 : a->dims / 2)) / vec);
-    p.per_cta = int(std::max<int64_t>(1, std::min<int64_t>({int64_t(4 * RT / items), p.tokens / 296, int64_t(RT_ANGLES / p.half)})));
+    p.per_cta = int(std::max<int64_t>(1, std::min<int64_t>({int64_t(8 * RT / items), p.tokens / 592, int64_t(RT_ANGLES / p.half)})));
     p.groups = p.per_cta > 1 ? 1 : int(std::max<int64_t>(1, std::min<int64_t>({(int64_t(items) + RT - 1) / RT, 296 / p.tokens, heads})));
     const int64_t blocks = (p.tokens + p.per_cta - 1) / p.per_cta * p.groups;
     if (blocks >= (int64_t(1) << 31)) return fail(TQ_ERR_UNSUPPORTED, "tq_rotary: too many tokens");
