@@ -104,18 +104,16 @@ __device__ __forceinline__ uint2 halves_of(uint64_t v) {
 
 // A CTA works on blocks of (lane, keys or values), gridDim.x apart, the next one's rows on their way in registers while this one is quantised.  Bound by instructions
 // as much as by memory: the places of a thread's vectors in a block are the same for all blocks, the maximum is taken on the types' own bits, sums are packed
-// (us for 8 x 65,519 tokens a side at d = 128, 402 MB: a CTA per block 110; one after the other with divisions inside 115; so 90, then FIGURE).
+// (us for 8 x 65,519 tokens a side at d = 128, 402 MB: a CTA per block 110; one after the other with divisions inside 115; so 90; without the divisions 67 = 6.0 TB/s).
 // The first block of a lane is the only one that reads the tail, and whoever works on it leaves the rest there, behind its own reads.
-template <typename E, bool E4M3> __global__ void __launch_bounds__(1024) blocks_write_kernel(const __grid_constant__ WriteParams p) {
+// FULL: block * d / 32 is a multiple of 32, so that a thread's vectors are block / 4 rows apart, all of them there.
+template <typename E, bool E4M3, bool FULL> __global__ void __launch_bounds__(1024) blocks_write_kernel(const __grid_constant__ WriteParams p) {
     __shared__ uint32_t top[2][32];
     const int per_row = p.d / 8, tid = threadIdx.x, n = p.block * per_row, units = p.units;          // (n: vectors of a block)
-    int row[WR_U], at[WR_U];                               // this thread's vectors of a block: row, value
-#pragma unroll
-    for (int u = 0; u < WR_U; ++u) {
-        const int i = tid + u * blockDim.x;
-        row[u] = i < n ? i / per_row : -1;
-        at[u] = (i - i / per_row * per_row) * 8;
-    }
+    const int row0 = tid / per_row, at = (tid - row0 * per_row) * 8;
+    // row and value of this thread's u-th vector of a block; negative: it has none
+    auto row_of = [&](int u) { return FULL ? row0 + u * (p.block >> 2) : tid + u * int(blockDim.x) < n ? (tid + u * int(blockDim.x)) / per_row : -1; };
+    auto at_of = [&](int u) { return FULL ? at : (tid + u * int(blockDim.x)) % per_row * 8; };
     // units i = (lane, side, block): the next one without a division
     const uint32_t step_ls = gridDim.x / uint32_t(units), step_unit = gridDim.x - step_ls * uint32_t(units);
     uint32_t ls = blockIdx.x / uint32_t(units), unit = blockIdx.x - ls * uint32_t(units);
@@ -140,9 +138,18 @@ template <typename E, bool E4M3> __global__ void __launch_bounds__(1024) blocks_
     Eight8<E> next[WR_U];
     auto load = [&]() {
         const int first = int(unit) * p.block - p.old;     // new token of the block's row 0 (negative: in the tail)
+        if (FULL && first >= 0) {
+            const E* from = src + ((first + row0) * st + at);
+            const int64_t step = (p.block >> 2) * st;
 #pragma unroll
-        for (int u = 0; u < WR_U; ++u)
-            if (row[u] >= 0) next[u] = load8<E>((first + row[u] < 0 ? tail + row[u] * p.d : src + (first + row[u]) * st) + at[u]);
+            for (int u = 0; u < WR_U; ++u, from += step) next[u] = load8<E>(from);
+        } else {
+#pragma unroll
+            for (int u = 0; u < WR_U; ++u) {
+                const int r = row_of(u);
+                if (r >= 0) next[u] = load8<E>((first + r < 0 ? tail + r * p.d : src + (first + r) * st) + at_of(u));
+            }
+        }
     };
     enter();
     if (p.whole > 0) load();
@@ -161,7 +168,7 @@ template <typename E, bool E4M3> __global__ void __launch_bounds__(1024) blocks_
 #pragma unroll
             for (int u = 0; u < WR_U; ++u) {
                 x[u] = next[u];
-                if (row[u] >= 0) mx = max(mx, largest8(x[u]));         // (magnitudes order like integers, NaN above infinity)
+                if (FULL || row_of(u) >= 0) mx = max(mx, largest8(x[u]));      // (magnitudes order like integers, NaN above infinity)
             }
             if (more) {
                 enter();
@@ -182,7 +189,7 @@ template <typename E, bool E4M3> __global__ void __launch_bounds__(1024) blocks_
             const uint64_t magic2 = two(12582912.f, 12582912.f);
 #pragma unroll
             for (int u = 0; u < WR_U; ++u) {
-                if (row[u] < 0) continue;
+                if (!FULL && row_of(u) < 0) continue;
                 uint32_t c[2];
 #pragma unroll
                 for (int k = 0; k < 2; ++k) {
@@ -207,11 +214,11 @@ template <typename E, bool E4M3> __global__ void __launch_bounds__(1024) blocks_
         }
         if (unit0 == 0) {
             // the rest: behind the whole blocks from row 0 on, or behind what the tail holds
-            const int row0 = p.whole > 0 ? 0 : p.old, rows = p.rest - row0;
+            const int to = p.whole > 0 ? 0 : p.old, rows = p.rest - to;
             const int64_t t0 = p.whole > 0 ? p.n_new - p.rest : 0;
             for (int i = tid; i < rows * per_row; i += blockDim.x) {
                 const int r = i / per_row, c = (i - r * per_row) * 8;
-                store8<E>(tail0 + int64_t(row0 + r) * p.d + c, load8<E>(src0 + (t0 + r) * st0 + c));
+                store8<E>(tail0 + int64_t(to + r) * p.d + c, load8<E>(src0 + (t0 + r) * st0 + c));
             }
         }
         if (!more) break;
@@ -319,6 +326,7 @@ extern "C" int tq_blocks_write(const tq_block_store* s, const tq_new_rows* k_new
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cudaLaunchConfig_t cfg{};
     const int threads = (s->block * s->d / (8 * WR_U) + 31) / 32 * 32;
+    const bool full = s->block * s->d / (8 * WR_U) == threads;
     // as many CTAs as the SMs hold (64 registers a thread)
     const int64_t room = int64_t(blocks_sm_count()) * std::min(32, 1024 / threads);
     cfg.gridDim = dim3(unsigned(std::min(blocks, room)));
@@ -326,9 +334,10 @@ extern "C" int tq_blocks_write(const tq_block_store* s, const tq_new_rows* k_new
     cfg.stream = static_cast<cudaStream_t>(stream);
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    if (s->dtype == TQ_F16) cudaLaunchKernelEx(&cfg, p.e4m3 ? blocks_write_kernel<__half, true> : blocks_write_kernel<__half, false>, p);
-    else if (s->dtype == TQ_BF16) cudaLaunchKernelEx(&cfg, p.e4m3 ? blocks_write_kernel<__nv_bfloat16, true> : blocks_write_kernel<__nv_bfloat16, false>, p);
-    else cudaLaunchKernelEx(&cfg, p.e4m3 ? blocks_write_kernel<float, true> : blocks_write_kernel<float, false>, p);
+    auto pick = [&](auto* full8, auto* full_i, auto* any8, auto* any_i) { cudaLaunchKernelEx(&cfg, full ? (p.e4m3 ? full8 : full_i) : (p.e4m3 ? any8 : any_i), p); };
+    if (s->dtype == TQ_F16) pick(blocks_write_kernel<__half, true, true>, blocks_write_kernel<__half, false, true>, blocks_write_kernel<__half, true, false>, blocks_write_kernel<__half, false, false>);
+    else if (s->dtype == TQ_BF16) pick(blocks_write_kernel<__nv_bfloat16, true, true>, blocks_write_kernel<__nv_bfloat16, false, true>, blocks_write_kernel<__nv_bfloat16, true, false>, blocks_write_kernel<__nv_bfloat16, false, false>);
+    else pick(blocks_write_kernel<float, true, true>, blocks_write_kernel<float, false, true>, blocks_write_kernel<float, true, false>, blocks_write_kernel<float, false, false>);
     return check_launch("tq_blocks_write");
 }
 
