@@ -65,9 +65,9 @@ __device__ __forceinline__ void angles(const RotaryParams& p, float2* cs, int64_
 // 16-bit types, vectors of VEC coordinates: dims / 2 (half layout) or dims (interleaved), d, strides and addresses are multiples of VEC.
 // A thread keeps one vector of the row (and its partner) and walks a run of the CTA's rows (token, head), ROWS loads under way at a time; the first ones are asked for
 // before the angles are formed, and a token's cosines and sines stay in registers over its heads.
-template <typename E, int VEC, bool INTERLEAVED> __global__ void __launch_bounds__(RT) rotary_kernel(const __grid_constant__ RotaryParams p) {
+template <typename E, int VEC, bool INTERLEAVED> __global__ void __launch_bounds__(RT, 4) rotary_kernel(const __grid_constant__ RotaryParams p) {
     using V = typename Vec<VEC>::T;
-    constexpr int ROWS = 4, W = INTERLEAVED ? VEC / 2 : VEC;       // angles of a vector
+    constexpr int ROWS = 2, W = INTERLEAVED ? VEC / 2 : VEC;       // angles of a vector
     __shared__ __align__(16) float2 cs[RT_ANGLES];
     const int64_t grp = blockIdx.x / p.groups, tok0 = grp * p.per_cta;
     const int share = int(blockIdx.x - grp * p.groups), n_tok = int(min(int64_t(p.per_cta), p.tokens - tok0));
@@ -225,10 +225,11 @@ extern "C" int tq_rotary(const tq_rotary_args* a, void* stream) {
         while (vec > 1 && (!aligned(r.x, 2 * vec) || !aligned(r.out, 2 * vec) || r.sb % vec || r.sh % vec || r.st % vec)) vec /= 2;
     }
     while (vec > 1 && (a->d % vec || (a->interleaved ? a->dims : a->dims / 2) % vec)) vec /= 2;
-    // Tokens per CTA: eight vectors a thread, so that the angles cost little, unless that leaves SMs without CTAs; heads shared between CTAs where there are
-    // fewer tokens than that.
+    // Tokens per CTA: some eight vectors a thread, so that the angles cost little, and whole waves of four CTAs per SM (8192 tokens x 40 heads, d = 128: 34 us with
+    // 2.3 waves); heads shared between CTAs where there are fewer tokens than that.
     const int items = heads * std::max(1, (a->d - (a->interleaved ? 0 : a->dims / 2)) / vec);
-    p.per_cta = int(std::max<int64_t>(1, std::min<int64_t>({int64_t(8 * RT / items), p.tokens / 592, int64_t(RT_ANGLES / p.half)})));
+    const int64_t slots = 592, most = std::max<int64_t>(1, std::min<int64_t>(10 * RT / items, RT_ANGLES / p.half)), waves = (p.tokens + slots * most - 1) / (slots * most);
+    p.per_cta = int((p.tokens + slots * waves - 1) / (slots * waves));
     p.groups = p.per_cta > 1 ? 1 : int(std::max<int64_t>(1, std::min<int64_t>({(int64_t(items) + RT - 1) / RT, 296 / p.tokens, heads})));
     const int64_t blocks = (p.tokens + p.per_cta - 1) / p.per_cta * p.groups;
     if (blocks >= (int64_t(1) << 31)) return fail(TQ_ERR_UNSUPPORTED, "tq_rotary: too many tokens");
