@@ -95,7 +95,7 @@ template <int D> struct AttendPlan {
     static constexpr uint32_t SIDE = 16 * D, STAGE = 2 * SIDE + 16;          // keys, values, their scales
     static constexpr int KW = D / 16, VW = D / 32;     // words of a lane per key row (two a tile) and value row (four)
     static constexpr int RS = D + 4;                   // floats of a partial row: sums, maximum, sum of weights
-    static constexpr size_t RING = size_t(AW) * ST * STAGE, RED = size_t(AW) * HPG * RS * 4, OWN = size_t(HPG) * RS * 4, QB = size_t(3) * KW * 32 * 4, SMEM = (RING > RED + OWN ? RING : RED + OWN) + QB;
+    static constexpr size_t RING = size_t(AW) * ST * STAGE, RED = size_t(AW) * HPG * RS * 4, OWN = size_t(HPG) * RS * 4, QB = size_t(5) * KW * 32 * 4, SMEM = (RING > RED + OWN ? RING : RED + OWN) + QB;
 };
 
 struct AttendGrid {
@@ -234,8 +234,7 @@ template <int D, bool E4M3, bool FINE> __global__ void __launch_bounds__(AW * 32
     }
     const uint32_t ring = static_cast<uint32_t>(__cvta_generic_to_shared(smem)) + uint32_t(warp) * ST * P::STAGE;
     const int n_code = z.n_sink + z.n_win;
-    pdl_wait();
-    pdl_trigger();
+    bool waited = false;                               // (what only the parameters say is worked out before the kernel in front has ended)
 
     for (uint32_t at = u_first; at < u_last;) {
         const uint32_t job = at / uint32_t(z.n_units), lane_u = job / uint32_t(z.groups);
@@ -244,7 +243,7 @@ template <int D, bool E4M3, bool FINE> __global__ void __launch_bounds__(AW * 32
         const int grp = int(job - lane_u * uint32_t(z.groups)), b = int(lane_u / uint32_t(p.Hkv)), kv = int(lane_u) - b * p.Hkv;
         const int64_t lane_c = lane_u;
 
-        // ---- this warp's tiles of codes are asked for first
+        // ---- queries and this warp's first tiles of codes are asked for
         const uint8_t* kc = p.kc + lane_c * p.cap * D + lane * 16;
         const uint8_t* vc = p.vc + lane_c * p.cap * D + lane * 16;
         const float* sc = (lane ? p.vs : p.ks) + lane_c * (p.cap >> p.shift);
@@ -272,18 +271,28 @@ template <int D, bool E4M3, bool FINE> __global__ void __launch_bounds__(AW * 32
             next += AW;
             fill = fill == ring + (ST - 1) * P::STAGE ? ring : fill + P::STAGE;
         };
+        const int rows = min(HPG, p.Tq * p.G - grp * HPG), r0 = grp * HPG;
+        const char* q_row;                             // row g's
+        {
+            const int r = min(r0 + g, r0 + rows - 1), ti = r / p.G, h = kv * p.G + r - ti * p.G;
+            q_row = static_cast<const char*>(p.q) + 2 * (b * p.q_sb + h * p.q_sh + ti * p.q_st);
+        }
+        if (!waited) {
+            pdl_wait();
+            pdl_trigger();
+            waited = true;
+        }
+        uint2 qx[P::KW];
+#pragma unroll
+        for (int w = 0; w < P::KW; ++w) {
+            qx[w] = *reinterpret_cast<const uint2*>(q_row + 2 * key_dim<D>(w, t));
+            if (g >= rows) qx[w] = make_uint2(0u, 0u);
+        }
 #pragma unroll
         for (int i = 0; i < ST - 1; ++i) ask();
-
         // ---- the group's queries as B operands (row g's coordinates in the order of the key codes)
-        const int rows = min(HPG, p.Tq * p.G - grp * HPG), r0 = grp * HPG;
         Cols c;
         uint32_t bq[N][P::KW];
-        auto query = [&](int w) -> uint2 {             // coordinates key_dim(w, t) ... + 3 of row g
-            const int r = r0 + g, ti = r / p.G, h = kv * p.G + r - ti * p.G;
-            if (g >= rows) return make_uint2(0u, 0u);
-            return *reinterpret_cast<const uint2*>(static_cast<const char*>(p.q) + 2 * (b * p.q_sb + h * p.q_sh + ti * p.q_st + key_dim<D>(w, t)));
-        };
         auto f4 = [&](uint2 v, float (&x)[4], float f) {
             if (bf) {
                 x[0] = __uint_as_float(v.x << 16) * f; x[1] = __uint_as_float(v.x & 0xffff0000u) * f; x[2] = __uint_as_float(v.y << 16) * f; x[3] = __uint_as_float(v.y & 0xffff0000u) * f;
@@ -293,16 +302,13 @@ template <int D, bool E4M3, bool FINE> __global__ void __launch_bounds__(AW * 32
             }
         };
         auto mag = [](uint2 v) { const uint32_t m = 0x7fff7fffu, y = __vmaxu2(v.x & m, v.y & m); return max(y & 0xffffu, y >> 16); };
+        uint32_t* sq = reinterpret_cast<uint32_t*>(smem + P::SMEM - P::QB);
         float q_max;
         {
             // every warp looks at the whole query (its scale), and turns a word in eight of it into operands for all
-            uint32_t* sq = reinterpret_cast<uint32_t*>(smem + P::SMEM - P::QB);
-            uint2 x[P::KW];
             uint32_t mx = 0;
 #pragma unroll
-            for (int w = 0; w < P::KW; ++w) x[w] = query(w);
-#pragma unroll
-            for (int w = 0; w < P::KW; ++w) mx = max(mx, mag(x[w]));
+            for (int w = 0; w < P::KW; ++w) mx = max(mx, mag(qx[w]));
             mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
             mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
             q_max = bf ? __uint_as_float(mx << 16) : __half2float(__ushort_as_half(uint16_t(mx)));
@@ -314,15 +320,16 @@ template <int D, bool E4M3, bool FINE> __global__ void __launch_bounds__(AW * 32
                 if ((w & (AW - 1)) != warp) continue;
                 float y[4];
                 uint32_t part[N];
-                f4(x[w], y, f);
+                f4(qx[w], y, f);
                 if constexpr (E4M3) {
-                    part[0] = bf ? pack_h2(y[0], y[1]) : x[w].x;
-                    part[1] = bf ? pack_h2(y[2], y[3]) : x[w].y;
+                    part[0] = bf ? pack_h2(y[0], y[1]) : qx[w].x;
+                    part[1] = bf ? pack_h2(y[2], y[3]) : qx[w].y;
                 } else {
                     digits_of<N>(y, part);
                 }
 #pragma unroll
                 for (int n = 0; n < N; ++n) sq[(n * P::KW + w) * 32 + lane] = part[n];
+                *reinterpret_cast<uint2*>(sq + ((3 * P::KW + 2 * w) * 32 + 2 * lane)) = qx[w];       // (for the tail)
             }
             __syncthreads();
 #pragma unroll
@@ -416,30 +423,42 @@ template <int D, bool E4M3, bool FINE> __global__ void __launch_bounds__(AW * 32
         for (int u = t0 + ((warp - (t0 - u0)) & (AW - 1)); u < u1; u += AW) {
             const int tok = p.n8 + (z.tail_unit + u - n_code) * 16;
             if (hidden(tok)) continue;
-            // (rows that no query sees are not read: what they hold must not reach the sums)
-            auto row = [&](int j, bool keys) -> const char* {
-                if (j >= p.total || (j < lo_min && j >= p.sinks)) return nullptr;
+            // (a row that no query sees reads as zeros: what it holds must not reach the sums)
+            auto row = [&](int j, bool keys, bool& in) -> const char* {
+                in = j < p.total && (j >= lo_min || j < p.sinks);
+                const int r = in ? j - p.n8 : 0;
                 if (p.kn != nullptr && j == p.total - 1)
                     return keys ? static_cast<const char*>(p.kn) + 2 * (b * p.kn_sb + kv * p.kn_sh) : static_cast<const char*>(p.vn) + 2 * (b * p.vn_sb + kv * p.vn_sh);
-                return static_cast<const char*>(keys ? p.kt : p.vt) + 2 * (lane_c * p.block + (j - p.n8)) * D;
+                return static_cast<const char*>(keys ? p.kt : p.vt) + 2 * (lane_c * p.block + r) * D;
             };
             auto half4 = [&](uint2& v, float f) {
                 v.x = pack_h2(__uint_as_float(v.x << 16) * f, __uint_as_float(v.x & 0xffff0000u) * f);
                 v.y = pack_h2(__uint_as_float(v.y << 16) * f, __uint_as_float(v.y & 0xffff0000u) * f);
             };
             uint2 k[2][P::KW], v[4][P::VW];
+            bool k_in[2], v_in[4];
 #pragma unroll
             for (int r = 0; r < 2; ++r) {
-                const char* src = row(tok + g + 8 * r, true);
+                const char* src = row(tok + g + 8 * r, true, k_in[r]);
 #pragma unroll
-                for (int w = 0; w < P::KW; ++w) k[r][w] = src ? *reinterpret_cast<const uint2*>(src + 2 * key_dim<D>(w, t)) : make_uint2(0u, 0u);
+                for (int w = 0; w < P::KW; ++w) k[r][w] = *reinterpret_cast<const uint2*>(src + 2 * key_dim<D>(w, t));
             }
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                const char* src = row(tok + 2 * t + (r & 1) + 8 * (r >> 1), false);
+                const char* src = row(tok + 2 * t + (r & 1) + 8 * (r >> 1), false, v_in[r]);
 #pragma unroll
-                for (int w = 0; w < P::VW; ++w) v[r][w] = src ? *reinterpret_cast<const uint2*>(src + 2 * value_dim<D>(w, g)) : make_uint2(0u, 0u);
+                for (int w = 0; w < P::VW; ++w) v[r][w] = *reinterpret_cast<const uint2*>(src + 2 * value_dim<D>(w, g));
             }
+#pragma unroll
+            for (int r = 0; r < 2; ++r)
+#pragma unroll
+                for (int w = 0; w < P::KW; ++w)
+                    if (!k_in[r]) k[r][w] = make_uint2(0u, 0u);
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+#pragma unroll
+                for (int w = 0; w < P::VW; ++w)
+                    if (!v_in[r]) v[r][w] = make_uint2(0u, 0u);
             float kn[2] = {1.f, 1.f}, s[4] = {0.f, 0.f, 0.f, 0.f};
             Cols ct = c;
             if (bf) {
@@ -461,7 +480,7 @@ template <int D, bool E4M3, bool FINE> __global__ void __launch_bounds__(AW * 32
                 const float qf = bf ? stage_scale(__float_as_uint(q_max)) : 1.f, inv = p.scale_log2 / qf;
 #pragma unroll
                 for (int w = 0; w < P::KW; ++w) {
-                    uint2 x = query(w);
+                    uint2 x = *reinterpret_cast<const uint2*>(sq + ((3 * P::KW + 2 * w) * 32 + 2 * lane));
                     if (bf) half4(x, qf);
                     mma16816(s, k[0][w].x, k[1][w].x, k[0][w].y, k[1][w].y, x.x, x.y);
                 }
