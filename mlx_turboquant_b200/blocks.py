@@ -129,9 +129,9 @@ def attend_blocks(queries: torch.Tensor, k_codes, k_scales, v_codes, v_scales, k
     the first ``sinks`` of the cache.  ``new`` = (keys, values), (B, H, 1, D): one more token, which joins the cache and is attended to, in the
     same launch unless it completes a block (the cache then holds ``length + 1`` tokens).  ``out`` (contiguous, the queries' shape and type)
     receives the result."""
-    if out is None:
-        res = _lib.host().blocks_attend(queries, k_codes, k_scales, v_codes, v_scales, k_tail, v_tail, length, window or 0, sinks,
-                                        scale, *(new if new is not None else (None, None))) if window != 0 else None
+    if window != 0:
+        res = _lib.host().blocks_attend(queries, k_codes, k_scales, v_codes, v_scales, k_tail, v_tail, length, window or 0, sinks, scale,
+                                        *(new if new is not None else (None, None)), out)
         if res is not None:
             if type(res) is int:
                 _lib.check(res)
@@ -178,3 +178,177 @@ def attend_blocks(queries: torch.Tensor, k_codes, k_scales, v_codes, v_scales, k
         a.workspace, a.workspace_bytes = ws.data_ptr(), need
     _lib.check(_lib.launch(dev, "tq_blocks_attend", C.byref(a), _lib.stream_ptr(dev)))
     return out
+
+
+class BlockKVCache:
+    """KV cache of a layer in 8-bit blocks, behind the protocol of ``TurboQuantKVCache``.
+
+    ``codes``: ``"int8"`` or ``"e4m3"``; ``block``: tokens that share a scale (16, 32, 64 or 128).  With ``window`` a query sees the last ``window`` tokens
+    up to its own and the first ``sinks`` ones; blocks that no later query can see are dropped when their room is wanted, so that the storage stays bounded
+    by the window and the longest piece of prompt.  float16, bfloat16 (or, on slower kernels, float32) tokens, of one type per cache."""
+
+    step = 256
+
+    def __init__(self, head_dim: int = 128, num_kv_heads: int = 1, codes: str = "int8", block: int = 64, window: int | None = None, sinks: int = 0):
+        if codes not in ("int8", "e4m3"):
+            raise ValueError(f"codes must be 'int8' or 'e4m3', got {codes!r}")
+        if block not in BLOCKS:
+            raise ValueError(f"blocks have 16, 32, 64 or 128 tokens, got {block}")
+        if window is not None and window < 1:
+            raise ValueError(f"a window holds the query's own token at least, got {window}")
+        if sinks < 0 or (sinks and window is None):
+            raise ValueError("sinks are the first tokens that stay visible next to a window")
+        self.head_dim, self.num_kv_heads, self.codes, self.block = head_dim, num_kv_heads, codes, block
+        self.window, self.sinks = window, sinks
+        self.offset = 0                # tokens seen
+        self._dropped = 0              # of them no longer stored: whole blocks between the sinks and the window
+        self._store: tuple | None = None
+
+    # ---- storage ------------------------------------------------------------------------------------
+    @property
+    def _length(self) -> int:
+        return self.offset - self._dropped
+
+    def _sink_end(self) -> int:
+        return -(-self.sinks // self.block) * self.block
+
+    def _allocate(self, b: int, h: int, cap: int, dtype, device) -> tuple:
+        codes = torch.int8 if self.codes == "int8" else torch.float8_e4m3fn
+        out = []
+        for _ in range(2):
+            out += [torch.empty((b, h, cap, self.head_dim), dtype=codes, device=device), torch.empty((b, h, cap // self.block), dtype=torch.float32, device=device)]
+        return tuple(out + [torch.empty((b, h, self.block, self.head_dim), dtype=dtype, device=device) for _ in range(2)])
+
+    def _reserve(self, keys: torch.Tensor, t: int) -> None:
+        """Room for the whole blocks that ``t`` more tokens fill: drops what no query can see any more, or grows."""
+        n = self.block
+        if self._store is None:
+            if keys.dim() != 4 or keys.shape[3] != self.head_dim or keys.shape[1] != self.num_kv_heads:
+                raise ValueError(f"tokens must be (B, {self.num_kv_heads}, T, {self.head_dim}), got {tuple(keys.shape)}")
+            cap = max(-(-(t + n) // n) * n, self.step)
+            self._store = self._allocate(keys.shape[0], keys.shape[1], -(-cap // n) * n, keys.dtype, keys.device)
+            return
+        cap = self._store[0].shape[2]
+        need = (self._length + t) // n * n
+        if need <= cap:
+            return
+        first, last = self._sink_end(), self._length // n * n                  # (blocks [first, last) are the window's)
+        drop = 0 if self.window is None else max(0, (self._length - self.window + 1) // n * n - first)
+        if drop and 2 * (need - drop) <= cap:                                  # (half of the storage at least comes free: copies stay rare)
+            for i in (0, 2):
+                codes, scales = self._store[i].view(torch.int8), self._store[i + 1]
+                codes[:, :, first:last - drop] = codes[:, :, first + drop:last].clone()
+                scales[:, :, first // n:(last - drop) // n] = scales[:, :, (first + drop) // n:last // n].clone()
+            self._dropped += drop
+            return
+        keep = last - drop if drop else last
+        new = self._allocate(*self._store[0].shape[:2], -(-max(need - drop, 2 * cap if not drop else 2 * (need - drop)) // n) * n, self._store[4].dtype, self._store[0].device)
+        for i in (0, 2):
+            old, to = self._store[i].view(torch.int8), new[i].view(torch.int8)
+            to[:, :, :min(first, keep)] = old[:, :, :min(first, keep)]
+            to[:, :, first:keep] = old[:, :, first + drop:last]
+            new[i + 1][:, :, :min(first, keep) // n] = self._store[i + 1][:, :, :min(first, keep) // n]
+            new[i + 1][:, :, first // n:keep // n] = self._store[i + 1][:, :, (first + drop) // n:last // n]
+        self._store = (*new[:4], *self._store[4:])
+        self._dropped += drop
+
+    # ---- protocol -------------------------------------------------------------------------------------
+    def update(self, keys: torch.Tensor, values: torch.Tensor) -> None:
+        """Append (B, H, T, D) tokens."""
+        _lib.require_cuda(keys, values)
+        t = keys.shape[2] if keys.dim() == 4 else 0
+        self._reserve(keys, t)
+        write_blocks(keys, values, *self._store, self._length)
+        self.offset += t
+
+    def attend(self, queries: torch.Tensor, scale: float | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+        """softmax(scale q K^T) V for the last T_q tokens: (B, H_q, T_q, D), or (B, H_q, D) for the last one; ``out`` receives the result."""
+        if self._store is None or self.offset == 0:
+            raise ValueError("attend on an empty cache")
+        if queries.dim() == 3:
+            res = self.attend(queries.unsqueeze(2), scale, None if out is None else out.view(*queries.shape[:2], 1, queries.shape[2]))
+            return out if out is not None else res.squeeze(2)
+        if self._dropped and self._length - queries.shape[2] - self.window + 1 < self._sink_end():
+            raise ValueError(f"the window of the first of {queries.shape[2]} query tokens is no longer stored: attend to the tokens of the last update")
+        return attend_blocks(queries, *self._store, self._length, window=self.window, sinks=self.sinks, scale=scale, out=out)
+
+    def decode_step(self, queries: torch.Tensor, keys: torch.Tensor, values: torch.Tensor, scale: float | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+        """``update`` with one token, then ``attend``: one launch unless the token completes a block."""
+        if keys.dim() != 4 or keys.shape[2] != 1 or (queries.dim() == 4 and queries.shape[2] != 1):
+            self.update(keys, values)
+            return self.attend(queries, scale, out)
+        if queries.dim() == 3:
+            res = self.decode_step(queries.unsqueeze(2), keys, values, scale, None if out is None else out.view(*queries.shape[:2], 1, queries.shape[2]))
+            return out if out is not None else res.squeeze(2)
+        _lib.require_cuda(queries, keys, values)
+        self._reserve(keys, 1)
+        res = attend_blocks(queries, *self._store, self._length, window=self.window, sinks=self.sinks, scale=scale, out=out, new=(keys, values))
+        self.offset += 1
+        return res
+
+    def update_and_fetch(self, keys: torch.Tensor, values: torch.Tensor):
+        """Append, and return all tokens dense, of the tokens' type (caches without a window)."""
+        if self.window is not None:
+            raise NotImplementedError("a cache with a window drops what it hides: use update and attend")
+        self.update(keys, values)
+        return read_blocks(*self._store, self._length)
+
+    def make_mask(self, N: int, offset: int = 0, return_array: bool = False, window_size: int | None = None) -> Any | None:
+        """``None`` for a single-token step, ``"causal"`` otherwise; the cache's own window is part of ``attend``."""
+        if window_size is not None and window_size != self.window:
+            raise NotImplementedError(f"this cache has a window of {self.window}, not {window_size}")
+        return None if N == 1 and not return_array else "causal"
+
+    def size(self) -> int:
+        return self.offset
+
+    def empty(self) -> bool:
+        return self.offset == 0
+
+    def is_trimmable(self) -> bool:
+        return False
+
+    @property
+    def nbytes(self) -> int:
+        """Bytes of the stored tokens: codes, scales and the tail's rows."""
+        if self._store is None:
+            return 0
+        b, h, _, d = self._store[0].shape
+        whole, rest = self._length // self.block, self._length % self.block
+        return 2 * b * h * (whole * (self.block * d + 4) + rest * d * self._store[4].element_size())
+
+    # ---- checkpoint -----------------------------------------------------------------------------------
+    @property
+    def state(self):
+        """k_codes, k_scales, v_codes, v_scales (whole blocks only), k_tail, v_tail; or six ``None``."""
+        if self._store is None:
+            return (None,) * 6
+        whole = self._length // self.block
+        return tuple(t[:, :, :whole * self.block] if i in (0, 2) else t[:, :, :whole] if i in (1, 3) else t for i, t in enumerate(self._store))
+
+    @state.setter
+    def state(self, v):
+        if len(v) != 6:
+            raise ValueError(f"state must have 6 elements, got {len(v)}")
+        if all(t is None for t in v):
+            self._store = None
+            return
+        _lib.require_cuda(*v)
+        store = tuple(t.contiguous() for t in v)
+        _store(*store, 0)
+        if store[4].shape[2] != self.block or store[0].shape[3] != self.head_dim or store[0].dtype is not (torch.int8 if self.codes == "int8" else torch.float8_e4m3fn):
+            raise ValueError("the state is of a cache with other blocks, codes or head_dim")
+        self._store = store
+
+    @property
+    def meta_state(self):
+        return {"offset": str(self.offset), "dropped": str(self._dropped), "head_dim": str(self.head_dim), "codes": self.codes, "block": str(self.block),
+                "window": "" if self.window is None else str(self.window), "sinks": str(self.sinks)}
+
+    @meta_state.setter
+    def meta_state(self, v):
+        offset, dropped = int(v["offset"]), int(v["dropped"])
+        if self._store is not None and (offset - dropped) // self.block * self.block > self._store[0].shape[2]:
+            raise ValueError(f"{offset - dropped} tokens in storage for {self._store[0].shape[2]}")
+        self.offset, self._dropped = offset, dropped
+        self.window, self.sinks = (int(v["window"]) if v["window"] else None), int(v["sinks"])

@@ -12,6 +12,8 @@ library work, not part of the compressed path).  Two ways through the cache:
   (append and attention in one launch), ``cache.update(k, v)`` then the causal ``cache.attend(q)`` for a prefill
   chunk.  Caches with a QJL sketch take the dense way for multi-token calls.
 
+Scaled, partial or interleaved rotary embeddings go through ``rope.apply_rotary``.
+
 ``GraphedDecoder`` replays the library part of a decode step (everything between two cache calls) as CUDA graphs.
 
 ``generate`` is the greedy loop of the reference's command line (cli.py:81-104) without its tokenizer.
@@ -23,6 +25,8 @@ from dataclasses import dataclass
 
 import torch
 import torch.nn.functional as F
+
+from . import rope as rotary
 
 
 @dataclass
@@ -38,6 +42,19 @@ class ModelArgs:
     rope_theta: float = 500000.0
     vocab_size: int = 128256
     rms_norm_eps: float = 1e-5
+    rope_scaling: dict | None = None             # {"rope_type": "linear" | "llama3" | "yarn", "factor": ...}; see rope.frequencies
+    rope_traditional: bool = False               # neighbouring coordinates are turned together, not the halves of a head
+    partial_rotary_factor: float = 1.0           # how much of a head is turned
+    fused_rope: bool = False                     # the rotary kernel (rope.apply_rotary) for plain embeddings too: angles in float64, one launch
+
+    @property
+    def rotary_kernel(self) -> bool:
+        """Whether queries and keys go through ``rope.apply_rotary``: what the torch code below does not do, or by choice."""
+        return bool(self.fused_rope or self.rope_scaling or self.rope_traditional or self.partial_rotary_factor != 1.0)
+
+    def rotary_frequencies(self, device):
+        dims = int(self.head_dim * self.partial_rotary_factor) // 2 * 2
+        return rotary.frequencies(dims, self.rope_theta, self.rope_scaling, device)
 
 
 def _rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float) -> torch.Tensor:
@@ -71,6 +88,7 @@ class Attention(torch.nn.Module):
         self.n_heads, self.n_kv_heads, self.head_dim = args.num_attention_heads, args.num_key_value_heads, args.head_dim
         self.scale = self.head_dim ** -0.5
         self.rope_theta = args.rope_theta
+        self.args = args
         kw = dict(bias=False, dtype=dtype, device=device)
         # one fused projection for q, k and v (same arithmetic as three separate matrices)
         self.qkv_proj = torch.nn.Linear(args.hidden_size, (self.n_heads + 2 * self.n_kv_heads) * self.head_dim, **kw)
@@ -82,13 +100,18 @@ class Attention(torch.nn.Module):
         qkv = self.qkv_proj(x).view(B, L, hq + 2 * hkv, d).transpose(1, 2)            # (B, heads, L, d)
         offset = cache.offset if cache is not None else 0                               # read before the update
         # queries and keys sit at the same positions: one pass over both; the tables are shared by layers at one offset
-        tables = rope_memo.get((offset, L)) if rope_memo is not None else None
-        if tables is None:
-            tables = rope_tables(offset, L, d, self.rope_theta, x.device)
-            if rope_memo is not None:
-                rope_memo[(offset, L)] = tables
-        qk = apply_rope(qkv[:, :hq + hkv], tables)
-        queries, keys, values = qk[:, :hq], qk[:, hq:], qkv[:, hq + hkv:]
+        values = qkv[:, hq + hkv:]
+        if self.args.rotary_kernel:
+            freqs, factor = self.args.rotary_frequencies(x.device)
+            queries, keys = rotary.apply_rotary(qkv[:, :hq], qkv[:, hq:hq + hkv], freqs, offset, interleaved=self.args.rope_traditional, factor=factor)
+        else:
+            tables = rope_memo.get((offset, L)) if rope_memo is not None else None
+            if tables is None:
+                tables = rope_tables(offset, L, d, self.rope_theta, x.device)
+                if rope_memo is not None:
+                    rope_memo[(offset, L)] = tables
+            qk = apply_rope(qkv[:, :hq + hkv], tables)
+            queries, keys = qk[:, :hq], qk[:, hq:]
         if cache is not None and packed and hasattr(cache, "attend") and (L == 1 or not getattr(cache, "qjl_correction", False)):
             # attention straight from packed storage: one launch for a decode step (the token's append included), the
             # causal multi-token kernel for prefill chunks (caches with a QJL sketch take the dense route there)
@@ -196,6 +219,7 @@ class GraphedDecoder:
     ``model(tok, cache=caches, packed=True)``.
     """
 
+    @torch.no_grad()
     def __init__(self, model: LlamaShaped, caches: list, first_tokens: torch.Tensor):
         a = model.args
         self.model, self.caches = model, caches
@@ -211,12 +235,14 @@ class GraphedDecoder:
         self.attn = torch.zeros(B, hq, 1, d, dtype=dt, device=dev)
         half = d // 2
         self._inv = a.rope_theta ** (-torch.arange(0, half, device=dev, dtype=torch.float32) / half)
+        self._rotary = a.rotary_frequencies(dev) if a.rotary_kernel else None
+        self._pos64 = torch.full((1,), int(caches[0].offset), dtype=torch.int64, device=dev)
         n = len(model.layers)
         pieces = [self._piece(i) for i in range(n + 1)]
         # warm up on a side stream (library handles, autotuning), then capture each piece
         side = torch.cuda.Stream(device=dev)
         side.wait_stream(torch.cuda.current_stream(dev))
-        saved = (self.tok.clone(), self.pos.clone())
+        saved = (self.tok.clone(), self.pos.clone(), self._pos64.clone())
         with torch.cuda.stream(side):
             for _ in range(2):
                 for f in pieces:
@@ -232,6 +258,7 @@ class GraphedDecoder:
             self.graphs.append(g)
         self.tok.copy_(saved[0])
         self.pos.copy_(saved[1])
+        self._pos64.copy_(saved[2])
 
     def _pre_attention(self, i: int, h: torch.Tensor) -> None:
         m, a = self.model, self.model.args
@@ -239,6 +266,12 @@ class GraphedDecoder:
         hq, hkv, d = att.n_heads, att.n_kv_heads, att.head_dim
         B = h.shape[0]
         qkv = att.qkv_proj(_rms_norm(h, m.layers[i].input_layernorm, a.rms_norm_eps)).view(B, 1, hq + 2 * hkv, d).transpose(1, 2)
+        if self._rotary is not None:
+            q, k = rotary.apply_rotary(qkv[:, :hq], qkv[:, hq:hq + hkv], self._rotary[0], positions=self._pos64, interleaved=a.rope_traditional, factor=self._rotary[1])
+            self.q.copy_(q)
+            self.k.copy_(k)
+            self.v.copy_(qkv[:, hq + hkv:])
+            return
         ang = self.pos[:, None] * self._inv[None, :]                                  # (1, d/2): this step's position
         cos, sin = ang.cos(), ang.sin()
         qk = apply_rope(qkv[:, :hq + hkv], (torch.cat([cos, cos], dim=-1), torch.cat([-sin, sin], dim=-1)))
@@ -272,6 +305,8 @@ class GraphedDecoder:
             logits = m.lm_head(_rms_norm(h, m.norm, m.args.rms_norm_eps))
             self.tok.copy_(logits[:, -1].argmax(-1, keepdim=True))
             self.pos.add_(1.0)
+            if self._rotary is not None:
+                self._pos64.add_(1)
 
         return first if i == 0 else last if i == n else middle
 

@@ -91,6 +91,13 @@ struct Params {
     int* status;
 };
 
+__device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+                 : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+    return ok != 0;
+}
+
 // Sixteen codes as the two 16-byte chunks of an fp16 operand row
 __device__ __forceinline__ void expand16(uint4 raw, int e4m3, uint4& lo, uint4& hi) {
     if (e4m3) {

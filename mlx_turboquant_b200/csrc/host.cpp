@@ -425,10 +425,10 @@ PyObject* blocks_read(PyObject*, PyObject* const* a, Py_ssize_t n) {
     return PyTuple_Pack(2, THPObjectPtr(THPVariable_Wrap(k)).get(), THPObjectPtr(THPVariable_Wrap(v)).get());
     END_HANDLE_TH_ERRORS
 }
-// blocks_attend(queries, storage x 6, length, window or 0, sinks, scale or None, new keys or None, new values or None) -> result
+// blocks_attend(queries, storage x 6, length, window or 0, sinks, scale or None, new keys or None, new values or None, out or None) -> result
 PyObject* blocks_attend(PyObject*, PyObject* const* a, Py_ssize_t n) {
     HANDLE_TH_ERRORS
-    if (n != 13 || !is_tensor(a[0]) || !PyLong_Check(a[7]) || !PyLong_Check(a[8]) || !PyLong_Check(a[9])) return none();
+    if (n != 14 || !is_tensor(a[0]) || !PyLong_Check(a[7]) || !PyLong_Check(a[8]) || !PyLong_Check(a[9])) return none();
     const int device = c10::cuda::current_device();
     const at::Tensor& q = tensor(a[0]);
     tq_blocks_attend_args r;
@@ -446,7 +446,14 @@ PyObject* blocks_attend(PyObject*, PyObject* const* a, Py_ssize_t n) {
     int64_t t = 0;
     if (a[11] != Py_None && (r.t_q != 1 || length % s.block + 1 == s.block || !new_rows(a[11], a[12], tensor(a[5]), device, r.k_new, r.v_new, t) || t != 1)) return none();
     if (r.window < 0 || r.sinks < 0 || r.t_q > length + t) return none();
-    at::Tensor out = empty(q.sizes(), q.scalar_type(), device), ws;
+    at::Tensor out, ws;
+    if (a[13] == Py_None) {
+        out = empty(q.sizes(), q.scalar_type(), device);
+    } else {
+        if (!is_tensor(a[13])) return none();
+        out = tensor(a[13]);
+        if (!here(out, device) || out.sizes() != q.sizes() || out.scalar_type() != q.scalar_type() || !out.is_contiguous() || reinterpret_cast<uintptr_t>(out.data_ptr()) % 16) return none();
+    }
     r.out = out.data_ptr();
     r.workspace_bytes = tq_blocks_attend_workspace(&r);
     if (r.workspace_bytes) {
@@ -458,7 +465,12 @@ PyObject* blocks_attend(PyObject*, PyObject* const* a, Py_ssize_t n) {
         Release gil;
         rc = tq_blocks_attend(&r, stream_of(device));
     }
-    return rc ? status(rc) : THPVariable_Wrap(out);
+    if (rc) return status(rc);
+    if (a[13] != Py_None) {
+        Py_INCREF(a[13]);
+        return a[13];
+    }
+    return THPVariable_Wrap(out);
     END_HANDLE_TH_ERRORS
 }
 

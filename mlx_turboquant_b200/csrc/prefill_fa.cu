@@ -101,6 +101,13 @@ struct Params {
     int* status;
 };
 
+__device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+                 : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+    return ok != 0;
+}
+
 template <int D>
 __global__ void __launch_bounds__(Plan<D>::NT, 1) fa_kernel(const __grid_constant__ Params p, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,
                                                          const __grid_constant__ CUtensorMap qmap_rot, const __grid_constant__ CUtensorMap qmap_raw) {

@@ -12,6 +12,7 @@ import warnings
 
 import torch
 
+from .blocks import BlockKVCache
 from .cache import TurboQuantKVCache
 
 
@@ -144,12 +145,17 @@ def _is_sliding_window_cache(c) -> bool:
 def apply_turboquant(model, key_bits: float = 4, value_bits: float = 2, residual_window: int = 128,
                      head_dim: int | None = None, num_kv_heads: int | None = None, num_layers: int | None = None,
                      rotation_seed: int = 42, skip_layers: list[int] | None = None, auto_detect_outliers: bool = True,
-                     fp16_sink_size: int = 0, chunk_size: int = 0, qjl_correction: bool = False, qjl_n_proj: int = 32):
+                     fp16_sink_size: int = 0, chunk_size: int = 0, qjl_correction: bool = False, qjl_n_proj: int = 32,
+                     block_cache: str | None = None):
     """Make ``model.make_cache()`` return TurboQuant caches (patch.py:136-371); returns the same model.
 
     Arguments and defaults are the reference's.  Layers listed in ``skip_layers`` (or auto-detected as
     outliers), linear-attention layers and sliding-window layers keep an uncompressed / model-default cache.
+    With ``block_cache`` ("int8" or "e4m3"; new here) skipped layers and outliers get an 8-bit ``BlockKVCache``, and so do sliding-window
+    layers whose default cache says how long the window is (``max_size``, and ``keep`` first tokens).
     """
+    if block_cache not in (None, "int8", "e4m3"):
+        raise ValueError(f"block_cache must be 'int8', 'e4m3' or None, got {block_cache!r}")
     config = _get_model_config(model)
     hd = head_dim or config["head_dim"]
     nkv = num_kv_heads or config["num_kv_heads"]
@@ -193,10 +199,15 @@ def apply_turboquant(model, key_bits: float = 4, value_bits: float = 2, residual
         return [KVCache() for _ in range(nl)]
 
     swa_layers: set[int] = set()
+    windows: dict[int, tuple[int, int]] = {}         # (window, sinks) of the sliding-window layers that get block caches
     try:
         for i, c in enumerate(_build_default_caches()):
             if i not in linear_attn_layers and _is_sliding_window_cache(c):
-                swa_layers.add(i)
+                size, keep = getattr(c, "max_size", None), int(getattr(c, "keep", 0) or 0)
+                if block_cache is not None and isinstance(size, int) and size > keep:
+                    windows[i] = (size - keep, keep)     # (the kept tokens are part of the size)
+                else:
+                    swa_layers.add(i)
     except Exception:
         pass
     if swa_layers:
@@ -211,8 +222,10 @@ def apply_turboquant(model, key_bits: float = 4, value_bits: float = 2, residual
         for i in range(nl):
             if i in default_cache_layers:
                 caches.append(defaults[i])
+            elif i in windows:
+                caches.append(BlockKVCache(head_dim=hd, num_kv_heads=nkv, codes=block_cache, window=windows[i][0], sinks=windows[i][1]))
             elif i in layers_to_skip:
-                caches.append(KVCache())
+                caches.append(KVCache() if block_cache is None else BlockKVCache(head_dim=hd, num_kv_heads=nkv, codes=block_cache))
             else:
                 caches.append(TurboQuantKVCache(
                     head_dim=hd, num_kv_heads=nkv, key_bits=key_bits, value_bits=value_bits,
@@ -226,6 +239,8 @@ def apply_turboquant(model, key_bits: float = 4, value_bits: float = 2, residual
         "residual_window": residual_window, "fp16_sink_size": fp16_sink_size, "chunk_size": chunk_size,
         "qjl_correction": qjl_correction, "qjl_n_proj": qjl_n_proj,
     }
+    if block_cache is not None:
+        model._turboquant_config["block_cache"] = block_cache
     return model
 
 
