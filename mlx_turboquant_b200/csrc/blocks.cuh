@@ -36,6 +36,7 @@ struct BlockAttendParams {
 };
 
 int launch_blocks_plain(const BlockAttendParams& p, cudaStream_t s);
+double blocks_split_us(const BlockAttendParams& p);      // what a call is expected to cost in blocks_attend.cu's kernel
 bool blocks_fa_takes(const BlockAttendParams& p);
 size_t blocks_fa_workspace(const BlockAttendParams& p);
 int launch_blocks_fa(const BlockAttendParams& p, cudaStream_t s);

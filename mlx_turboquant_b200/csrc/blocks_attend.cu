@@ -104,6 +104,7 @@ struct AttendGrid {
     int cluster;                                       // CTAs of a (lane, group) that join their sums over distributed shared memory; 0: runs of tiles
     int merge;                                         // the merge kernel follows
     uint32_t per, jobs;                                // tiles of a CTA's run; lanes x groups
+    double us;                                         // what the call is expected to cost
 };
 
 // Which coordinates a lane's words are: a lane of t (keys) or g (values) holds 16-byte pieces of a row where the row has enough of them for all lanes, else parts of one.
@@ -683,6 +684,34 @@ template <int D> __global__ void __launch_bounds__(MG_T) blocks_merge_kernel(con
     *reinterpret_cast<uint2*>(dst) = p.dtype == TQ_BF16 ? make_uint2(pack_bf2(x.x * il, x.y * il), pack_bf2(x.z * il, x.w * il)) : make_uint2(pack_h2(x.x * il, x.y * il), pack_h2(x.z * il, x.w * il));
 }
 
+// How many clusters of each size the card holds at a time (a cluster lies within one group of SMs, so 148 SMs hold fewer of
+// six or seven CTAs than their number says).
+template <int D> int clusters_at_once(int size) {
+    using P = AttendPlan<D>;
+    static std::atomic<int> known[64][9];                  // (zero: not asked yet)
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) { cudaGetLastError(); return 0; }
+    int n = known[dev][size].load();
+    if (n != 0) return n;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = unsigned(size);
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(unsigned(size) * 512);
+    cfg.blockDim = dim3(AW * 32);
+    cfg.dynamicSmemBytes = P::SMEM;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    if (cudaFuncSetAttribute(blocks_attend_kernel<D, false, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, int(P::SMEM)) != cudaSuccess ||
+        cudaOccupancyMaxActiveClusters(&n, blocks_attend_kernel<D, false, false>, &cfg) != cudaSuccess || n <= 0) {
+        cudaGetLastError();
+        n = blocks_sm_count() * P::PER_SM / size;
+    }
+    known[dev][size].store(n);
+    return n;
+}
+
 template <int D> AttendGrid grid_of(const BlockAttendParams& p) {
     using P = AttendPlan<D>;
     const Visible v = visible_of(p.total, p.Tq, p.window, p.sinks);
@@ -696,20 +725,23 @@ template <int D> AttendGrid grid_of(const BlockAttendParams& p) {
     z.n_units = z.n_sink + z.n_win + (p.total - p.n8 + 15) / 16 - z.tail_unit;
     z.groups = int((int64_t(p.Tq) * p.G + HPG - 1) / HPG);
     const int64_t jobs = int64_t(p.B) * p.Hkv * z.groups, units = jobs * z.n_units, ctas = int64_t(blocks_sm_count()) * P::PER_SM;
-    if (units >= (int64_t(1) << 31) || jobs >= (int64_t(1) << 28)) { z.jobs = 0; return z; }
+    if (units >= (int64_t(1) << 31) || jobs >= (int64_t(1) << 28)) { z.jobs = 0; z.us = 1e30; return z; }
     z.jobs = uint32_t(jobs);
     z.per = uint32_t(std::max<int64_t>(AW, (units + ctas - 1) / ctas));
-    // A (lane, group) in one launch, by a cluster of up to eight CTAs, or runs of tiles over the whole card and a merge.  In us, from what calls of 8 to 512 lanes
-    // measured: a tile 0.05 with one CTA on an SM and 0.1 with two, a cluster's joining 1, the merge 4.
-    auto tile_us = [&](int64_t n) { return n * 2 > ctas ? 0.1 : 0.05; };
-    double best = double(z.per) * tile_us((units + z.per - 1) / z.per) + (z.per % uint32_t(z.n_units) ? 4.0 : 0.0);
-    for (int c = 1; c <= 8 && (c == 1 || c * AW <= z.n_units + AW - 1); ++c) {
-        const int64_t n = jobs * c;
-        const double us = double((n + ctas - 1) / ctas) * double((z.n_units + c - 1) / c) * tile_us(n) + (c > 1 ? 1.0 : 0.0);
-        if (us < best) { best = us; z.cluster = c; }
-    }
-    z.merge = !z.cluster && z.per % uint32_t(z.n_units) != 0;        // (otherwise every row has one CTA)
     z.slots = std::min((z.n_units - 2) / int(z.per) + 2, z.n_units);
+    z.merge = z.per % uint32_t(z.n_units) != 0;            // (otherwise every row has one CTA)
+    // A (lane, group) in one launch, by a cluster of up to eight CTAs, or runs of tiles over the whole card and a merge.  In us, fitted to 190 calls at d = 64, 128 and 256
+    // (8 to 256 lanes, 1 to 16 groups, 100 to 16,000 tokens; the choice is within 1% of the best on the mean, 20% at the worst): a tile at d = 128 0.15 with one CTA on an SM
+    // and 0.18 with two, a wave of CTAs 7, every further (lane, group) in a run 12, a cluster's joining 2.5, the merge 8 and 4 for every thousand partials.
+    const double width = D <= 64 ? 0.52 : D <= 96 ? 0.76 : D <= 128 ? 1.0 : 1.3;
+    auto tile_us = [&](int64_t n) { return width * (P::PER_SM == 2 && n * 2 > ctas ? 0.18 : 0.15); };
+    z.us = double(z.per) * tile_us((units + z.per - 1) / z.per) + 7.0 + 12.0 * std::max(0.0, double(z.per) / z.n_units - 0.5) + (z.merge ? 8.0 + 0.004 * double(jobs) * z.slots : 0.0);
+    for (int c = 1; c <= 8 && (c == 1 || c * AW <= z.n_units + AW - 1); ++c) {
+        const int64_t n = c == 1 ? ctas : clusters_at_once<D>(c);
+        if (n <= 0) continue;
+        const double us = double((jobs + n - 1) / n) * (double((z.n_units + c - 1) / c) * tile_us(jobs * c) + 7.0) + (c > 1 ? 2.5 : 0.0);
+        if (us < z.us) { z.us = us; z.cluster = c; z.merge = 0; }
+    }
     return z;
 }
 template <int D> size_t split_workspace(const BlockAttendParams& p) {
@@ -806,6 +838,8 @@ size_t workspace_of(const BlockAttendParams& p) {
 }
 
 }  // namespace
+
+double blocks_split_us(const BlockAttendParams& p) { return p.D == 64 ? grid_of<64>(p).us : p.D == 96 ? grid_of<96>(p).us : p.D == 128 ? grid_of<128>(p).us : grid_of<256>(p).us; }
 
 int launch_blocks_plain(const BlockAttendParams& p, cudaStream_t s) {
     const int64_t rows = int64_t(p.B) * p.Hq * p.Tq;

@@ -272,29 +272,59 @@ __global__ void __launch_bounds__(Plan<D, FUSED>::NT, 1) blocks_fa_kernel(const 
                         if (more) fetch(next, u);
                     }
                     if (more) fetch_scales(next);
-                } else if (ct < TN) {
-                    // a thread per token: 16-bit rows, bfloat16 ones under their power of two
-                    const int tok = base_of(i) + ct;
-                    const bool in = tok < c.total, bf = c.dtype == TQ_BF16;
-                    const int64_t at = (lane_c * c.block + (tok - c.n8)) * D;
-                    const uint4* src = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(side ? c.vt : c.kt) + at);
-                    const uint4* values = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(c.vt) + at);
-                    uint32_t mx = 0, mv = 0;
-                    if (in) {
-#pragma unroll 4
-                        for (int x = 0; x < D / 8; ++x) { mx = max(mx, largest16(src[x])); mv = max(mv, largest16(values[x])); }
+                } else {
+                    // 16-bit rows, bfloat16 ones under their power of two: half a warp per token, four tokens at a time.  (A thread per token took 7 us a tile.)
+                    const int base = base_of(i), half = ct >> 4, l16 = ct & 15;
+                    const bool bf = c.dtype == TQ_BF16;
+                    constexpr int V = D > 128 ? 2 : 1;
+                    const uint16_t* const rows = static_cast<const uint16_t*>(side ? c.vt : c.kt) + lane_c * c.block * D;
+                    const uint16_t* const value_rows = static_cast<const uint16_t*>(c.vt) + lane_c * c.block * D;
+#pragma unroll 1
+                    for (int u0 = 0; u0 < TN / 8; u0 += 4) {
+                        uint4 x[4][V];
+                        uint32_t mx[4], mv[4];
+#pragma unroll
+                        for (int u = 0; u < 4; ++u) {
+                            const int tok = base + half + 8 * (u0 + u);
+                            mx[u] = mv[u] = 0;
+#pragma unroll
+                            for (int w = 0; w < V; ++w) {
+                                x[u][w] = make_uint4(0u, 0u, 0u, 0u);
+                                if (tok < c.total && l16 + 16 * w < D / 8) {
+                                    const int64_t at = int64_t(tok - c.n8) * D + (l16 + 16 * w) * 8;
+                                    x[u][w] = *reinterpret_cast<const uint4*>(rows + at);
+                                    if (!side) mv[u] = max(mv[u], largest16(*reinterpret_cast<const uint4*>(value_rows + at)));
+                                }
+                            }
+                        }
+#pragma unroll
+                        for (int u = 0; u < 4; ++u) {
+                            const int row = half + 8 * (u0 + u);
+                            const bool in = base + row < c.total;
+#pragma unroll
+                            for (int w = 0; w < V; ++w) mx[u] = max(mx[u], largest16(x[u][w]));
+                            if (side) mv[u] = mx[u];
+#pragma unroll
+                            for (int off = 1; off < 16; off <<= 1) {
+                                mx[u] = max(mx[u], __shfl_xor_sync(0xffffffffu, mx[u], off));
+                                mv[u] = max(mv[u], __shfl_xor_sync(0xffffffffu, mv[u], off));
+                            }
+                            const float f = bf ? stage_scale(mx[u] << 16) : 1.f;
+                            const bool fine = mv[u] < (bf ? 0x7f80u : 0x7c00u);
+#pragma unroll
+                            for (int w = 0; w < V; ++w) {
+                                if (l16 + 16 * w >= D / 8) continue;
+                                uint4 y = bf ? bf_to_half(x[u][w], f) : x[u][w];
+                                if (side && !fine) y = make_uint4(0u, 0u, 0u, 0u);
+                                st_shared(tile + chunk_place(row, l16 + 16 * w), y);
+                            }
+                            if (l16 == 0)
+                                reinterpret_cast<float*>(smem + P::OFF_SC + s * P::SC)[side * TN + row] =
+                                    !in ? 0.f : side ? (fine ? 1.f / f : 0.f) : (fine ? c.scale_log2 / f : __uint_as_float(0x7fffffffu));
+                        }
                     }
-                    const float f = bf ? stage_scale(mx << 16) : 1.f;
-                    const bool fine = mv < (bf ? 0x7f80u : 0x7c00u);
-#pragma unroll 4
-                    for (int x = 0; x < D / 8; ++x) {
-                        uint4 w = make_uint4(0u, 0u, 0u, 0u);
-                        if (in && (fine || !side)) w = bf ? bf_to_half(src[x], f) : src[x];
-                        st_shared(tile + chunk_place(ct, x), w);
-                    }
-                    v = !in ? 0.f : side ? (fine ? 1.f / f : 0.f) : (fine ? c.scale_log2 / f : __uint_as_float(0x7fffffffu));
                 }
-                if (ct < TN) reinterpret_cast<float*>(smem + P::OFF_SC + s * P::SC)[side * TN + ct] = v;
+                if (ct < TN && !sg.tiles.is_tail(sg.t_lo + i)) reinterpret_cast<float*>(smem + P::OFF_SC + s * P::SC)[side * TN + ct] = v;
                 if (side && ct == 0) *reinterpret_cast<int2*>(smem + P::OFF_SC + s * P::SC + 2 * TN * 4) = make_int2(base_of(i), sg.tiles.is_tail(sg.t_lo + i) ? c.total : c.n8);
                 fence_proxy_async();
                 mbar_arrive(bar(full + st));
@@ -387,15 +417,19 @@ __global__ void __launch_bounds__(Plan<D, FUSED>::NT, 1) blocks_fa_kernel(const 
                 const int gl = p.lane0 + sg.lane_c, b = gl / c.Hkv, h0 = (gl - b * c.Hkv) * c.G + sg.hg * HPG;
                 const uint16_t* src = static_cast<const uint16_t*>(c.q) + b * c.q_sb + int64_t(h0) * c.q_sh + int64_t(sg.tq0 + q * p.QT) * c.q_st;
                 constexpr int CPR = D / 8;                         // 16-byte chunks of a row
-#pragma unroll 1
-                for (int r0 = 0; r0 < 16; r0 += 8) {               // eight rows at a time: a row's chunks sit with neighbouring lanes of one load
-                    uint4 x[CPR / 4];
+                uint4 both[2][CPR / 4];                            // eight rows at a time: a row's chunks sit with neighbouring lanes of one load
 #pragma unroll
-                    for (int u = 0; u < CPR / 4; ++u) {            // lane = row r0 + (lane >> 2), chunk 4 u + (lane & 3)
-                        const int m = m0 + r0 + (lane >> 2);
-                        x[u] = make_uint4(0u, 0u, 0u, 0u);
-                        if (valid(m)) x[u] = *reinterpret_cast<const uint4*>(src + (m & (p.GP - 1)) * c.q_sh + int64_t(m >> gp_bits) * c.q_st + (4 * u + (lane & 3)) * 8);
+                for (int e = 0; e < 2; ++e)
+#pragma unroll
+                    for (int u = 0; u < CPR / 4; ++u) {            // lane = row 8 e + (lane >> 2), chunk 4 u + (lane & 3)
+                        const int m = m0 + 8 * e + (lane >> 2);
+                        both[e][u] = make_uint4(0u, 0u, 0u, 0u);
+                        if (valid(m)) both[e][u] = *reinterpret_cast<const uint4*>(src + (m & (p.GP - 1)) * c.q_sh + int64_t(m >> gp_bits) * c.q_st + (4 * u + (lane & 3)) * 8);
                     }
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const int r0 = 8 * e;
+                    uint4 (&x)[CPR / 4] = both[e];
                     if (c.dtype == TQ_BF16) {
                         uint32_t mx = 0;
 #pragma unroll
@@ -406,7 +440,7 @@ __global__ void __launch_bounds__(Plan<D, FUSED>::NT, 1) blocks_fa_kernel(const 
                         const float f = big >= 0.0078125f && big < 32768.f ? 1.f : stage_scale(mx << 16);
 #pragma unroll
                         for (int u = 0; u < CPR / 4; ++u) x[u] = bf_to_half(x[u], f);
-                        row_mul[r0 >> 3] = 1.f / f;
+                        row_mul[e] = 1.f / f;
                         scaled = scaled || __any_sync(0xffffffffu, f != 1.f);
                     }
 #pragma unroll
@@ -716,30 +750,38 @@ template <int D> __global__ void __launch_bounds__(EX_T) blocks_fa_expand_kernel
             *reinterpret_cast<uint4*>(dst + chunk_place(row, 2 * cc + 1)) = hi;
         }
     } else {
-        // a warp per token
+        // a warp per token, four at a time
         const int lane_t = tid & 31;
-        const bool bf = c.dtype == TQ_BF16;
-        for (int r = tid >> 5; r < TN; r += EX_T / 32) {
-            const int tok = base + r;
-            const bool in = tok < c.total, mine = lane_t < D / 8;
-            const int64_t src = (lane * c.block + (tok - c.n8)) * D + lane_t * 8;
-            uint4 k = make_uint4(0u, 0u, 0u, 0u), v = k;
-            if (in && mine) {
-                k = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(c.kt) + src);
-                v = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(c.vt) + src);
+        const bool bf = c.dtype == TQ_BF16, mine = lane_t < D / 8;
+        for (int r0 = tid >> 5; r0 < TN; r0 += 4 * EX_T / 32) {
+            uint4 k[4], v[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                const int tok = base + r0 + u * (EX_T / 32);
+                k[u] = v[u] = make_uint4(0u, 0u, 0u, 0u);
+                if (tok < c.total && mine) {
+                    const int64_t src = (lane * c.block + (tok - c.n8)) * D + lane_t * 8;
+                    k[u] = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(c.kt) + src);
+                    v[u] = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(c.vt) + src);
+                }
             }
-            const uint32_t mk = __reduce_max_sync(0xffffffffu, largest16(k)), mv = __reduce_max_sync(0xffffffffu, largest16(v));
-            const bool fine = mv < (bf ? 0x7f80u : 0x7c00u);
-            const float fk = bf ? stage_scale(mk << 16) : 1.f, fv = bf ? stage_scale(mv << 16) : 1.f;
-            if (bf) { k = bf_to_half(k, fk); v = bf_to_half(v, fv); }
-            if (!fine) v = make_uint4(0u, 0u, 0u, 0u);
-            if (mine) {
-                *reinterpret_cast<uint4*>(tiles + chunk_place(r, lane_t)) = k;
-                *reinterpret_cast<uint4*>(tiles + K_TILE + chunk_place(r, lane_t)) = v;
-            }
-            if (lane_t == 0) {
-                scales[r] = !in ? 0.f : fine ? c.scale_log2 / fk : __uint_as_float(0x7fffffffu);
-                scales[TN + r] = in && fine ? 1.f / fv : 0.f;
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                const int r = r0 + u * (EX_T / 32);
+                const bool in = base + r < c.total;
+                const uint32_t mk = __reduce_max_sync(0xffffffffu, largest16(k[u])), mv = __reduce_max_sync(0xffffffffu, largest16(v[u]));
+                const bool fine = mv < (bf ? 0x7f80u : 0x7c00u);
+                const float fk = bf ? stage_scale(mk << 16) : 1.f, fv = bf ? stage_scale(mv << 16) : 1.f;
+                if (bf) { k[u] = bf_to_half(k[u], fk); v[u] = bf_to_half(v[u], fv); }
+                if (!fine) v[u] = make_uint4(0u, 0u, 0u, 0u);
+                if (mine) {
+                    *reinterpret_cast<uint4*>(tiles + chunk_place(r, lane_t)) = k[u];
+                    *reinterpret_cast<uint4*>(tiles + K_TILE + chunk_place(r, lane_t)) = v[u];
+                }
+                if (lane_t == 0) {
+                    scales[r] = !in ? 0.f : fine ? c.scale_log2 / fk : __uint_as_float(0x7fffffffu);
+                    scales[TN + r] = in && fine ? 1.f / fv : 0.f;
+                }
             }
         }
     }
@@ -802,9 +844,8 @@ template <int D, bool FUSED> Layout layout_of(const BlockAttendParams& p) {
 }
 
 // Runs of key tiles for the CTAs: where each one starts in the sequence of row blocks.  The row blocks of every (lane, head group) have the same tiles.  Either equal
-// runs, wherever that cuts a row block, or runs of whole row blocks.  A cut costs partials and their merge, 18 us and more where every CTA has one, or some
-// CUT tiles; whole row blocks cost what the longest run has more than the others.
-constexpr int CUT = 20;
+// runs, wherever that cuts a row block, or runs of whole row blocks.  A cut costs partials and their merge: 5 us and, where every CTA of 148 has two of 256 rows, d = 128,
+// 40 MB, 18 more; whole row blocks cost what the longest run has more than the others, a tile 1 us (fused) or 1.3 (two query tiles).
 template <int D, bool FUSED> void divide(Params& p, int lanes) {
     const BlockAttendParams& a = p.a;
     const int rows = Plan<D, FUSED>::NQ * p.QT, q0 = a.total - a.Tq;
@@ -838,7 +879,8 @@ template <int D, bool FUSED> void divide(Params& p, int lanes) {
         return longest;
     };
     const int64_t whole = fill(true);
-    if (whole > (total + most - 1) / most + CUT) fill(false);
+    const double cut_us = 5.0 + 0.45e-6 * double(most) * 2 * Plan<D, FUSED>::ROWS * (D + 4) * 4, tile_us = Plan<D, FUSED>::NQ == 1 ? 1.0 : 1.3;
+    if (double(whole - (total + most - 1) / most) * tile_us > cut_us) fill(false);
 }
 
 template <int D, bool FUSED> int launch(const BlockAttendParams& a, unsigned char* ws, cudaStream_t st) {
@@ -891,20 +933,51 @@ template <int D, bool FUSED> int launch(const BlockAttendParams& a, unsigned cha
     return TQ_OK;
 }
 
-// Whether the codes are converted in the attention kernel: one or two tiles of 128 query rows per lane and head group
-bool fused(const BlockAttendParams& p) {
-    const int g = std::min(p.G, HPG), gp = g <= 1 ? 1 : g <= 2 ? 2 : g <= 4 ? 4 : 8;
-    return int64_t(p.Tq) * gp <= 2 * TM;
+// What a call is expected to cost, in us, fitted to 300 calls (d = 64, 128 and 256; 8 to 128 lanes; 100 to 12,000 tokens; 8 to 1024 query rows a lane): set-up 13, a key
+// tile of a CTA's run 1.1 (fused) or 1.2 at d = 128, a cut 1.4 and the partials' bytes, for expanded tiles another launch and six bytes a coordinate, read and written.
+// Measured, fused / expanded, 4 heads on 1 at d = 128: 8 lanes x 12,000 tokens, 128 query rows a lane 35 / 52, 512 64 / 70, 1024 111 / 94; 64 lanes x 12,000, 256 rows
+// 220 / 235, 384 325 / 325, 512 425 / 336; 64 lanes x 700, 256 22 / 33, 1024 67 / 52.
+template <int D, bool FUSED> double cost(const BlockAttendParams& p) {
+    const Layout l = layout_of<D, FUSED>(p);
+    const int64_t lanes = int64_t(p.B) * p.Hkv, jobs = lanes * l.HG * l.n_blk, sms = blocks_sm_count();
+    const int rows = Plan<D, FUSED>::NQ * l.QT;
+    double n = 0;                                          // tiles of a row block, on the mean of the first and the last
+    for (int blk : {0, l.n_blk - 1}) n += 0.5 * Tiles(p, p.total - p.Tq + blk * rows, p.total - p.Tq + std::min((blk + 1) * rows, p.Tq) - 1).n;
+    const double tile = (FUSED ? 1.1 : 1.2) * (D <= 64 ? 0.84 : D <= 96 ? 0.92 : D <= 128 ? 1.0 : 0.92), runs = std::min(double(sms), double(jobs) * n / 4);
+    const double whole = double((jobs + sms - 1) / sms) * n * tile, cut = std::max(4.0, double(jobs) * n / double(sms)) * tile + 1.4 + 2.7e-7 * runs * 2 * Plan<D, FUSED>::ROWS * (D + 4) * 4;
+    return 13.0 + (runs < double(jobs) ? whole : std::min(whole, cut)) + (FUSED ? 0.0 : 2.2 + 1.9e-7 * double(lanes) * l.all.n * TN * 6 * D);
 }
-template <int D> size_t workspace(const BlockAttendParams& p) { return fused(p) ? layout_of<D, true>(p).bytes : layout_of<D, false>(p).bytes; }
-template <int D> int launch_any(const BlockAttendParams& p, unsigned char* ws, cudaStream_t s) { return fused(p) ? launch<D, true>(p, ws, s) : launch<D, false>(p, ws, s); }
+// Whether the codes are converted in the attention kernel (not at d = 256, where its eight converting warps cannot keep up: 3 times the other way's time).
+template <int D> bool fused(const BlockAttendParams& p) {
+    if constexpr (D > 128) return false;
+    else return cost<D, true>(p) <= cost<D, false>(p);
+}
+template <int D> double least(const BlockAttendParams& p) {
+    if constexpr (D > 128) return cost<D, false>(p);
+    else return std::min(cost<D, true>(p), cost<D, false>(p));
+}
+template <int D> size_t workspace(const BlockAttendParams& p) {
+    if constexpr (D <= 128)
+        if (fused<D>(p)) return layout_of<D, true>(p).bytes;
+    return layout_of<D, false>(p).bytes;
+}
+template <int D> int launch_any(const BlockAttendParams& p, unsigned char* ws, cudaStream_t s) {
+    if constexpr (D <= 128)
+        if (fused<D>(p)) return launch<D, true>(p, ws, s);
+    return launch<D, false>(p, ws, s);
+}
 
 }  // namespace bfa
 
-// Whether this kernel takes the call: enough query rows per KV head for tiles of 128 to be worth their set-up
+// Whether this kernel takes the call rather than blocks_attend.cu's, which reads the codes once for every eight query rows of a lane.  us measured, that one / this one,
+// 4 heads on 1 at d = 128: 8 lanes x 12,000 tokens, 32 rows a lane 25 / 33, 64 40 / 35, 128 66 / 35; 64 lanes x 12,000, 16 69 / 110, 32 122 / 118, 64 225 / 118; 64 lanes x 700,
+// 32 17 / 21, 64 31 / 21; 64 lanes x 100, 64 16 / 17, 128 30 / 17.  The choice among all the ways is within 1.4% of the best on the mean of the calls swept, 40% at the worst
+// (of 11 us).
 bool blocks_fa_takes(const BlockAttendParams& p) {
     if (p.dtype == TQ_F32 || (p.D != 64 && p.D != 96 && p.D != 128 && p.D != 256) || p.kn != nullptr) return false;
-    return int64_t(p.Tq) * p.G >= 64 && int64_t(p.B) * p.Hkv * p.G * p.Tq < (int64_t(1) << 29);
+    if (int64_t(p.Tq) * p.G <= HPG || int64_t(p.B) * p.Hkv * p.G * p.Tq >= (int64_t(1) << 29)) return false;
+    const double us = p.D == 64 ? bfa::least<64>(p) : p.D == 96 ? bfa::least<96>(p) : p.D == 128 ? bfa::least<128>(p) : bfa::least<256>(p);
+    return us < blocks_split_us(p);
 }
 size_t blocks_fa_workspace(const BlockAttendParams& p) {
     return p.D == 64 ? bfa::workspace<64>(p) : p.D == 96 ? bfa::workspace<96>(p) : p.D == 128 ? bfa::workspace<128>(p) : bfa::workspace<256>(p);

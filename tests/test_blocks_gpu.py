@@ -190,6 +190,62 @@ def test_pieces_of_a_prompt(d, codes, dtype):
     assert _lib.lib().tq_device_status() == 0
 
 
+def repeated(store, n):
+    return [x.repeat(n, *[1] * (x.dim() - 1)) for x in store]
+
+
+def check_repeated(q, store, n, kd, vd, total, kernel=None, **kw):
+    """n times the batch: every copy's results within the bounds, and by the kernel that is meant."""
+    from mlx_turboquant_b200 import blocks
+    got = None
+    with torch.profiler.profile(activities=[torch.profiler.ProfilerActivity.CUDA], acc_events=True) as p:
+        got = blocks.attend_blocks(q.repeat(n, 1, 1, 1), *store, total, **kw)
+        torch.cuda.synchronize()
+    names = " ".join(e.key for e in p.key_averages())
+    assert kernel is None or kernel in names, names
+    for x in got.chunk(n):
+        check_attention(x, q, kd, vd, q.shape[-1] ** -0.5, kw.get("window"), kw.get("sinks", 0))
+
+
+@pytest.mark.parametrize("d,codes,dtype", ((128, torch.int8, torch.bfloat16), (128, torch.float8_e4m3fn, torch.float16), (64, torch.float8_e4m3fn, torch.bfloat16), (96, torch.int8, torch.float16),
+                                           (256, torch.int8, torch.bfloat16)))
+def test_many_lanes_of_several_tokens(d, codes, dtype):
+    """What takes the tile products: row blocks that fill a tile in part, one to eight heads on a KV head and more, tails of every length, windows and sinks."""
+    for b, hq, h, total, t, n in ((1, 4, 1, 100, 60, 130), (1, 16, 2, 257, 33, 70), (2, 6, 2, 300, 130, 40), (1, 3, 3, 200, 200, 50), (1, 20, 2, 191, 17, 80), (1, 7, 1, 640, 64, 150)):
+        store = filled(b, h, total, d, 64, codes, dtype, seed=t)
+        q = rows(b, hq, t, d, dtype, 5, std=0)
+        kd, vd = dense(store, total)
+        many = repeated(store, n)
+        check_repeated(q, many, n, kd, vd, total, "blocks_fa")
+        for window, sinks in ((1, 0), (20, 3), (64, 70), (150, 4)):
+            check_repeated(q, many, n, kd, vd, total, window=window, sinks=sinks)
+
+
+@pytest.mark.parametrize("t", (40, 190))
+@pytest.mark.parametrize("dtype", (torch.float16, torch.bfloat16))
+def test_many_lanes_where_tokens_are_not_finite(dtype, t):
+    from mlx_turboquant_b200 import blocks
+    for total, at, side, bad in ((250, 247, 0, float("nan")), (250, 248, 1, float("nan")), (250, 246, 1, float("inf")), (200, 199, 1, float("-inf"))):
+        store, q = filled(1, 2, total, 64, 128, torch.int8, dtype, room=0), rows(1, 8, t, 64, dtype, 3, std=0)
+        kd, vd = dense(store, total)
+        store[4 + side][:, :, at - 128, 7] = bad
+        got = blocks.attend_blocks(q.repeat(64, 1, 1, 1), *repeated(store, 64), total)
+        first = t - (total - at)
+        for x in got.chunk(64):
+            check_attention(x[:, :, :first], q[:, :, :first], kd[:, :, :at], vd[:, :, :at], 0.125)
+            assert bool((~x[:, :, first:].isfinite()).any(-1).all())
+        # behind every query's window, or behind the last token
+        store = filled(1, 2, total, 64, 128, torch.int8, dtype, room=0)
+        ref = blocks.attend_blocks(q.repeat(64, 1, 1, 1), *repeated(store, 64), total, window=5)
+        low, cut = total - t + 1 - 5, 128
+        for x, s in ((store[4], store[1]), (store[5], store[3])):
+            x[:, :, total - cut:] = bad
+            x[:, :, :max(low - cut, 0)] = bad
+            if low >= cut:
+                s[:, :, 0] = float("nan")
+        assert torch.equal(blocks.attend_blocks(q.repeat(64, 1, 1, 1), *repeated(store, 64), total, window=5), ref)
+
+
 def test_query_magnitudes():
     """bfloat16 queries of very different rows, outside the fp16 range."""
     from mlx_turboquant_b200 import blocks
@@ -201,6 +257,8 @@ def test_query_magnitudes():
     for t in (1, 20, 200):
         q = (rows(1, 4, t, 128, torch.float32, 2, std=0) * torch.exp2(60 - 30 * torch.rand(1, 4, t, 1).cuda())).bfloat16()
         check_attention(blocks.attend_blocks(q, *store, 500), q, k, v, 128 ** -0.5)
+        if t > 1:
+            check_repeated(q, repeated(store, 150), 150, k, v, 500, "blocks_fa")
 
 
 @pytest.mark.parametrize("dtype", (torch.float16, torch.bfloat16, torch.float32))
