@@ -167,6 +167,12 @@ __global__ void __launch_bounds__(Plan<D, FUSED>::NT, 1) blocks_fa_kernel(const 
     };
     const int last_job = to.tile > 0 ? to.job : to.job - 1;
 
+    // registers for the softmax warps from the others: 640 x 96 at launch, 512 x 112 + 128 x 32 (spilled ones cost 3%)
+    if constexpr (NQ == 2) {
+        static_assert(P::SW * 32 == 512 && P::NT == 640, "warpgroups");
+        if (warp < P::SW) asm volatile("setmaxnreg.inc.sync.aligned.u32 112;");
+        else asm volatile("setmaxnreg.dec.sync.aligned.u32 32;");
+    }
     auto wait_bar = [&](int which, int phase) -> bool {
         const uint32_t addr = bar(which);
         for (uint32_t i = 0; i < WAIT_LIMIT; ++i) {
@@ -405,6 +411,7 @@ __global__ void __launch_bounds__(Plan<D, FUSED>::NT, 1) blocks_fa_kernel(const 
         int j = 0, seg = 0;
         float row_mul[2];                                          // one over the power of two that a query row was laid out under
         bool scaled = false;                                       // ... is not one for some row of the warp
+        const bool whole_blocks = c.block >= TN;
         // Query rows of a row block as K-major fp16 operands, by the warp that will hold their results.  (The products that read the rows before have ended:
         // the warp has seen the scores of the last tile.)  bfloat16 rows far from fp16's range under a power of two.
         auto lay_out = [&](const Segment& sg) -> bool {
@@ -488,43 +495,55 @@ __global__ void __launch_bounds__(Plan<D, FUSED>::NT, 1) blocks_fa_kernel(const 
             }
             // A row that has seen no token yet keeps m_ref = -1e30, has lvsc for a bias and asks for a reference at its first one.
             float vsc = 1.f, vthr = 0.f, lvsc = 0.f;               // (vthr 0: the first tile with a non-zero value scale picks the scale); log2(vsc)
-            float m_ref[2] = {-1e30f, -1e30f};
+            float m_ref[2] = {-1e30f, -1e30f}, bias[2] = {0.f, 0.f};       // bias = log2(vsc) - reference
+            float thr[2] = {pos[0] >= 0 ? -1.f : INFINITY, pos[1] >= 0 ? -1.f : INFINITY};       // a tile's sum above this asks for another reference; a row's first tile always does
             u64 l2[2] = {pk(0.f, 0.f), pk(0.f, 0.f)};              // this thread's share of the rows' sums
-            auto bias_of = [&](int k) { return m_ref[k] > -1e30f ? lvsc - m_ref[k] : lvsc; };
             for (int i = 0; i < n; ++i, ++j) {
                 const int s = j % NSC;
-                ok = wait_bar(SC_FULL + s, j / NSC) && wait_bar(S_FULL + sbuf(q, j), sph(j));
-                if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+                {
+                    const uint32_t sc_bar = bar(SC_FULL + s), s_bar = bar(S_FULL + sbuf(q, j)), sc_par = uint32_t(j / NSC) & 1u, s_par = uint32_t(sph(j)) & 1u;
+                    if (!__all_sync(0xffffffffu, mbar_try(s_bar, s_par) && mbar_try(sc_bar, sc_par))) {
+                        ok = wait_bar(S_FULL + sbuf(q, j), sph(j)) && wait_bar(SC_FULL + s, j / NSC);
+                        if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+                    }
+                }
                 tc_fence_after();
-                const int2 at_end = *reinterpret_cast<const int2*>(smem + P::OFF_SC + s * P::SC + 2 * TN * 4);
+                const float* sc = reinterpret_cast<const float*>(smem + P::OFF_SC + s * P::SC);
+                const int2 at_end = *reinterpret_cast<const int2*>(sc + 2 * TN);
                 const int base = at_end.x, end = at_end.y;         // (the tile's tokens lie before `end`)
-                const float* kn = reinterpret_cast<const float*>(smem + P::OFF_SC + s * P::SC) + t2;
-                const float* vn = kn + TN;
+                const float *kn = sc + t2, *vn = kn + TN;
+                const bool one = whole_blocks && end == c.n8;      // the tile's tokens share a block, and its scales
                 const uint32_t s_col = t_frag + sbuf(q, j) * TN;
                 constexpr int NR = TN / 8;
                 uint32_t v[4 * NR];                                // of eight columns: two of row g, two of row g + 8
                 tmem_ld_frag64(s_col, v);
+                const float k1 = sc[0], v1 = sc[TN];
                 u64 nv[NR];
+                if (!one) {
 #pragma unroll
-                for (int r = 0; r < NR; ++r) nv[r] = *reinterpret_cast<const u64*>(kn + 8 * r);
+                    for (int r = 0; r < NR; ++r) nv[r] = *reinterpret_cast<const u64*>(kn + 8 * r);
+                }
                 tmem_ld_wait();
                 if (scaled) {
 #pragma unroll
                     for (int r = 0; r < 4 * NR; ++r) v[r] = __float_as_uint(__uint_as_float(v[r]) * row_mul[(r >> 1) & 1]);
                 }
                 // t = score * key scale - reference + log2(value scale)
+                auto place = [&](auto scale_of) {
 #pragma unroll
-                for (int k = 0; k < 2; ++k) {
-                    uint32_t* x = v + 2 * k;
-                    const float bias = bias_of(k);
-                    const u64 b2 = pk(bias, bias);
+                    for (int k = 0; k < 2; ++k) {
+                        uint32_t* x = v + 2 * k;
+                        const u64 b2 = pk(bias[k], bias[k]);
 #pragma unroll
-                    for (int r = 0; r < NR; ++r) {
-                        float x0, x1;
-                        upk(fma2(pk(__uint_as_float(x[4 * r]), __uint_as_float(x[4 * r + 1])), nv[r], b2), x0, x1);
-                        x[4 * r] = __float_as_uint(x0); x[4 * r + 1] = __float_as_uint(x1);
+                        for (int r = 0; r < NR; ++r) {
+                            float x0, x1;
+                            upk(fma2(pk(__uint_as_float(x[4 * r]), __uint_as_float(x[4 * r + 1])), scale_of(r), b2), x0, x1);
+                            x[4 * r] = __float_as_uint(x0); x[4 * r + 1] = __float_as_uint(x1);
+                        }
                     }
-                }
+                };
+                if (one) place([&](int) { return pk(k1, k1); });
+                else place([&](int r) { return nv[r]; });
                 if (base + TN - 1 > min(tile_first, end - 1) || (base < tile_lo && base + TN > c.sinks)) {      // some token of the tile is hidden from some row
 #pragma unroll
                     for (int k = 0; k < 2; ++k) {
@@ -540,14 +559,16 @@ __global__ void __launch_bounds__(Plan<D, FUSED>::NT, 1) blocks_fa_kernel(const 
                 // Weights, their sums, P = weight * value scale (both carry vsc) as fp16.  A row needs another reference when a weight exceeds
                 // 2^MAX_SLACK, which its sum then does too: the sums are looked at behind the exponentials and no maximum is taken in the common case.
                 // The lanes share the check of the tile's value scales, eight tokens' pairs each.
-                const float2 v2 = *reinterpret_cast<const float2*>(vn + 8 * g);
-                float vmax = fmaxf(v2.x, v2.y);
+                float vmax = v1;
+                if (!one) {
+                    const float2 v2 = *reinterpret_cast<const float2*>(vn + 8 * g);
+                    vmax = fmaxf(v2.x, v2.y);
 #pragma unroll
-                for (int r = 0; r < NR; ++r) nv[r] = *reinterpret_cast<const u64*>(vn + 8 * r);
+                    for (int r = 0; r < NR; ++r) nv[r] = *reinterpret_cast<const u64*>(vn + 8 * r);
+                }
                 uint32_t w[2 * NR];
                 u64 ls[2];
-#pragma unroll 1
-                for (int pass = 0;; ++pass) {
+                auto weigh = [&](auto scale_of) {
                     ls[0] = ls[1] = pk(0.f, 0.f);
 #pragma unroll
                     for (int r = 0; r < NR; ++r)
@@ -556,20 +577,25 @@ __global__ void __launch_bounds__(Plan<D, FUSED>::NT, 1) blocks_fa_kernel(const 
                             const u64 x = pk(ex2(__uint_as_float(v[4 * r + 2 * k])), ex2(__uint_as_float(v[4 * r + 2 * k + 1])));
                             ls[k] = add2(ls[k], x);
                             float x0, x1;
-                            upk(mul2(x, nv[r]), x0, x1);
+                            upk(mul2(x, scale_of(r)), x0, x1);
                             w[2 * r + k] = pack_h2(x0, x1);
                         }
+                };
+#pragma unroll 1
+                for (int pass = 0;; ++pass) {
+                    if (one) weigh([&](int) { return pk(v1, v1); });
+                    else weigh([&](int r) { return nv[r]; });
                     bool again = vmax > vthr;
 #pragma unroll
                     for (int k = 0; k < 2; ++k) {
                         float x0, x1;
                         upk(ls[k], x0, x1);
-                        again = again || x0 + x1 > (m_ref[k] > -1e30f ? float(1 << int(MAX_SLACK)) * vsc : pos[k] >= base ? -1.f : INFINITY);      // (a row's first token: always)
+                        again = again || x0 + x1 > thr[k];
                     }
                     if (pass > 0 || !__any_sync(0xffffffffu, again)) break;
                     // Reference maximum / value scale: refreshed for the whole warp when any row needs it (rare after the first tile):
                     // the rows' sums and their O in tensor memory are rescaled.
-                    float a[2], bias[2] = {bias_of(0), bias_of(1)}, mx[2] = {-INFINITY, -INFINITY}, ratio = 1.f;
+                    float a[2], mx[2] = {-INFINITY, -INFINITY}, ratio = 1.f;
 #pragma unroll
                     for (int k = 0; k < 2; ++k) {
 #pragma unroll
@@ -593,7 +619,9 @@ __global__ void __launch_bounds__(Plan<D, FUSED>::NT, 1) blocks_fa_kernel(const 
                         const float mn = fmaxf(fmaxf(m_ref[k], mx[k] - bias[k]), -1e30f);
                         a[k] = ex2(m_ref[k] - mn) * ratio;
                         m_ref[k] = mn;
-                        const float delta = bias_of(k) - bias[k];
+                        const float moved = mn > -1e30f ? lvsc - mn : lvsc, delta = moved - bias[k];
+                        bias[k] = moved;
+                        if (mn > -1e30f) thr[k] = float(1 << int(MAX_SLACK)) * vsc;
                         l2[k] = mul2(l2[k], pk(a[k], a[k]));
                         uint32_t* x = v + 2 * k;
 #pragma unroll
