@@ -8,9 +8,7 @@
 //   * 8 NQ softmax warps, two rows' shares per thread: tcgen05.ld of the scores as fragments, one packed multiply-add each, ex2, P (fp16) back into tensor
 //     memory; a row's reference maximum is looked at through its sum.  They also lay out their rows of the queries, the next row block's before they write
 //     this one's results;
-//   * a warp per query tile issues S = Q K^T and O += P V, the next key tile's scores while the softmax works on this one's: they are free
-//     again as soon as they sit in registers, the weights have buffers of their own (in one place, with the weights over the scores, a warp waited 500 of 1960 clocks a
-//     tile for products that waited for weights);
+//   * a warp per query tile issues S = Q K^T and O += P V, scores two key tiles ahead;
 //   * keys and values as fp16 operands, by one of two ways:
 //     - expanded (NQ = 2; 1 at d = 256): blocks_fa_expand_kernel has written the tiles to workspace memory once, as they have to lie in shared memory, and two
 //       threads keep four tiles of each in flight (bulk copies).  What many row blocks share is converted once;
@@ -47,7 +45,7 @@ constexpr int TILE_INFO = 2 * TN + 4;                  // words that go with a t
 
 template <int D, bool FUSED> struct Plan {
     static constexpr int NQ = FUSED || D == 256 ? 1 : 2;       // query tiles per CTA
-    static constexpr int SP = 2 * TN;                  // tensor-memory columns of a query tile's scores (64) and of its weights as fp16 (two buffers of 32)
+    static constexpr int SB = 2;                       // score buffers per query tile
     static constexpr int ST = D == 256 ? 2 : 4;        // key tiles (and value tiles) in shared memory
     static constexpr int NBLK = (D + 63) / 64;         // 64-column blocks of a row
     static constexpr int DP = NBLK * 64;               // columns of O (d = 96: nobody reads the last 32)
@@ -60,12 +58,12 @@ template <int D, bool FUSED> struct Plan {
     static constexpr uint32_t OFF_BAR = OFF_SC + NSC * SC;
     static constexpr uint32_t OFF_SLOT = OFF_BAR + 8 * 48;                   // [0] tensor-memory base, [1] abort
     static constexpr size_t NEED = OFF_SLOT + 16 + 1024, SMEM = NEED > 116 * 1024 ? NEED : 116 * 1024;      // one CTA per SM: it takes all of the tensor memory
-    static constexpr uint32_t COL_O = NQ * SP;                               // scores and weights first, then the accumulators
+    static constexpr uint32_t COL_O = NQ * SB * TN;                          // scores first, then the accumulators
     static constexpr int ROWS = NQ * TM;               // of a row block
     static_assert(COL_O + NQ * DP <= 512, "tensor memory");
     static_assert(SMEM <= 227 * 1024, "shared memory");
 };
-enum Bars { K_FULL = 0, K_FREE = 4, V_FULL = 8, V_FREE = 12, SC_FULL = 16, SC_FREE = 24, S_FULL = 32, S_FREE = 34, P_FULL = 36, O_DONE = 40, ALL_DONE = 42, Q_FULL = 44, DRAIN = 46 };       // (48 of 8 bytes)
+enum Bars { K_FULL = 0, K_FREE = 4, V_FULL = 8, V_FREE = 12, SC_FULL = 16, SC_FREE = 24, S_FULL = 32, P_FULL = 36, O_DONE = 40, ALL_DONE = 42, Q_FULL = 44, DRAIN = 46 };       // (48 of 8 bytes)
 
 // The key tiles of a range of query positions, in their order: sinks, the window's in blocks, the tail's
 struct Tiles {
@@ -130,7 +128,7 @@ __device__ __forceinline__ bool finite_scale(float v) { return fabsf(v) <= 3.402
 template <int D, bool FUSED>
 __global__ void __launch_bounds__(Plan<D, FUSED>::NT, 1) blocks_fa_kernel(const __grid_constant__ Params p) {
     using P = Plan<D, FUSED>;
-    constexpr int NQ = P::NQ, DP = P::DP, ST = P::ST;
+    constexpr int NQ = P::NQ, DP = P::DP, SB = P::SB, ST = P::ST;
     extern __shared__ __align__(16) unsigned char smem_raw[];
     const uint32_t raw_addr = static_cast<uint32_t>(__cvta_generic_to_shared(smem_raw));
     const uint32_t sbase = (raw_addr + 1023u) & ~1023u;
@@ -144,9 +142,9 @@ __global__ void __launch_bounds__(Plan<D, FUSED>::NT, 1) blocks_fa_kernel(const 
     if (tid == 0) {
         for (int i = 0; i < 4; ++i) {
             mbar_init(bar(K_FULL + i), FUSED ? 128 : 1); mbar_init(bar(K_FREE + i), NQ); mbar_init(bar(V_FULL + i), FUSED ? 128 : 1); mbar_init(bar(V_FREE + i), NQ);
-            mbar_init(bar(P_FULL + i), 256);
+            mbar_init(bar(S_FULL + i), 1); mbar_init(bar(P_FULL + i), 256);
         }
-        for (int i = 0; i < 2; ++i) { mbar_init(bar(S_FULL + i), 1); mbar_init(bar(S_FREE + i), 256); mbar_init(bar(O_DONE + i), 1); mbar_init(bar(ALL_DONE + i), 1); mbar_init(bar(Q_FULL + i), 256); mbar_init(bar(DRAIN + i), 1); }
+        for (int i = 0; i < 2; ++i) { mbar_init(bar(O_DONE + i), 1); mbar_init(bar(ALL_DONE + i), 1); mbar_init(bar(Q_FULL + i), 256); mbar_init(bar(DRAIN + i), 1); }
         for (int i = 0; i < NSC; ++i) { mbar_init(bar(SC_FULL + i), FUSED ? 256 : 1); mbar_init(bar(SC_FREE + i), NQ * 256); }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         slot[1] = 0u;
@@ -194,10 +192,9 @@ __global__ void __launch_bounds__(Plan<D, FUSED>::NT, 1) blocks_fa_kernel(const 
     auto drain = [&](int which, int phase) {
         for (uint32_t i = 0; i < WAIT_LIMIT && !mbar_try(bar(which), uint32_t(phase & 1)); ++i) {}
     };
-    // weights' buffer of (query tile q, key tile j of the run): its barrier, its phase, its first column
-    auto pbuf = [](int q, int j) { return q * 2 + (j & 1); };
-    auto pph = [](int j) { return j >> 1; };
-    auto pcol = [](int q, int j) { return uint32_t(q * P::SP + TN + (j & 1) * (TN / 2)); };
+    // score buffer of (query tile q, key tile j of the run) and the phase of its barriers
+    auto sbuf = [](int q, int j) { return q * SB + j % SB; };
+    auto sph = [](int j) { return j / SB; };
 
     if (!FUSED && warp >= P::SW + NQ) {
         // ======================= expanded tiles: one thread the keys and scales, one the values =======================
@@ -370,16 +367,16 @@ __global__ void __launch_bounds__(Plan<D, FUSED>::NT, 1) blocks_fa_kernel(const 
         for (int job = from.job; job <= last_job && ok; ++job, ++seg) {
             const int n = uniform(segment(job).n);
             auto issue_qk = [&](int j) {                           // S = Q K^T of key tile j
-                const uint32_t s = tmem + q * P::SP;
+                const uint32_t s = tmem + sbuf(q, j) * TN;
 #pragma unroll
                 for (int ks = 0; ks < D / 16; ++ks)
                     umma_ss(s, desc_k(sbase + P::OFF_Q + q * P::Q_TILE, P::QBLK, ks), desc_k(sbase + P::OFF_K + (j % ST) * P::K_TILE, P::KBLK, ks),
                             idesc_of(TN, false), ks > 0 ? 1u : 0u);
-                umma_commit(bar(S_FULL + q));
+                umma_commit(bar(S_FULL + sbuf(q, j)));
                 umma_commit(bar(K_FREE + j % ST));
             };
             auto issue_pv = [&](int j) {                           // O += P V
-                const uint32_t a = tmem + pcol(q, j);
+                const uint32_t a = tmem + sbuf(q, j) * TN;
 #pragma unroll
                 for (int ks = 0; ks < TN / 16; ++ks)
                     umma_ts(tmem + P::COL_O + q * DP, a + ks * 8, desc_mn(sbase + P::OFF_V + (j % ST) * P::K_TILE, P::KBLK, ks), idesc_of(DP, true),
@@ -389,23 +386,21 @@ __global__ void __launch_bounds__(Plan<D, FUSED>::NT, 1) blocks_fa_kernel(const 
                 if (j == j0 + n - 1) umma_commit(bar(ALL_DONE + q));       // (a barrier of its own: a parity wait on O_DONE could be two phases early or one late)
             };
             ok = wait_one(Q_FULL + q, seg);
-            ok = ok && wait_one(K_FULL + j0 % ST, j0 / ST);
-            if (!ok) break;
-            tc_fence_after();
-            any = true;
-            issue_qk(j0);
-            for (int j = j0; j < j0 + n && ok; ++j) {
-                const int jn = j + 1;
-                if (jn < j0 + n) {                                 // the next scores, once this tile's are in registers
-                    ok = wait_all(S_FREE + q, j, K_FULL + jn % ST, jn / ST, S_FREE + q, j);
-                    if (!ok) break;
-                    tc_fence_after();
-                    issue_qk(jn);
-                }
-                ok = wait_all(P_FULL + pbuf(q, j), pph(j), V_FULL + j % ST, j / ST, V_FULL + j % ST, j / ST);
+            for (int j = j0; j < j0 + min(n, SB) && ok; ++j) {
+                ok = wait_one(K_FULL + j % ST, j / ST);
                 if (!ok) break;
                 tc_fence_after();
-                issue_pv(j);                                       // (the tensor core takes one thread's products in order: scores j + 2 are full only behind these)
+                any = true;
+                issue_qk(j);
+            }
+            for (int j = j0; j < j0 + n && ok; ++j) {
+                const int jn = j + SB;                             // the key tile whose scores go where P of tile j sits now
+                const bool more = jn < j0 + n;
+                ok = wait_all(P_FULL + sbuf(q, j), sph(j), V_FULL + j % ST, j / ST, more ? K_FULL + jn % ST : P_FULL + sbuf(q, j), more ? jn / ST : sph(j));
+                if (!ok) break;
+                tc_fence_after();
+                issue_pv(j);
+                if (more) issue_qk(jn);                            // (the tensor core takes one thread's products in order)
             }
             j0 += n;
         }
@@ -485,10 +480,9 @@ __global__ void __launch_bounds__(Plan<D, FUSED>::NT, 1) blocks_fa_kernel(const 
                 // a warp without a row: the others' exponentials have the pipe to themselves.  (What it leaves in tensor memory meets rows that nobody reads.  A
                 // score buffer is full again only behind the products that every warp of the query tile has arrived for, so that no arrival is a phase early.)
                 for (int i = 0; i < n && ok; ++i, ++j) {
-                    ok = __all_sync(0xffffffffu, wait_bar(SC_FULL + j % NSC, j / NSC) && wait_bar(S_FULL + q, j));
+                    ok = __all_sync(0xffffffffu, wait_bar(SC_FULL + j % NSC, j / NSC) && wait_bar(S_FULL + sbuf(q, j), sph(j)));
                     if (!ok) break;
-                    mbar_arrive(bar(S_FREE + q));
-                    mbar_arrive(bar(P_FULL + pbuf(q, j)));
+                    mbar_arrive(bar(P_FULL + sbuf(q, j)));
                     mbar_arrive(bar(SC_FREE + j % NSC));
                 }
                 if (job < last_job && ok) enter(job + 1);
@@ -512,9 +506,9 @@ __global__ void __launch_bounds__(Plan<D, FUSED>::NT, 1) blocks_fa_kernel(const 
             for (int i = 0; i < n; ++i, ++j) {
                 const int s = j % NSC;
                 {
-                    const uint32_t sc_bar = bar(SC_FULL + s), s_bar = bar(S_FULL + q), sc_par = uint32_t(j / NSC) & 1u, s_par = uint32_t(j) & 1u;
+                    const uint32_t sc_bar = bar(SC_FULL + s), s_bar = bar(S_FULL + sbuf(q, j)), sc_par = uint32_t(j / NSC) & 1u, s_par = uint32_t(sph(j)) & 1u;
                     if (!__all_sync(0xffffffffu, mbar_try(s_bar, s_par) && mbar_try(sc_bar, sc_par))) {
-                        ok = wait_bar(S_FULL + q, j) && wait_bar(SC_FULL + s, j / NSC);
+                        ok = wait_bar(S_FULL + sbuf(q, j), sph(j)) && wait_bar(SC_FULL + s, j / NSC);
                         if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
                     }
                 }
@@ -524,7 +518,7 @@ __global__ void __launch_bounds__(Plan<D, FUSED>::NT, 1) blocks_fa_kernel(const 
                 const int base = at_end.x, end = at_end.y;         // (the tile's tokens lie before `end`)
                 const float *kn = sc + t2, *vn = kn + TN;
                 const bool one = whole_blocks && end == c.n8;      // the tile's tokens share a block, and its scales
-                const uint32_t s_col = t_frag + q * P::SP;
+                const uint32_t s_col = t_frag + sbuf(q, j) * TN;
                 constexpr int NR = TN / 8;
                 uint32_t v[4 * NR];                                // of eight columns: two of row g, two of row g + 8
                 tmem_ld_frag64(s_col, v);
@@ -535,8 +529,6 @@ __global__ void __launch_bounds__(Plan<D, FUSED>::NT, 1) blocks_fa_kernel(const 
                     for (int r = 0; r < NR; ++r) nv[r] = *reinterpret_cast<const u64*>(kn + 8 * r);
                 }
                 tmem_ld_wait();
-                tc_fence_before();
-                mbar_arrive(bar(S_FREE + q));
                 if (scaled) {
 #pragma unroll
                     for (int r = 0; r < 4 * NR; ++r) v[r] = __float_as_uint(__uint_as_float(v[r]) * row_mul[(r >> 1) & 1]);
@@ -662,10 +654,10 @@ __global__ void __launch_bounds__(Plan<D, FUSED>::NT, 1) blocks_fa_kernel(const 
                 if (!ok) break;
                 l2[0] = add2(l2[0], ls[0]);
                 l2[1] = add2(l2[1], ls[1]);
-                tmem_st_half64(t_frag + pcol(q, j), w);
+                tmem_st_half64(s_col, w);
                 tmem_st_wait();
                 tc_fence_before();
-                mbar_arrive(bar(P_FULL + pbuf(q, j)));
+                mbar_arrive(bar(P_FULL + sbuf(q, j)));
                 mbar_arrive(bar(SC_FREE + s));
             }
             if (!ok) break;
@@ -975,16 +967,16 @@ template <int D, bool FUSED> int launch(const BlockAttendParams& a, unsigned cha
 }
 
 // What a call is expected to cost, in us, fitted to 300 calls (d = 64, 128 and 256; 8 to 128 lanes; 100 to 12,000 tokens; 8 to 1024 query rows a lane): set-up 13, a key
-// tile of a CTA's run 1.1 (fused) or 1.2 at d = 128, a cut 1.4 and the partials' bytes, for expanded tiles another launch and six bytes a coordinate, read and written.
-// Measured, fused / expanded, 4 heads on 1 at d = 128: 8 lanes x 12,000 tokens, 128 query rows a lane 35 / 52, 512 64 / 70, 1024 111 / 94; 64 lanes x 12,000, 256 rows
-// 220 / 235, 384 325 / 325, 512 425 / 336; 64 lanes x 700, 256 22 / 33, 1024 67 / 52.
+// tile of a CTA's run 1.25 (fused) or 1.1 at d = 128, a cut 1.4 and the partials' bytes, for expanded tiles another launch and six bytes a coordinate, read and written.
+// Measured, fused / expanded, 4 heads on 1 at d = 128: 8 lanes x 12,000 tokens, 128 query rows a lane 36 / 52, 512 64 / 68, 1024 109 / 87; 64 lanes x 12,000, 256 rows
+// 257 / 262, 384 378 / 341, 512 444 / 329; 64 lanes x 700, 256 22 / 33, 1024 70 / 51.
 template <int D, bool FUSED> double cost(const BlockAttendParams& p) {
     const Layout l = layout_of<D, FUSED>(p);
     const int64_t lanes = int64_t(p.B) * p.Hkv, jobs = lanes * l.HG * l.n_blk, sms = blocks_sm_count();
     const int rows = Plan<D, FUSED>::NQ * l.QT;
     double n = 0;                                          // tiles of a row block, on the mean of the first and the last
     for (int blk : {0, l.n_blk - 1}) n += 0.5 * Tiles(p, p.total - p.Tq + blk * rows, p.total - p.Tq + std::min((blk + 1) * rows, p.Tq) - 1).n;
-    const double tile = (FUSED ? 1.1 : 1.2) * (D <= 64 ? 0.84 : D <= 96 ? 0.92 : D <= 128 ? 1.0 : 0.92), runs = std::min(double(sms), double(jobs) * n / 4);
+    const double tile = (FUSED ? 1.25 : 1.1) * (D <= 64 ? 0.84 : D <= 96 ? 0.92 : D <= 128 ? 1.0 : 0.92), runs = std::min(double(sms), double(jobs) * n / 4);
     const double whole = double((jobs + sms - 1) / sms) * n * tile, cut = std::max(4.0, double(jobs) * n / double(sms)) * tile + 1.4 + 2.7e-7 * runs * 2 * Plan<D, FUSED>::ROWS * (D + 4) * 4;
     return 13.0 + (runs < double(jobs) ? whole : std::min(whole, cut)) + (FUSED ? 0.0 : 2.2 + 1.9e-7 * double(lanes) * l.all.n * TN * 6 * D);
 }
@@ -1011,8 +1003,8 @@ template <int D> int launch_any(const BlockAttendParams& p, unsigned char* ws, c
 }  // namespace bfa
 
 // Whether this kernel takes the call rather than blocks_attend.cu's, which reads the codes once for every eight query rows of a lane.  us measured, that one / this one,
-// 4 heads on 1 at d = 128: 8 lanes x 12,000 tokens, 32 rows a lane 25 / 33, 64 40 / 35, 128 66 / 35; 64 lanes x 12,000, 16 69 / 110, 32 122 / 118, 64 225 / 118; 64 lanes x 700,
-// 32 17 / 21, 64 31 / 21; 64 lanes x 100, 64 16 / 17, 128 30 / 17.  The choice among all the ways is within 1.4% of the best on the mean of the calls swept, 40% at the worst
+// 4 heads on 1 at d = 128: 8 lanes x 12,000 tokens, 32 rows a lane 25 / 34, 64 39 / 33, 128 66 / 36; 64 lanes x 12,000, 16 72 / 109, 32 122 / 123, 64 250 / 138; 64 lanes x 700,
+// 32 17 / 21, 64 31 / 21; 64 lanes x 100, 64 16 / 17, 128 30 / 17.  The choice among all the ways was within 1.4% of the best on the mean of the calls swept, 40% at the worst
 // (of 11 us).
 bool blocks_fa_takes(const BlockAttendParams& p) {
     if (p.dtype == TQ_F32 || (p.D != 64 && p.D != 96 && p.D != 128 && p.D != 256) || p.kn != nullptr) return false;
