@@ -128,7 +128,7 @@ def attend_blocks(queries: torch.Tensor, k_codes, k_scales, v_codes, v_scales, k
     ``queries`` (B, H_q, T_q, D) of the tails' type; H_q a multiple of H.  With ``window`` a query sees the last ``window`` tokens up to its own and
     the first ``sinks`` of the cache.  ``new`` = (keys, values), (B, H, 1, D): one more token, which joins the cache and is attended to, in the
     same launch unless it completes a block (the cache then holds ``length + 1`` tokens).  ``out`` (contiguous, the queries' shape and type)
-    receives the result."""
+    receives the result and must not overlap what is read."""
     if window != 0:
         res = _lib.host().blocks_attend(queries, k_codes, k_scales, v_codes, v_scales, k_tail, v_tail, length, window or 0, sinks, scale,
                                         *(new if new is not None else (None, None)), out)
@@ -168,7 +168,8 @@ def attend_blocks(queries: torch.Tensor, k_codes, k_scales, v_codes, v_scales, k
     if t > s.length + (a.k_new.x is not None):
         raise ValueError(f"{t} query tokens over {s.length} in the cache: write their keys and values first")
     a.n_q_heads, a.t_q, a.q = queries.shape[1], t, _rows(q)
-    a.scale, a.window, a.sinks, a.out = float(s.d ** -0.5 if scale is None else scale), int(window or 0), int(sinks), out.data_ptr()
+    a.scale, a.out = float(s.d ** -0.5 if scale is None else scale), out.data_ptr()
+    a.window, a.sinks = min(int(window or 0), 1 << 62), min(int(sinks), 1 << 62)
     if out.numel() == 0:
         return out
     # Any content, so that the allocator's memory serves: one call's scratch is its own, in captured graphs and on every stream.
@@ -194,6 +195,8 @@ class BlockKVCache:
             raise ValueError(f"codes must be 'int8' or 'e4m3', got {codes!r}")
         if block not in BLOCKS:
             raise ValueError(f"blocks have 16, 32, 64 or 128 tokens, got {block}")
+        if head_dim <= 0 or head_dim % 32 or head_dim > 256:
+            raise ValueError(f"head_dim must be a multiple of 32 up to 256, got {head_dim}")
         if window is not None and window < 1:
             raise ValueError(f"a window holds the query's own token at least, got {window}")
         if sinks < 0 or (sinks and window is None):
@@ -257,8 +260,14 @@ class BlockKVCache:
         """Append (B, H, T, D) tokens."""
         _lib.require_cuda(keys, values)
         t = keys.shape[2] if keys.dim() == 4 else 0
+        fresh = self._store is None
         self._reserve(keys, t)
-        write_blocks(keys, values, *self._store, self._length)
+        try:
+            write_blocks(keys, values, *self._store, self._length)
+        except Exception:
+            if fresh:                                          # (the storage took its type and batch from tokens that were refused)
+                self._store = None
+            raise
         self.offset += t
 
     def attend(self, queries: torch.Tensor, scale: float | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
@@ -281,8 +290,14 @@ class BlockKVCache:
             res = self.decode_step(queries.unsqueeze(2), keys, values, scale, None if out is None else out.view(*queries.shape[:2], 1, queries.shape[2]))
             return out if out is not None else res.squeeze(2)
         _lib.require_cuda(queries, keys, values)
+        fresh = self._store is None
         self._reserve(keys, 1)
-        res = attend_blocks(queries, *self._store, self._length, window=self.window, sinks=self.sinks, scale=scale, out=out, new=(keys, values))
+        try:
+            res = attend_blocks(queries, *self._store, self._length, window=self.window, sinks=self.sinks, scale=scale, out=out, new=(keys, values))
+        except Exception:
+            if fresh:
+                self._store = None
+            raise
         self.offset += 1
         return res
 
@@ -331,10 +346,10 @@ class BlockKVCache:
         if len(v) != 6:
             raise ValueError(f"state must have 6 elements, got {len(v)}")
         if all(t is None for t in v):
-            self._store = None
+            self._store, self.offset, self._dropped = None, 0, 0
             return
         _lib.require_cuda(*v)
-        store = tuple(t.contiguous() for t in v)
+        store = tuple(t.clone(memory_format=torch.contiguous_format) for t in v)       # (the cache that the state came from goes on writing to its own)
         _store(*store, 0)
         if store[4].shape[2] != self.block or store[0].shape[3] != self.head_dim or store[0].dtype is not (torch.int8 if self.codes == "int8" else torch.float8_e4m3fn):
             raise ValueError("the state is of a cache with other blocks, codes or head_dim")

@@ -16,6 +16,9 @@ import torch
 from . import _lib
 
 _tables: dict[tuple, tuple[torch.Tensor, float]] = {}
+# what each kind of scaling understands besides its name; anything else is refused rather than left out
+_KEYS = {"default": (), "linear": ("factor",), "llama3": ("factor", "low_freq_factor", "high_freq_factor", "original_max_position_embeddings"),
+         "yarn": ("factor", "original_max_position_embeddings", "beta_fast", "beta_slow", "attention_factor")}
 
 
 def frequencies(dims: int, base: float = 10000.0, scaling: dict | None = None, device="cuda") -> tuple[torch.Tensor, float]:
@@ -33,7 +36,16 @@ def frequencies(dims: int, base: float = 10000.0, scaling: dict | None = None, d
         raise ValueError(f"an even number of coordinates is turned, got {dims}")
     s = dict(scaling or {})
     kind = s.get("rope_type", s.get("type", "default"))
+    if kind not in _KEYS:
+        raise ValueError(f"unsupported rope scaling {kind!r}: default, linear, llama3 or yarn")
+    unknown = [k for k, v in s.items() if v is not None and k not in ("rope_type", "type", *_KEYS[kind])]
+    if unknown:
+        raise ValueError(f"rope scaling {kind!r} does not know {', '.join(sorted(unknown))}")
+    if "factor" in _KEYS[kind] and not float(s.get("factor") or 0.0) > 0.0:
+        raise ValueError(f"rope scaling {kind!r} needs a positive factor, got {s.get('factor')!r}")
     device = torch.device(device)
+    if device.type == "cuda" and device.index is None:
+        device = torch.device("cuda", torch.cuda.current_device())
     key = (dims, float(base), kind, tuple(sorted((k, v) for k, v in s.items() if isinstance(v, (int, float)))), device)
     if key not in _tables:
         f = float(base) ** (-torch.arange(0, dims, 2, dtype=torch.float64) / dims)
@@ -52,8 +64,6 @@ def frequencies(dims: int, base: float = 10000.0, scaling: dict | None = None, d
             ramp = ((torch.arange(dims // 2, dtype=torch.float64) - first) / max(last - first, 0.001)).clamp(0.0, 1.0)
             f = f * (ramp / slow + (1 - ramp))
             result = float(s.get("attention_factor") or (0.1 * math.log(slow) + 1.0 if slow > 1 else 1.0))
-        elif kind != "default":
-            raise ValueError(f"unsupported rope scaling {kind!r}: default, linear, llama3 or yarn")
         _tables[key] = (f.to(device), result)
     return _tables[key]
 

@@ -48,6 +48,22 @@ def test_frequencies():
             rope.frequencies(**{"device": "cpu", **bad})
 
 
+def test_scalings_that_are_not_understood():
+    from mlx_turboquant_b200 import rope
+    for bad in ({"rope_type": "linear"}, {"rope_type": "linear", "factor": 0.0}, {"rope_type": "llama3", "factor": None}, {"rope_type": "yarn", "factor": 4.0, "mscale": 1.0},
+                {"rope_type": "yarn", "factor": 4.0, "truncate": False}, {"rope_type": "default", "factor": 2.0}, {"rope_type": "longrope", "factor": 4.0}):
+        with pytest.raises(ValueError):
+            rope.frequencies(16, scaling=bad, device="cpu")
+    rope.frequencies(16, scaling={"rope_type": "yarn", "factor": 4.0, "attention_factor": None}, device="cpu")
+
+
+def test_head_dims_that_have_no_kernel():
+    from mlx_turboquant_b200 import BlockKVCache
+    for d in (0, -32, 80, 288):
+        with pytest.raises(ValueError):
+            BlockKVCache(head_dim=d)
+
+
 def test_library_refuses_bad_arguments():
     """Host checks in front of any launch; the addresses are never followed."""
     from mlx_turboquant_b200 import _lib
@@ -210,6 +226,36 @@ def test_state_goes_round():
         BlockKVCache(128, 2, "int8", 32).state = c.state
     with pytest.raises(ValueError):
         z.meta_state = {**c.meta_state, "offset": "100000"}
+
+
+@pytest.mark.gpu
+def test_a_restored_cache_writes_to_its_own_storage():
+    from mlx_turboquant_b200 import BlockKVCache
+    x = torch.randn(1, 2, 70, 64, device="cuda").half()
+    a, z = BlockKVCache(64, 2, block=32), BlockKVCache(64, 2, block=32)
+    a.update(x[:, :, :64], -x[:, :, :64])                         # (whole blocks: the state is the storage from end to end)
+    z.state, z.meta_state = a.state, a.meta_state
+    z.update(torch.ones_like(x[:, :, :6]), torch.ones_like(x[:, :, :6]))
+    k, v = a.update_and_fetch(x[:, :, 64:], -x[:, :, 64:])
+    assert torch.equal(k[:, :, 64:], x[:, :, 64:]) and torch.equal(v[:, :, 64:], -x[:, :, 64:])
+    z.state = (None,) * 6
+    assert z.empty()
+    z.update(x, x)
+    assert z.offset == 70
+
+
+@pytest.mark.gpu
+def test_a_refused_first_update_leaves_nothing():
+    from mlx_turboquant_b200 import BlockKVCache
+    c, x = BlockKVCache(64, 2), torch.randn(1, 2, 5, 64, device="cuda")
+    for bad in ((x.double(), x.double()), (x, x.half()), (x, x[:, :, :4])):
+        with pytest.raises((TypeError, ValueError)):
+            c.update(*bad)
+        with pytest.raises((TypeError, ValueError)):
+            c.decode_step(x[:, :, :1], bad[0][:, :, :1], bad[1][:, :1, :1])
+        assert c.empty() and c.state == (None,) * 6
+    c.update(x.half(), x.half())
+    assert c.offset == 5
 
 
 @pytest.mark.gpu

@@ -279,6 +279,46 @@ def test_the_new_token_joins(length, dtype):
     check_attention(got, q, kd, vd, 128 ** -0.5)
 
 
+def test_the_new_token_joins_many_heads():
+    """Several groups of query heads a lane, of which one appends, over runs and clusters of CTAs."""
+    from mlx_turboquant_b200 import blocks
+    for b, hq, h, length in ((1, 20, 1, 5000), (3, 32, 2, 700), (2, 17, 1, 37), (40, 16, 1, 900)):
+        a, z = (filled(b, h, length, 128, 64, torch.int8, torch.bfloat16, seed=2, room=64) for _ in range(2))
+        k, v, q = rows(b, h, 1, 128, torch.bfloat16, 4), rows(b, h, 1, 128, torch.bfloat16, 5), rows(b, hq, 1, 128, torch.bfloat16, 6, std=0)
+        got = blocks.attend_blocks(q, *a, length, new=(k, v), window=4000, sinks=3)
+        blocks.write_blocks(k, v, *z, length)
+        assert all(torch.equal(x, y) for x, y in zip(a, z))
+        kd, vd = dense(z, length + 1)
+        check_attention(got, q, kd, vd, 128 ** -0.5, 4000, 3)
+
+
+def test_scales_and_windows_at_their_ends():
+    from mlx_turboquant_b200 import blocks
+    for dtype in (torch.bfloat16, torch.float32):
+        store = filled(2, 2, 300, 64, 32, torch.int8, dtype)
+        k, v = dense(store, 300)
+        for t in (1, 3, 150):
+            q = rows(2, 8, t, 64, dtype, 1, std=0)
+            for scale in (0.0, -0.2):
+                check_attention(blocks.attend_blocks(q, *store, 300, scale=scale), q, k, v, scale)
+            assert torch.equal(blocks.attend_blocks(q, *store, 300, window=1 << 70, sinks=1 << 70), blocks.attend_blocks(q, *store, 300))
+            assert torch.equal(blocks.attend_blocks(q, *store, 300, window=1 << 40, sinks=1 << 40), blocks.attend_blocks(q, *store, 300))
+
+
+def test_lanes_in_several_rounds():
+    """More expanded tiles than the workspace is given: some lanes after the others."""
+    total, t, n = 16500, 130, 70
+    store = filled(1, 1, total, 128, 64, torch.int8, torch.bfloat16)
+    q = rows(1, 4, t, 128, torch.bfloat16, 3, std=0)
+    from mlx_turboquant_b200 import blocks
+    got = blocks.attend_blocks(q.expand(n, -1, -1, -1), *repeated(store, n), total)
+    k, v = dense(store, total)
+    for i in (0, n // 2, n - 1):
+        check_attention(got[i:i + 1], q, k, v, 128 ** -0.5)
+    tol = 2 * (2.0 ** -11 + 2.0 ** -14 + 2.0 ** -8) * float(v.abs().max())           # (each within the bound of one result)
+    assert float((got.float() - got[:1].float()).abs().max()) <= tol
+
+
 def test_hidden_values_do_not_count():
     """NaN and infinities in tokens that no query sees: behind the window in blocks and in the tail, behind the last token."""
     from mlx_turboquant_b200 import blocks
