@@ -4,6 +4,7 @@
 //
 // Bound by memory: two bytes in and two out per coordinate.  A CTA owns a few tokens: it forms their cosines and sines once in shared memory,
 // dims / 2 per token (angle and turns in float64, the fraction of a turn in float32), and all heads of the tokens use them.
+// Measured: 8192 tokens x 40 heads of 128, bfloat16, 33 us = 5.0 TB/s (48 with one token at a time, 36 with 2.3 waves of CTAs); 4 tokens 5.8.
 #include <algorithm>
 
 #include "decode_dev.cuh"
