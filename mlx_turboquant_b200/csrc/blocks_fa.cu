@@ -17,15 +17,16 @@
 //       tiles per lane, where writing fp16 rows and reading them back would cost more than the products.
 // blocks_fa_merge_kernel joins the partials of row blocks that several CTAs worked on, in their order.
 //
-// Measured: 2048 queries over 16,384 tokens, 32 heads on 8, d = 128: 548 us, of 309 at the measured rate of products (940 TFLOP/s); expansion 20 and merge 19 of it.
-// Bound by the softmax: of some 1960 clocks per pair of query tiles and key tile, the special-function unit is busy 1024, the tensor pipe 1240, issue 1000; warps of a query
-// tile wait 500 for each other and for products (schedulers that hold a product-issuing warp are the slower ones).  Tried without gain: a warp for scores and another for
-// results (574), weights in tensor-memory buffers of their own (550), one exponential in four by a polynomial (1.5%), naps between looks at barriers, key tiles of
-// 128 tokens (663).
+// Measured: 2048 queries over 16,384 tokens, 32 heads on 8, d = 128: 540 us, of 309 at the measured rate of products (950 TFLOP/s); expansion 20 and merge 19 of it.
+// Bound by both together: of some 1900 clocks per pair of query tiles and key tile the tensor pipe is busy 1240 and the special-function unit 770; a score buffer is full again some
+// 1600 after its weights (both query tiles' products, in one queue), and a tile's softmax takes 1350, issue slots shared with the other query tile's. Tried without gain: a warp for
+// scores and another for results (574), weights in tensor-memory buffers of their own (550), the values' scale in the exponent (542), naps between looks at barriers, key tiles of 128
+// tokens (663).
 // Every mbarrier wait is bounded; one that runs out leaves status 114 (tq_device_status) and raises a flag that ends every other wait; copies and products in
 // flight are waited for (bounded), tensor memory is freed on every path.
 #include <algorithm>
 #include <atomic>
+#include <type_traits>
 
 #include "blocks.cuh"
 #include "fa_dev.cuh"
@@ -130,6 +131,29 @@ __device__ __forceinline__ uint4 bf_to_half(uint4 x, float f) {
 // A token whose values are not finite would reach rows that it is hidden from as 0 * inf: its value row is zeros, its value scale 0, its key scale (and with it the
 // scores of those who see it) NaN.
 __device__ __forceinline__ bool finite_scale(float v) { return fabsf(v) <= 3.4028235e38f; }
+
+// 2^x of two values without the special-function unit, whose rate is what the softmax of a tile would otherwise wait for: 2^round(x) times a polynomial of degree 4 on
+// [-1/2, 1/2] that is 1 at 0, fitted to the least relative error (2^-18.4).  x outside [-127, 127] counts as the end it passed; up to -127 the result is 0.
+__device__ __forceinline__ float unit_of(float x) {        // [-127, 127] -> [0, 1], clamped (NaN: 0)
+    float y;
+    asm("fma.rn.sat.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(x), "f"(1.f / 254.f), "f"(0.5f));
+    return y;
+}
+__device__ __forceinline__ u64 ex2_by_fma(float x0, float x1) {
+    constexpr float ROUND = 12582912.f;                    // 3 * 2^22: the integer part ends up in the low bits
+    const u64 y = pk(unit_of(x0), unit_of(x1)), width = pk(254.f, 254.f);
+    const u64 t = fma2(y, width, pk(ROUND - 127.f, ROUND - 127.f));
+    const u64 f = fma2(y, width, fma2(t, pk(-1.f, -1.f), pk(ROUND - 127.f, ROUND - 127.f)));
+    u64 p = fma2(f, pk(0.00958285294f, 0.00958285294f), pk(0.0559064262f, 0.0559064262f));
+    p = fma2(p, f, pk(0.240240991f, 0.240240991f));
+    p = fma2(p, f, pk(0.693124175f, 0.693124175f));
+    p = fma2(p, f, pk(1.f, 1.f));
+    float p0, p1, t0, t1;
+    upk(p, p0, p1);
+    upk(t, t0, t1);
+    return pk(__uint_as_float(__float_as_uint(p0) + (__float_as_uint(t0) << 23)), __uint_as_float(__float_as_uint(p1) + (__float_as_uint(t1) << 23)));
+}
+constexpr int POLY_EVERY = 4;                          // (none 551 us for 2048 queries x 16,384, every fourth pair 539, every second 570: issue)
 
 template <int D, bool FUSED>
 __global__ void __launch_bounds__(Plan<D, FUSED>::NT, 1) blocks_fa_kernel(const __grid_constant__ Params p) {
@@ -579,13 +603,14 @@ __global__ void __launch_bounds__(Plan<D, FUSED>::NT, 1) blocks_fa_kernel(const 
                 }
                 uint32_t w[2 * NR];
                 u64 ls[2];
-                auto weigh = [&](auto scale_of) {
+                auto weigh = [&](auto scale_of, auto sharing) {
                     ls[0] = ls[1] = pk(0.f, 0.f);
 #pragma unroll
                     for (int r = 0; r < NR; ++r)
 #pragma unroll
                         for (int k = 0; k < 2; ++k) {
-                            const u64 x = pk(ex2(__uint_as_float(v[4 * r + 2 * k])), ex2(__uint_as_float(v[4 * r + 2 * k + 1])));
+                            const float y0 = __uint_as_float(v[4 * r + 2 * k]), y1 = __uint_as_float(v[4 * r + 2 * k + 1]);
+                            const u64 x = decltype(sharing)::value && r % POLY_EVERY == POLY_EVERY - 1 ? ex2_by_fma(y0, y1) : pk(ex2(y0), ex2(y1));
                             ls[k] = add2(ls[k], x);
                             float x0, x1;
                             upk(mul2(x, scale_of(r)), x0, x1);
@@ -594,8 +619,8 @@ __global__ void __launch_bounds__(Plan<D, FUSED>::NT, 1) blocks_fa_kernel(const 
                 };
 #pragma unroll 1
                 for (int pass = 0;; ++pass) {
-                    if (one) weigh([&](int) { return pk(v1, v1); });
-                    else weigh([&](int r) { return nv[r]; });
+                    if (one) weigh([&](int) { return pk(v1, v1); }, std::bool_constant<NQ == 2>{});      // (of every token that is not finite, the other columns' sums tell)
+                    else weigh([&](int r) { return nv[r]; }, std::false_type{});
                     bool again = vmax > vthr;
 #pragma unroll
                     for (int k = 0; k < 2; ++k) {
