@@ -917,15 +917,16 @@ template <int D, bool FUSED> void divide(Params& p, int lanes) {
     int64_t per_y = 0;
     for (int i = 0; i < p.n_blk; ++i) per_y += tiles_of(i);
     const int64_t total = per_y * lanes * p.HG;
-    // at least four tiles a CTA: its set-up, and a partial more to join, cost about as much
-    const int most = int(std::max<int64_t>(1, std::min<int64_t>(p.ctas, total / 4)));
+    const int64_t jobs = int64_t(lanes) * p.HG * p.n_blk;
+    const int ctas = p.ctas, most = int(std::max<int64_t>(1, std::min<int64_t>(ctas, total / 4)));      // (cut: at least four tiles a CTA: a partial more to join costs about as much)
     auto fill = [&](bool whole) -> int64_t {               // -> tiles of the longest run
         int blk = 0, n = 0;
         int64_t y = 0, before = 0, longest = 0, last = 0;  // tiles in front of row block `blk` of y
         p.start[0] = Params::Start{0, 0};
-        for (int i = 1; i <= most; ++i) {
-            int64_t at = total * i / most;
-            const int64_t ny = i == most ? int64_t(lanes) * p.HG : at / per_y, off = at - ny * per_y;
+        const int want = whole ? ctas : most;
+        for (int i = 1; i <= want; ++i) {
+            int64_t at = total * i / want;
+            const int64_t ny = i == want ? int64_t(lanes) * p.HG : at / per_y, off = at - ny * per_y;
             if (ny != y) { y = ny; blk = 0; before = 0; }
             while (blk < p.n_blk && before + tiles_of(blk) <= off) before += tiles_of(blk++);
             Params::Start s{int(y * p.n_blk + blk), int(off - before)};
@@ -942,7 +943,14 @@ template <int D, bool FUSED> void divide(Params& p, int lanes) {
         p.ctas = n;
         return longest;
     };
-    const int64_t whole = fill(true);
+    int64_t whole = 0;                                     // tiles of the longest run of whole row blocks
+    if (jobs <= ctas) {                                    // a CTA each (64 row blocks of two tiles: 17 us as runs of four)
+        for (int i = 0; i < p.n_blk; ++i) whole = std::max<int64_t>(whole, tiles_of(i));
+        for (int i = 0; i <= int(jobs); ++i) p.start[i] = Params::Start{i, 0};
+        p.ctas = int(jobs);
+    } else {
+        whole = fill(true);
+    }
     const double cut_us = 5.0 + 0.45e-6 * double(most) * 2 * Plan<D, FUSED>::ROWS * (D + 4) * 4, tile_us = Plan<D, FUSED>::NQ == 1 ? 1.0 : 1.3;
     if (double(whole - (total + most - 1) / most) * tile_us > cut_us) fill(false);
 }
@@ -997,19 +1005,19 @@ template <int D, bool FUSED> int launch(const BlockAttendParams& a, unsigned cha
     return TQ_OK;
 }
 
-// What a call is expected to cost, in us, fitted to 300 calls (d = 64, 128 and 256; 8 to 128 lanes; 100 to 12,000 tokens; 8 to 1024 query rows a lane): set-up 13, a key
-// tile of a CTA's run 1.25 (fused) or 1.1 at d = 128, a cut 1.4 and the partials' bytes, for expanded tiles another launch and six bytes a coordinate, read and written.
-// Measured, fused / expanded, 4 heads on 1 at d = 128: 8 lanes x 12,000 tokens, 128 query rows a lane 36 / 52, 512 64 / 68, 1024 109 / 87; 64 lanes x 12,000, 256 rows
-// 257 / 262, 384 378 / 341, 512 444 / 329; 64 lanes x 700, 256 22 / 33, 1024 70 / 51.
+// What a call is expected to cost, in us, fitted to 300 calls (d = 64, 128 and 256; 8 to 128 lanes; 100 to 12,000 tokens; 16 to 1024 query rows a lane): set-up 7.7, a key
+// tile of a CTA's run 1.3 (fused) or 1.1 at d = 128, a cut 3.2 and the partials' bytes, for expanded tiles another launch and six bytes a coordinate, read and written.
+// Measured, fused / expanded, 4 heads on 1 at d = 128: 8 lanes x 12,000 tokens, 128 query rows a lane 36 / 52, 512 63 / 65, 1024 109 / 85; 64 lanes x 12,000, 256 rows
+// 217 / 221, 384 322 / 296, 512 432 / 319; 64 lanes x 700, 256 22 / 32, 1024 67 / 48.
 template <int D, bool FUSED> double cost(const BlockAttendParams& p) {
     const Layout l = layout_of<D, FUSED>(p);
     const int64_t lanes = int64_t(p.B) * p.Hkv, jobs = lanes * l.HG * l.n_blk, sms = blocks_sm_count();
     const int rows = Plan<D, FUSED>::NQ * l.QT;
     double n = 0;                                          // tiles of a row block, on the mean of the first and the last
     for (int blk : {0, l.n_blk - 1}) n += 0.5 * Tiles(p, p.total - p.Tq + blk * rows, p.total - p.Tq + std::min((blk + 1) * rows, p.Tq) - 1).n;
-    const double tile = (FUSED ? 1.25 : 1.1) * (D <= 64 ? 0.84 : D <= 96 ? 0.92 : D <= 128 ? 1.0 : 0.92), runs = std::min(double(sms), double(jobs) * n / 4);
-    const double whole = double((jobs + sms - 1) / sms) * n * tile, cut = std::max(4.0, double(jobs) * n / double(sms)) * tile + 1.4 + 2.7e-7 * runs * 2 * Plan<D, FUSED>::ROWS * (D + 4) * 4;
-    return 13.0 + (runs < double(jobs) ? whole : std::min(whole, cut)) + (FUSED ? 0.0 : 2.2 + 1.9e-7 * double(lanes) * l.all.n * TN * 6 * D);
+    const double tile = (FUSED ? 1.3 : 1.1) * (D <= 64 ? 0.7 : D <= 96 ? 0.85 : D <= 128 ? 1.0 : 0.86), runs = std::min(double(sms), double(jobs) * n / 4);
+    const double whole = double((jobs + sms - 1) / sms) * n * tile, cut = std::max(4.0, double(jobs) * n / double(sms)) * tile + 3.2 + 4.6e-7 * runs * 2 * Plan<D, FUSED>::ROWS * (D + 4) * 4;
+    return 7.7 + (runs < double(jobs) ? whole : std::min(whole, cut)) + (FUSED ? 0.0 : 4.0 + 2.1e-7 * double(lanes) * l.all.n * TN * 6 * D);
 }
 // Whether the codes are converted in the attention kernel (not at d = 256, where its eight converting warps cannot keep up: 3 times the other way's time).
 template <int D> bool fused(const BlockAttendParams& p) {
@@ -1034,9 +1042,9 @@ template <int D> int launch_any(const BlockAttendParams& p, unsigned char* ws, c
 }  // namespace bfa
 
 // Whether this kernel takes the call rather than blocks_attend.cu's, which reads the codes once for every eight query rows of a lane.  us measured, that one / this one,
-// 4 heads on 1 at d = 128: 8 lanes x 12,000 tokens, 32 rows a lane 25 / 34, 64 39 / 33, 128 66 / 36; 64 lanes x 12,000, 16 72 / 109, 32 122 / 123, 64 250 / 138; 64 lanes x 700,
-// 32 17 / 21, 64 31 / 21; 64 lanes x 100, 64 16 / 17, 128 30 / 17.  The choice among all the ways was within 1.4% of the best on the mean of the calls swept, 40% at the worst
-// (of 11 us).
+// 4 heads on 1 at d = 128: 8 lanes x 12,000 tokens, 32 rows a lane 25 / 34, 64 39 / 34, 128 66 / 36; 64 lanes x 12,000, 16 72 / 109, 32 131 / 130, 64 259 / 136; 64 lanes x 700,
+// 32 17 / 21, 64 31 / 21; 64 lanes x 100, 32 9 / 10, 64 16 / 10, 128 30 / 10.  The choice among all the ways was within 0.7% of the best on the mean of the calls swept; the
+// largest miss (58%, of 20 us) has d = 256.
 bool blocks_fa_takes(const BlockAttendParams& p) {
     if (p.dtype == TQ_F32 || (p.D != 64 && p.D != 96 && p.D != 128 && p.D != 256) || p.kn != nullptr) return false;
     if (int64_t(p.Tq) * p.G <= HPG || int64_t(p.B) * p.Hkv * p.G * p.Tq >= (int64_t(1) << 29)) return false;
