@@ -3,10 +3,10 @@
 // Codes are exact as fp16; the blocks' scales stay float32 and meet the scores as a multiply-add and the softmax weights as a factor.  A key tile is 64 tokens of
 // those that some query of the call sees: sinks, the window's blocks, the tail.
 //
-// blocks_fa_kernel: one CTA per SM takes an equal run of the flat sequence (lane x head group, row block, key tile), so that no SM waits for another's second
-// row block; a row block is NQ tiles of 128 rows = 128 / GP query tokens x the GP query heads of a GQA group.
-//   * 8 NQ softmax warps, two rows' shares per thread: tcgen05.ld of the scores as fragments, one packed multiply-add each, ex2, P (fp16) back into tensor
-//     memory; a row's reference maximum is looked at through its sum.  They also lay out their rows of the queries, the next row block's before they write
+// blocks_fa_kernel: one CTA per SM takes a run of the flat sequence (lane x head group, row block, key tile): a row block each where there are few, otherwise whole row
+// blocks or equal runs wherever that cuts them, by what each costs (divide()); a row block is NQ tiles of 128 rows = 128 / GP query tokens x the GP query heads of a GQA group.
+//   * 8 NQ softmax warps, two rows' shares per thread: tcgen05.ld of the scores as fragments, one packed multiply-add each, ex2 (a quarter of them
+//     by a polynomial), P (fp16) back into tensor memory; a row's reference maximum is looked at through its sum.  They also lay out their rows of the queries, the next row block's before they write
 //     this one's results;
 //   * a warp per query tile issues S = Q K^T and O += P V, scores two key tiles ahead (N = 64: 48 clocks an instruction with Q in shared memory, of 32 with it in tensor
 //     memory, where there is no room for it; 620 a tile and query tile with the values' products);
@@ -17,7 +17,7 @@
 //       tiles per lane, where writing fp16 rows and reading them back would cost more than the products.
 // blocks_fa_merge_kernel joins the partials of row blocks that several CTAs worked on, in their order.
 //
-// Measured: 2048 queries over 16,384 tokens, 32 heads on 8, d = 128: 540 us, of 309 at the measured rate of products (950 TFLOP/s); expansion 20 and merge 19 of it.
+// Measured: 2048 queries over 16,384 tokens, 32 heads on 8, d = 128: 535 us, of 309 at the measured rate of products (960 TFLOP/s); expansion 20 and merge 19 of it.
 // Bound by both together: of some 1900 clocks per pair of query tiles and key tile the tensor pipe is busy 1240 and the special-function unit 770; a score buffer is full again some
 // 1600 after its weights (both query tiles' products, in one queue), and a tile's softmax takes 1350, issue slots shared with the other query tile's. Tried without gain: a warp for
 // scores and another for results (574), weights in tensor-memory buffers of their own (550), the values' scale in the exponent (542), naps between looks at barriers, key tiles of 128
