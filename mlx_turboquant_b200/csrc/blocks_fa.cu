@@ -781,8 +781,8 @@ template <int D> __global__ void __launch_bounds__(EX_T) blocks_fa_expand_kernel
     const int base = (p.all.is_tail(ord) ? c.n8 : 0) + p.all.tile_of(ord) * TN;
     unsigned char* tiles = const_cast<unsigned char*>(p.tiles) + at * 2 * K_TILE;
     float* scales = const_cast<float*>(p.scales) + at * TILE_INFO;
+    pdl_wait();                                            // (the tiles' memory may be what the kernel in front still reads or writes)
     if (tid == 0) *reinterpret_cast<int2*>(scales + 2 * TN) = make_int2(base, p.all.is_tail(ord) ? c.total : c.n8);
-    pdl_wait();
     if (!p.all.is_tail(ord)) {
         constexpr int U = 2 * PIECES / EX_T;               // (1024 / 16 = 64 tokens x D / 16 pieces x 2: a multiple of 256 for every D)
         static_assert(2 * PIECES % EX_T == 0, "pieces");

@@ -63,6 +63,9 @@ __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, int sr
 __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N> __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 // Programmatic dependent launch: wait for the previous grid on the stream / let the next grid start its prologue.
+// A kernel that is launched this way stores NOTHING to global memory before its wait, and reads only what no earlier kernel can still be writing: parameters,
+// tables that the library built long before.  Workspaces count too: the allocator hands memory on in stream order, so that a call's scratch, or its result, can be memory that
+// the kernel in front still works on.  (tests/test_dependency_waits.py reads the kernels for it.)
 __device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void pdl_trigger() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 __device__ __forceinline__ uint32_t pack_h2(float lo, float hi) {
