@@ -16,9 +16,32 @@ import torch
 from . import _lib
 
 _tables: dict[tuple, tuple[torch.Tensor, float]] = {}
-# what each kind of scaling understands besides its name; anything else is refused rather than left out
-_KEYS = {"default": (), "linear": ("factor",), "llama3": ("factor", "low_freq_factor", "high_freq_factor", "original_max_position_embeddings"),
-         "yarn": ("factor", "original_max_position_embeddings", "beta_fast", "beta_slow", "attention_factor")}
+# what each kind of scaling understands besides its name, and what stands for a setting that is absent or None (REQUIRED: it has to be there); anything else is
+# refused rather than left out
+REQUIRED = object()
+_SETTINGS = {"default": {}, "linear": {"factor": REQUIRED},
+             "llama3": {"factor": REQUIRED, "low_freq_factor": 1.0, "high_freq_factor": 4.0, "original_max_position_embeddings": 8192.0},
+             "yarn": {"factor": REQUIRED, "original_max_position_embeddings": 4096.0, "beta_fast": 32.0, "beta_slow": 1.0, "attention_factor": None}}
+
+
+def _settings(scaling: dict | None) -> tuple[str, dict]:
+    """The kind of a model's ``rope_scaling`` entry and its settings as Python floats (or None)."""
+    s = dict(scaling or {})
+    kind = s.get("rope_type", s.get("type", "default"))
+    if kind not in _SETTINGS:
+        raise ValueError(f"unsupported rope scaling {kind!r}: default, linear, llama3 or yarn")
+    unknown = [k for k, v in s.items() if v is not None and k not in ("rope_type", "type", *_SETTINGS[kind])]
+    if unknown:
+        raise ValueError(f"rope scaling {kind!r} does not know {', '.join(sorted(unknown))}")
+    out = {}
+    for name, default in _SETTINGS[kind].items():
+        value = s.get(name)
+        if value is None and default is REQUIRED:
+            raise ValueError(f"rope scaling {kind!r} needs a {name}")
+        out[name] = default if value is None else float(value)
+    if "factor" in out and not out["factor"] > 0.0:
+        raise ValueError(f"rope scaling {kind!r} needs a positive factor, got {s['factor']!r}")
+    return kind, out
 
 
 def frequencies(dims: int, base: float = 10000.0, scaling: dict | None = None, device="cuda") -> tuple[torch.Tensor, float]:
@@ -34,36 +57,28 @@ def frequencies(dims: int, base: float = 10000.0, scaling: dict | None = None, d
     """
     if dims <= 0 or dims % 2:
         raise ValueError(f"an even number of coordinates is turned, got {dims}")
-    s = dict(scaling or {})
-    kind = s.get("rope_type", s.get("type", "default"))
-    if kind not in _KEYS:
-        raise ValueError(f"unsupported rope scaling {kind!r}: default, linear, llama3 or yarn")
-    unknown = [k for k, v in s.items() if v is not None and k not in ("rope_type", "type", *_KEYS[kind])]
-    if unknown:
-        raise ValueError(f"rope scaling {kind!r} does not know {', '.join(sorted(unknown))}")
-    if "factor" in _KEYS[kind] and not float(s.get("factor") or 0.0) > 0.0:
-        raise ValueError(f"rope scaling {kind!r} needs a positive factor, got {s.get('factor')!r}")
+    kind, s = _settings(scaling)
     device = torch.device(device)
     if device.type == "cuda" and device.index is None:
         device = torch.device("cuda", torch.cuda.current_device())
-    key = (dims, float(base), kind, tuple(sorted((k, v) for k, v in s.items() if isinstance(v, (int, float)))), device)
+    key = (dims, float(base), kind, tuple(s.values()), device)
     if key not in _tables:
         f = float(base) ** (-torch.arange(0, dims, 2, dtype=torch.float64) / dims)
         result = 1.0
         if kind == "linear":
-            f = f / float(s["factor"])
+            f = f / s["factor"]
         elif kind == "llama3":
-            low, high = float(s.get("low_freq_factor", 1.0)), float(s.get("high_freq_factor", 4.0))
-            turns = float(s.get("original_max_position_embeddings", 8192)) * f / (2 * math.pi)
+            low, high = s["low_freq_factor"], s["high_freq_factor"]
+            turns = s["original_max_position_embeddings"] * f / (2 * math.pi)
             keep = ((turns - low) / (high - low)).clamp(0.0, 1.0)
-            f = f * ((1 - keep) / float(s["factor"]) + keep)
+            f = f * ((1 - keep) / s["factor"] + keep)
         elif kind == "yarn":
-            length, slow = float(s.get("original_max_position_embeddings", 4096)), float(s["factor"])
-            at = [dims * math.log(length / (t * 2 * math.pi)) / (2 * math.log(base)) for t in (float(s.get("beta_fast", 32.0)), float(s.get("beta_slow", 1.0)))]
+            length, slow = s["original_max_position_embeddings"], s["factor"]
+            at = [dims * math.log(length / (t * 2 * math.pi)) / (2 * math.log(base)) for t in (s["beta_fast"], s["beta_slow"])]
             first, last = max(math.floor(at[0]), 0), min(math.ceil(at[1]), dims - 1)
             ramp = ((torch.arange(dims // 2, dtype=torch.float64) - first) / max(last - first, 0.001)).clamp(0.0, 1.0)
             f = f * (ramp / slow + (1 - ramp))
-            result = float(s.get("attention_factor") or (0.1 * math.log(slow) + 1.0 if slow > 1 else 1.0))
+            result = s["attention_factor"] or (0.1 * math.log(slow) + 1.0 if slow > 1 else 1.0)
         _tables[key] = (f.to(device), result)
     return _tables[key]
 

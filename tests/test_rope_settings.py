@@ -1,0 +1,49 @@
+"""The settings of scaled rotary positions: what a table is kept under, what is refused.  No GPU."""
+
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from mlx_turboquant_b200 import rope
+
+
+def table(dims=64, base=10000.0, **scaling):
+    return rope.frequencies(dims, base, scaling, "cpu")
+
+
+@pytest.mark.parametrize("number", (float, int, str, np.float32, np.float64, np.int64, torch.tensor))
+@pytest.mark.parametrize("kind,other", (("linear", {}), ("llama3", {"original_max_position_embeddings": 8192}), ("yarn", {"original_max_position_embeddings": 4096})))
+def test_every_setting_counts(kind, other, number):
+    """Two tables in a row whose settings differ in one number, of whatever type it comes in; each is that of a plain float."""
+    names = {"linear": ("factor",), "llama3": ("factor", "low_freq_factor", "high_freq_factor", "original_max_position_embeddings"),
+             "yarn": ("factor", "original_max_position_embeddings", "beta_fast", "beta_slow")}[kind]
+    values = {"factor": (4, 8), "low_freq_factor": (1, 2), "high_freq_factor": (4, 16), "original_max_position_embeddings": (8192, 1024), "beta_fast": (32, 8), "beta_slow": (1, 2)}
+    for name in names:
+        got = [table(rope_type=kind, **{"factor": 16.0, **other, name: number(v)}) for v in values[name]]
+        rope._tables.clear()
+        want = [table(rope_type=kind, **{"factor": 16.0, **other, name: float(v)}) for v in values[name]]
+        assert not torch.equal(got[0][0], got[1][0]), name
+        for g, w in zip(got, want):
+            assert torch.equal(g[0], w[0]) and g[1] == w[1], name
+    if kind == "yarn":
+        assert table(rope_type=kind, factor=4.0, **other, attention_factor=number(2))[1] == 2.0 and table(rope_type=kind, factor=4.0, **other, attention_factor=number(3))[1] == 3.0
+
+
+def test_none_is_as_good_as_absent():
+    for kind, names in (("llama3", ("low_freq_factor", "high_freq_factor")), ("yarn", ("beta_fast", "beta_slow", "attention_factor"))):
+        given = {"rope_type": kind, "factor": 8.0, "original_max_position_embeddings": 8192}
+        plain = table(**given)
+        for name in names:
+            f, m = table(**given, **{name: None})
+            assert torch.equal(f, plain[0]) and m == plain[1], name
+    assert torch.equal(table(rope_type="default", factor=None)[0], table()[0])
+
+
+def test_the_defaults_are_the_published_ones():
+    f, m = table(rope_type="yarn", factor=8.0, original_max_position_embeddings=4096)
+    g, n = table(rope_type="yarn", factor=8.0, original_max_position_embeddings=4096, beta_fast=32, beta_slow=1, attention_factor=0.1 * math.log(8.0) + 1)
+    assert torch.equal(f, g) and m == n
+    f, _ = table(rope_type="llama3", factor=8.0, original_max_position_embeddings=8192)
+    assert torch.equal(f, table(rope_type="llama3", factor=8.0, original_max_position_embeddings=8192, low_freq_factor=1, high_freq_factor=4)[0])
