@@ -53,6 +53,9 @@ class ModelArgs:
         return bool(self.fused_rope or self.rope_scaling or self.rope_traditional or self.partial_rotary_factor != 1.0)
 
     def rotary_frequencies(self, device):
+        scaling = self.rope_scaling or {}
+        if scaling.get("rope_type", scaling.get("type")) == "yarn" and scaling.get("original_max_position_embeddings") is None:
+            raise ValueError("rope_scaling 'yarn' needs original_max_position_embeddings: the length that the model was trained on")
         dims = int(self.head_dim * self.partial_rotary_factor) // 2 * 2
         return rotary.frequencies(dims, self.rope_theta, self.rope_scaling, device)
 

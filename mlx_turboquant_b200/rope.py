@@ -10,6 +10,7 @@ from __future__ import annotations
 
 import ctypes as C
 import math
+import warnings
 
 import torch
 
@@ -20,7 +21,7 @@ _tables: dict[tuple, tuple[torch.Tensor, float]] = {}
 # refused rather than left out
 REQUIRED = object()
 _SETTINGS = {"default": {}, "linear": {"factor": REQUIRED},
-             "llama3": {"factor": REQUIRED, "low_freq_factor": 1.0, "high_freq_factor": 4.0, "original_max_position_embeddings": 8192.0},
+             "llama3": {"factor": REQUIRED, "low_freq_factor": 1.0, "high_freq_factor": 4.0, "original_max_position_embeddings": REQUIRED},
              "yarn": {"factor": REQUIRED, "original_max_position_embeddings": 4096.0, "beta_fast": 32.0, "beta_slow": 1.0, "attention_factor": None}}
 
 
@@ -41,6 +42,10 @@ def _settings(scaling: dict | None) -> tuple[str, dict]:
         out[name] = default if value is None else float(value)
     if "factor" in out and not out["factor"] > 0.0:
         raise ValueError(f"rope scaling {kind!r} needs a positive factor, got {s['factor']!r}")
+    # a configuration without the length means the model's own, which only the caller knows
+    if kind == "yarn" and s.get("original_max_position_embeddings") is None:
+        warnings.warn(f"rope scaling 'yarn' without original_max_position_embeddings: {int(out['original_max_position_embeddings'])} positions are assumed; "
+                      "give the length that the model was trained on", UserWarning, stacklevel=3)
     return kind, out
 
 
@@ -50,10 +55,13 @@ def frequencies(dims: int, base: float = 10000.0, scaling: dict | None = None, d
     ``scaling`` is the ``rope_scaling`` entry of a model's config: ``{"rope_type": ..., "factor": ...}`` with
 
     * ``"linear"``: positions divided by ``factor``;
-    * ``"llama3"``: pairs that turn less than ``low_freq_factor`` times in ``original_max_position_embeddings`` positions are slowed by ``factor``,
-      those that turn more than ``high_freq_factor`` times stay, a blend in between;
-    * ``"yarn"``: the same with a ramp over the pairs' index between ``beta_fast`` and ``beta_slow`` turns, and a factor on the result
+    * ``"llama3"``: pairs that turn less than ``low_freq_factor`` (1) times in ``original_max_position_embeddings`` positions are slowed by ``factor``,
+      those that turn more than ``high_freq_factor`` (4) times stay, a blend in between;
+    * ``"yarn"``: the same with a ramp over the pairs' index between ``beta_fast`` (32) and ``beta_slow`` (1) turns, and a factor on the result
       (``attention_factor``, otherwise ``0.1 ln(factor) + 1``).
+
+    The length that a model was trained on, ``original_max_position_embeddings``, is wanted with both: configurations that leave it out mean the model's
+    ``max_position_embeddings``.  llama3 refuses without it; yarn assumes 4096 and says so in a warning.
     """
     if dims <= 0 or dims % 2:
         raise ValueError(f"an even number of coordinates is turned, got {dims}")

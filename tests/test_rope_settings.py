@@ -47,3 +47,19 @@ def test_the_defaults_are_the_published_ones():
     assert torch.equal(f, g) and m == n
     f, _ = table(rope_type="llama3", factor=8.0, original_max_position_embeddings=8192)
     assert torch.equal(f, table(rope_type="llama3", factor=8.0, original_max_position_embeddings=8192, low_freq_factor=1, high_freq_factor=4)[0])
+
+
+def test_a_scaling_without_its_length():
+    """Left out of a model's configuration, the length is the model's own: no number of this package's stands for it unsaid."""
+    from mlx_turboquant_b200.consumer import ModelArgs
+    for missing in ({}, {"original_max_position_embeddings": None}):
+        with pytest.raises(ValueError, match="original_max_position_embeddings"):
+            table(rope_type="llama3", factor=8.0, **missing)
+        with pytest.warns(UserWarning, match="4096 positions"):
+            f, _ = table(rope_type="yarn", factor=8.0, **missing)
+        assert torch.equal(f, table(rope_type="yarn", factor=8.0, original_max_position_embeddings=4096)[0])
+        for kind in ("llama3", "yarn"):
+            with pytest.raises(ValueError, match="original_max_position_embeddings"):
+                ModelArgs(head_dim=64, rope_scaling={"rope_type": kind, "factor": 8.0, **missing}).rotary_frequencies("cpu")
+    f, _ = ModelArgs(head_dim=64, rope_theta=10000.0, rope_scaling={"type": "yarn", "factor": 8.0, "original_max_position_embeddings": 2048}).rotary_frequencies("cpu")
+    assert torch.equal(f, table(rope_type="yarn", factor=8.0, original_max_position_embeddings=2048)[0])
