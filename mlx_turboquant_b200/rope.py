@@ -40,8 +40,11 @@ def _settings(scaling: dict | None) -> tuple[str, dict]:
         if value is None and default is REQUIRED:
             raise ValueError(f"rope scaling {kind!r} needs a {name}")
         out[name] = default if value is None else float(value)
-    if "factor" in out and not out["factor"] > 0.0:
-        raise ValueError(f"rope scaling {kind!r} needs a positive factor, got {s['factor']!r}")
+    bad = [f"{k} = {s[k]!r}" for k, v in out.items() if v is not None and not 0.0 < v < math.inf and (k != "attention_factor" or v != 0.0)]       # (0: the default)
+    if bad:
+        raise ValueError(f"rope scaling {kind!r} needs positive numbers, got {', '.join(bad)}")
+    if kind == "llama3" and not out["high_freq_factor"] > out["low_freq_factor"]:
+        raise ValueError(f"rope scaling 'llama3' blends between low_freq_factor and a larger high_freq_factor, got {out['low_freq_factor']} and {out['high_freq_factor']}")
     # a configuration without the length means the model's own, which only the caller knows
     if kind == "yarn" and s.get("original_max_position_embeddings") is None:
         warnings.warn(f"rope scaling 'yarn' without original_max_position_embeddings: {int(out['original_max_position_embeddings'])} positions are assumed; "
@@ -65,7 +68,11 @@ def frequencies(dims: int, base: float = 10000.0, scaling: dict | None = None, d
     """
     if dims <= 0 or dims % 2:
         raise ValueError(f"an even number of coordinates is turned, got {dims}")
+    if not (0.0 < float(base) < math.inf):
+        raise ValueError(f"the base of the frequencies must be positive, got {base}")
     kind, s = _settings(scaling)
+    if kind == "yarn" and float(base) <= 1.0:
+        raise ValueError(f"rope scaling 'yarn' needs a base above 1, got {base}")
     device = torch.device(device)
     if device.type == "cuda" and device.index is None:
         device = torch.device("cuda", torch.cuda.current_device())

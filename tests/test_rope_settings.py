@@ -63,3 +63,20 @@ def test_a_scaling_without_its_length():
                 ModelArgs(head_dim=64, rope_scaling={"rope_type": kind, "factor": 8.0, **missing}).rotary_frequencies("cpu")
     f, _ = ModelArgs(head_dim=64, rope_theta=10000.0, rope_scaling={"type": "yarn", "factor": 8.0, "original_max_position_embeddings": 2048}).rotary_frequencies("cpu")
     assert torch.equal(f, table(rope_type="yarn", factor=8.0, original_max_position_embeddings=2048)[0])
+
+
+def test_numbers_that_give_no_angles():
+    for bad in (float("inf"), float("nan"), -2.0, 0.0):
+        for kind in ("linear", "llama3", "yarn"):
+            with pytest.raises(ValueError):
+                table(rope_type=kind, factor=bad, **({} if kind == "linear" else {"original_max_position_embeddings": 4096}))
+        for kind, name in (("llama3", "original_max_position_embeddings"), ("yarn", "original_max_position_embeddings"), ("yarn", "beta_fast"), ("yarn", "beta_slow"), ("llama3", "low_freq_factor")):
+            with pytest.raises(ValueError):
+                table(**{"rope_type": kind, "factor": 2.0, "original_max_position_embeddings": 4096, name: bad})
+        with pytest.raises(ValueError):
+            table(base=bad)
+    for low, high in ((2, 2), (4, 1)):
+        with pytest.raises(ValueError):
+            table(rope_type="llama3", factor=8.0, original_max_position_embeddings=8192, low_freq_factor=low, high_freq_factor=high)
+    with pytest.raises(ValueError):
+        table(base=1.0, rope_type="yarn", factor=2.0, original_max_position_embeddings=4096)
