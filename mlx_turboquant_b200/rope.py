@@ -54,6 +54,7 @@ def _settings(scaling: dict | None) -> tuple[str, dict]:
 
 def frequencies(dims: int, base: float = 10000.0, scaling: dict | None = None, device="cuda") -> tuple[torch.Tensor, float]:
     """(radians per position of each of the ``dims / 2`` pairs, float64 on ``device``; the factor on the result), shared between calls.
+    The first call for a table copies it to the device: not inside a graph's capture.
 
     ``scaling`` is the ``rope_scaling`` entry of a model's config: ``{"rope_type": ..., "factor": ...}`` with
 
@@ -78,6 +79,8 @@ def frequencies(dims: int, base: float = 10000.0, scaling: dict | None = None, d
         device = torch.device("cuda", torch.cuda.current_device())
     key = (dims, float(base), kind, tuple(s.values()), device)
     if key not in _tables:
+        if device.type == "cuda" and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("rope.frequencies: this table is not made yet, and making it copies from the host, which a graph cannot capture; call it once before the capture")
         f = float(base) ** (-torch.arange(0, dims, 2, dtype=torch.float64) / dims)
         result = 1.0
         if kind == "linear":

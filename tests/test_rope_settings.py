@@ -80,3 +80,13 @@ def test_numbers_that_give_no_angles():
             table(rope_type="llama3", factor=8.0, original_max_position_embeddings=8192, low_freq_factor=low, high_freq_factor=high)
     with pytest.raises(ValueError):
         table(base=1.0, rope_type="yarn", factor=2.0, original_max_position_embeddings=4096)
+
+
+def test_no_table_is_made_inside_a_capture(monkeypatch):
+    """Nothing of a refused call stays: the table is made by the next one outside."""
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    with pytest.raises(RuntimeError, match="before the capture"):
+        rope.frequencies(48, 77.0, device="cuda:0")
+    assert not any(k[:2] == (48, 77.0) for k in rope._tables)
+    f, _ = table(48, 77.0)
+    assert rope.frequencies(48, 77.0, device="cpu")[0] is f                 # (the CPU's are never captured)
