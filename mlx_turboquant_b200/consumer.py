@@ -105,7 +105,10 @@ class Attention(torch.nn.Module):
         # queries and keys sit at the same positions: one pass over both; the tables are shared by layers at one offset
         values = qkv[:, hq + hkv:]
         if self.args.rotary_kernel:
-            freqs, factor = self.args.rotary_frequencies(x.device)
+            memo = rope_memo if rope_memo is not None else {}
+            if x.device not in memo:
+                memo[x.device] = self.args.rotary_frequencies(x.device)
+            freqs, factor = memo[x.device]
             queries, keys = rotary.apply_rotary(qkv[:, :hq], qkv[:, hq:hq + hkv], freqs, offset, interleaved=self.args.rope_traditional, factor=factor)
         else:
             tables = rope_memo.get((offset, L)) if rope_memo is not None else None

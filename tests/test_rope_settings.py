@@ -90,3 +90,15 @@ def test_no_table_is_made_inside_a_capture(monkeypatch):
     assert not any(k[:2] == (48, 77.0) for k in rope._tables)
     f, _ = table(48, 77.0)
     assert rope.frequencies(48, 77.0, device="cpu")[0] is f                 # (the CPU's are never captured)
+
+
+def test_a_forward_pass_looks_its_table_up_once(monkeypatch):
+    """Not for each layer of each step: the settings are read anew every time."""
+    from mlx_turboquant_b200 import consumer
+    args = consumer.ModelArgs(hidden_size=64, num_hidden_layers=5, num_attention_heads=2, num_key_value_heads=1, head_dim=32, intermediate_size=64, vocab_size=32, rope_scaling={"rope_type": "linear", "factor": 2.0})
+    m, calls, made = consumer.LlamaShaped(args, dtype=torch.float32, device="cpu"), [], rope.frequencies
+    monkeypatch.setattr(consumer.rotary, "frequencies", lambda *a, **kw: calls.append(a) or made(*a, **kw))
+    monkeypatch.setattr(consumer.rotary, "apply_rotary", lambda q, k, *a, **kw: (q, k))
+    for n in (1, 2):
+        m(torch.zeros(1, 3, dtype=torch.int64))
+        assert len(calls) == n
