@@ -181,6 +181,14 @@ def attend_blocks(queries: torch.Tensor, k_codes, k_scales, v_codes, v_scales, k
     return out
 
 
+def window_mask(offset: int, n: int, window: int, sinks: int, device) -> torch.Tensor:
+    """Which tokens ``n`` queries behind ``offset`` tokens see: (n, sinks before the window + tokens from the first query's window on)."""
+    low = max(0, offset - window + 1)
+    pos = torch.arange(offset, offset + n, device=device)[:, None]
+    tok = torch.cat([torch.arange(min(sinks, low), device=device), torch.arange(low, offset + n, device=device)])[None, :]
+    return (tok <= pos) & ((pos - tok < window) | (tok < sinks))
+
+
 class BlockKVCache:
     """KV cache of a layer in 8-bit blocks, behind the protocol of ``TurboQuantKVCache``.
 
@@ -302,17 +310,37 @@ class BlockKVCache:
         return res
 
     def update_and_fetch(self, keys: torch.Tensor, values: torch.Tensor):
-        """Append, and return all tokens dense, of the tokens' type (caches without a window)."""
-        if self.window is not None:
-            raise NotImplementedError("a cache with a window drops what it hides: use update and attend")
+        """Append, and return dense, of the tokens' type, what queries of the new tokens may see: all tokens, or with a window the first ``sinks`` of them
+        and those from the first new token's window on.  Which of these each query sees, ``make_mask`` says, asked before this call."""
+        if self.window is None:
+            self.update(keys, values)
+            return read_blocks(*self._store, self._length)
+        if not (keys.is_cuda and values.is_cuda):
+            raise NotImplementedError("mlx_turboquant_b200 runs on CUDA tensors only; a cache with a window has nothing to return on " + str(keys.device))
+        low, sinks = self._seen_from()
         self.update(keys, values)
-        return read_blocks(*self._store, self._length)
+        return tuple(self._visible(x, low - self._dropped, sinks) for x in read_blocks(*self._store, self._length))
+
+    def _seen_from(self) -> tuple[int, int]:
+        """The first token that the next one sees through its window, and how many sinks lie before that."""
+        low = max(0, self.offset - self.window + 1)
+        return low, min(self.sinks, low)
+
+    @staticmethod
+    def _visible(x: torch.Tensor, at: int, sinks: int) -> torch.Tensor:
+        return x[:, :, at - sinks:] if at == sinks or sinks == 0 else torch.cat([x[:, :, :sinks], x[:, :, at:]], dim=2)
 
     def make_mask(self, N: int, offset: int = 0, return_array: bool = False, window_size: int | None = None) -> Any | None:
-        """``None`` for a single-token step, ``"causal"`` otherwise; the cache's own window is part of ``attend``."""
-        if window_size is not None and window_size != self.window:
-            raise NotImplementedError(f"this cache has a window of {self.window}, not {window_size}")
-        return None if N == 1 and not return_array else "causal"
+        """The mask of ``N`` new tokens over what ``update_and_fetch`` returns for them; asked before that call.  ``None`` for a single token, ``"causal"`` where
+        that is all, otherwise a boolean tensor (N, tokens returned), true where a query sees a token.  ``attend`` needs none: the window is part of it.
+        ``window_size`` may be the window, or what the model's own cache calls its size: window and sinks together."""
+        if window_size is not None and (self.window is None or window_size not in (self.window, self.window + self.sinks)):
+            raise NotImplementedError(f"this cache has a window of {self.window} and {self.sinks} sinks, not {window_size}")
+        if N == 1 and not return_array:
+            return None
+        if self.window is None or (not return_array and self.offset + N - self.window <= self.sinks):
+            return "causal"
+        return window_mask(self.offset, N, self.window, self.sinks, torch.device("cuda") if self._store is None else self._store[0].device)
 
     def size(self) -> int:
         return self.offset

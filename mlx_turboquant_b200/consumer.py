@@ -127,13 +127,14 @@ class Attention(torch.nn.Module):
                 cache.update(keys.contiguous(), values.contiguous())
                 out = cache.attend(queries.contiguous(), self.scale)                   # (B, hq, L, d)
         else:
+            mask = None
             if cache is not None:
+                if getattr(cache, "window", None) is not None:                          # (its own mask: it returns what the window leaves)
+                    mask = cache.make_mask(L)
                 keys, values = cache.update_and_fetch(keys.contiguous(), values.contiguous())
             q = queries.float() if keys.dtype == torch.float32 else queries
             T = keys.shape[2]
-            if L == 1:
-                mask = None
-            else:                                                                       # causal, aligned to the end
+            if L > 1 and not isinstance(mask, torch.Tensor):                            # causal, aligned to the end
                 pos = torch.arange(T - L, T, device=x.device)
                 mask = torch.arange(T, device=x.device)[None, :] <= pos[:, None]
             out = F.scaled_dot_product_attention(q, keys.to(q.dtype), values.to(q.dtype), attn_mask=mask, scale=self.scale,

@@ -152,7 +152,8 @@ def apply_turboquant(model, key_bits: float = 4, value_bits: float = 2, residual
     Arguments and defaults are the reference's.  Layers listed in ``skip_layers`` (or auto-detected as
     outliers), linear-attention layers and sliding-window layers keep an uncompressed / model-default cache.
     With ``block_cache`` ("int8" or "e4m3"; new here) skipped layers and outliers get an 8-bit ``BlockKVCache``, and so do sliding-window
-    layers whose default cache says how long the window is (``max_size``, and ``keep`` first tokens).
+    layers whose default cache says how long the window is (``max_size``, and ``keep`` first tokens among them).  Such a cache serves callers of
+    ``update`` + ``attend``, and callers of ``update_and_fetch`` that take their mask from ``make_mask(N)`` before it.
     """
     if block_cache not in (None, "int8", "e4m3"):
         raise ValueError(f"block_cache must be 'int8', 'e4m3' or None, got {block_cache!r}")
