@@ -25,6 +25,11 @@ CODE_TYPES = {torch.int8: _lib.TQ_CODE_INT8, torch.float8_e4m3fn: _lib.TQ_CODE_E
 BLOCKS = (16, 32, 64, 128)
 
 
+def head_dim_ok(d: int) -> bool:
+    """Whether the kernels of the block cache take this head_dim."""
+    return 0 < d <= 256 and d % 32 == 0
+
+
 def _no_grad(*tensors) -> None:
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
         raise RuntimeError("the block cache has no backward pass: call it under torch.no_grad()")
@@ -203,7 +208,7 @@ class BlockKVCache:
             raise ValueError(f"codes must be 'int8' or 'e4m3', got {codes!r}")
         if block not in BLOCKS:
             raise ValueError(f"blocks have 16, 32, 64 or 128 tokens, got {block}")
-        if head_dim <= 0 or head_dim % 32 or head_dim > 256:
+        if not head_dim_ok(head_dim):
             raise ValueError(f"head_dim must be a multiple of 32 up to 256, got {head_dim}")
         if window is not None and window < 1:
             raise ValueError(f"a window holds the query's own token at least, got {window}")

@@ -12,7 +12,7 @@ import warnings
 
 import torch
 
-from .blocks import BlockKVCache
+from .blocks import BlockKVCache, head_dim_ok
 from .cache import TurboQuantKVCache
 
 
@@ -153,7 +153,8 @@ def apply_turboquant(model, key_bits: float = 4, value_bits: float = 2, residual
     outliers), linear-attention layers and sliding-window layers keep an uncompressed / model-default cache.
     With ``block_cache`` ("int8" or "e4m3"; new here) skipped layers and outliers get an 8-bit ``BlockKVCache``, and so do sliding-window
     layers whose default cache says how long the window is (``max_size``, and ``keep`` first tokens among them).  Such a cache serves callers of
-    ``update`` + ``attend``, and callers of ``update_and_fetch`` that take their mask from ``make_mask(N)`` before it.
+    ``update`` + ``attend``, and callers of ``update_and_fetch`` that take their mask from ``make_mask(N)`` before it.  Head dims that the block
+    cache has no kernels for (it takes multiples of 32 up to 256) leave those layers as they are without ``block_cache``, with a warning.
     """
     if block_cache not in (None, "int8", "e4m3"):
         raise ValueError(f"block_cache must be 'int8', 'e4m3' or None, got {block_cache!r}")
@@ -161,6 +162,10 @@ def apply_turboquant(model, key_bits: float = 4, value_bits: float = 2, residual
     hd = head_dim or config["head_dim"]
     nkv = num_kv_heads or config["num_kv_heads"]
     nl = num_layers or config["num_layers"]
+    if block_cache is not None and not head_dim_ok(hd):
+        warnings.warn(f"block_cache={block_cache!r} has no kernels for head_dim {hd} (multiples of 32 up to 256): skipped and sliding-window layers "
+                      "keep the caches that they have without it.", UserWarning, stacklevel=2)
+        block_cache = None
 
     if nkv <= 2 and key_bits < 4:   # few KV heads are more sensitive (patch.py:198-217)
         old, key_bits = key_bits, 4

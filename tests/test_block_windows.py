@@ -113,3 +113,15 @@ def test_the_caller_by_both_routes(keep):
         apart.append(float((a - w).abs().max()) / float(z.abs().max()))
     assert max(apart) > 0.06                                # (the windows do hide something here)
     assert dense[0].offset == 190
+
+
+@pytest.mark.parametrize("head_dim", (80, 112, 288, 48))
+def test_head_dims_without_kernels_leave_the_layers_as_they_were(head_dim):
+    from test_block_cache import _model, _RotatingKVCache
+    from mlx_turboquant_b200 import apply_turboquant
+    from mlx_turboquant_b200.patch import KVCache
+    m = _model(lambda i: _RotatingKVCache() if i == 2 else KVCache())
+    with pytest.warns(UserWarning, match="no kernels for head_dim"):
+        apply_turboquant(m, head_dim=head_dim, skip_layers=[0], block_cache="int8")
+    assert [type(c).__name__ for c in m.make_cache()] == ["KVCache", "TurboQuantKVCache", "_RotatingKVCache", "TurboQuantKVCache"]
+    assert "block_cache" not in m._turboquant_config
