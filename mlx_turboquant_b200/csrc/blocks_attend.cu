@@ -7,9 +7,10 @@
 // (cp.async, 16 bytes a lane).  mma.sync with the tokens as M (scores) and the coordinates as M (values): eight query rows share every code.  (The products
 // are tiny, N = 8: tcgen05 would want 64 rows of operands staged in shared memory.)  Which coordinate a fragment's row or column stands for is free as long
 // as queries and results agree.
-//   scores, int8: integer products m16n8k32 on the codes as they are; the query in fixed point, 15 bits of its largest element for bfloat16 tokens, 22 for
-//     fp16 ones, in digits of 7 bits; the sums are exact.  (As fp16 operands the key codes cost 80 of 476 instructions per tile of 16 tokens at d = 128; the
-//     card runs this kernel at its power limit, so that instructions count beside bytes.)
+//   scores, int8: integer products m16n8k32 on the codes as they are; the query in fixed point, 22 bits of its largest element, in digits of 7 bits; the sums are
+//     exact.  (Two digits, 15 bits, lose the small coordinates of a query that has one 1000 times as large: scores then move by per cents.  A third costs 2% at most: 8 x
+//     32,810 tokens 26.7 -> 27.2 us.  As fp16 operands the key codes cost 80 of 476 instructions per tile of 16 tokens at d = 128; the card runs this kernel at its power limit,
+//     so that instructions count beside bytes.)
 //   scores, e4m3: fp16 operands (codes are exact in them, and queries, bfloat16 ones under a power of two).  (mma.sync on e4m3 operands costs more than the
 //     conversions here: 404 instructions per tile against 376.)
 //   values: fp16, exact for both kinds of codes, times the softmax weights under their block's scale as fp16 - for fp16 tokens with a second part: the
@@ -225,7 +226,7 @@ template <int N> __device__ __forceinline__ void digits_of(const float (&x)[4], 
 
 template <int D, bool E4M3, bool FINE> __global__ void __launch_bounds__(AW * 32, AttendPlan<D>::PER_SM) blocks_attend_kernel(const __grid_constant__ BlockAttendParams p, const __grid_constant__ AttendGrid z) {
     using P = AttendPlan<D>;
-    constexpr int ST = P::ST, N = FINE && !E4M3 ? 3 : 2;       // words of a query's four coordinates: digits, or fp16 pairs
+    constexpr int ST = P::ST, N = E4M3 ? 2 : 3;       // words of a query's four coordinates: fp16 pairs, or digits
     constexpr bool bf = !FINE;
     extern __shared__ __align__(16) unsigned char smem[];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
@@ -317,7 +318,7 @@ template <int D, bool E4M3, bool FINE> __global__ void __launch_bounds__(AW * 32
             mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
             q_max = bf ? __uint_as_float(mx << 16) : __half2float(__ushort_as_half(uint16_t(mx)));
             // e4m3: bfloat16 queries under the power of two that takes the largest element to [2^7, 2^8); int8: the largest element in N digits of 7 bits
-            float f = E4M3 ? (bf ? stage_scale(__float_as_uint(q_max)) : 1.f) : q_max > 0.f ? fminf((FINE ? 2080000.f : 16250.f) / q_max, 3.4028235e38f) : 1.f;
+            float f = E4M3 ? (bf ? stage_scale(__float_as_uint(q_max)) : 1.f) : q_max > 0.f ? fminf(2080000.f / q_max, 3.4028235e38f) : 1.f;
             if (!E4M3 && !(q_max <= 3.4028235e38f)) f = __uint_as_float(0x7fffffffu);       // (integers know no NaN: the scale is one)
 #pragma unroll
             for (int w = 0; w < P::KW; ++w) {
@@ -395,7 +396,7 @@ template <int D, bool E4M3, bool FINE> __global__ void __launch_bounds__(AW * 32
                         for (int w = 0; w < P::KW; w += 2) mma_codes(acc[n], k0[w], k1[w], k0[w + 1], k1[w + 1], bq[n][w], bq[n][w + 1]);
                     }
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) s[k] = N == 3 ? float(acc[0][k]) * 16384.f + float(acc[1][k] * 128 + acc[N - 1][k]) : float(acc[0][k] * 128 + acc[1][k]);
+                    for (int k = 0; k < 4; ++k) s[k] = float(acc[0][k]) * 16384.f + float(acc[1][k] * 128 + acc[N - 1][k]);
                 }
             }
             const float kn = __uint_as_float(scales[0]), vn = __uint_as_float(scales[1]);

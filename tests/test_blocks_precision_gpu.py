@@ -1,0 +1,46 @@
+"""How far attention over the 8-bit block cache is from float64, held to bounds relative to sum(w |v|), the weights' own sum over the values: errors of the weights, each
+relative to its weight, cannot move a result by more than that.  (Relative to the largest value, as test_blocks_gpu has it, a result that averages many tokens may be off by several
+per cent of itself.)"""
+
+import pytest
+import torch
+
+from blocks_util import attention
+from test_blocks_gpu import dense, rows, storage
+
+pytestmark = pytest.mark.gpu
+
+CODES = (torch.int8, torch.float8_e4m3fn)
+
+
+@pytest.mark.parametrize("d", (64, 96, 128, 256))
+@pytest.mark.parametrize("codes", CODES)
+@pytest.mark.parametrize("dtype", (torch.float16, torch.bfloat16))
+@pytest.mark.parametrize("t", (1, 3, 40, 300))
+def test_queries_with_one_large_coordinate(d, codes, dtype, t):
+    """A coordinate of the queries 2048 times as large as the others, where the keys are zero: the others decide.
+
+    Queries may be held in 22 bits of their largest element: 2^-22 of it off each, which moves a score by delta = 2^-22 max|q| sum|k| scale at most and the result by
+    2 delta sum(w |v|) - here 0.002 to 0.004 of it; the keys have eight coordinates only so that this is small.  Beside it: weights rounded once to fp16, 2^-11 of sum(w |v|),
+    2^-14 of it for the rest (scores in float32, exponentials), the result's own rounding."""
+    from mlx_turboquant_b200 import blocks
+    b, hq, h, total, scale = 2, 8, 2, 330, d ** -0.5
+    k, v = rows(b, h, total, d, dtype, 1, std=0), rows(b, h, total, d, dtype, 2)
+    few = torch.zeros(d, device="cuda")
+    few[5:d:d // 8] = 3.0
+    k = (k * few).to(dtype)
+    k[..., 0] = 0
+    q = rows(b, hq, t, d, dtype, 3, std=0)
+    q[..., 0] = 2048.0
+    store = storage(b, h, total, d, 32, codes, dtype)
+    blocks.write_blocks(k, v, *store, 0)
+    kd, vd = dense(store, total)
+    for length in (total, 320):                            # (with and without a tail)
+        if length < t:
+            continue
+        ref = attention(q.cpu(), kd[:, :, :length], vd[:, :, :length], scale)
+        delta = 2.0 ** -22 * 2048 * float(kd.abs().sum(-1).max()) * scale
+        wv = attention(q.cpu(), kd[:, :, :length], vd[:, :, :length].abs(), scale)
+        tol = torch.finfo(dtype).eps / 2 * ref.abs() + wv * (2.0 ** -11 + 2.0 ** -14 + 2 * delta)
+        err = (blocks.attend_blocks(q, *store, length).double().cpu() - ref).abs()
+        assert bool((err <= tol).all()), (float((err / tol).max()), float(err.max()), delta)
