@@ -13,8 +13,9 @@
 //     so that instructions count beside bytes.)
 //   scores, e4m3: fp16 operands (codes are exact in them, and queries, bfloat16 ones under a power of two).  (mma.sync on e4m3 operands costs more than the
 //     conversions here: 404 instructions per tile against 376.)
-//   values: fp16, exact for both kinds of codes, times the softmax weights under their block's scale as fp16 - for fp16 tokens with a second part: the
-//     weights' rounding would be as large as the result's own.  (8-bit weights would lose the sum of many small ones.)
+//   values: fp16, exact for both kinds of codes, times the softmax weights under their block's scale as two fp16 parts, 22 bits: one part's rounding is as large as an fp16
+//     result's own, and a tenth of a bfloat16 one's.  The second part costs 0 to 5% (64 sequences x 16,384 tokens, 8 KV heads of 128, bfloat16: 375 to 385 us with and 368 to 385
+//     without it in turn, at the card's power limit; a window of 4096 34.2 and 34.7).
 // Where few (lane, group)s have few tiles each, a cluster of CTAs shares one and joins its sums over distributed shared memory: one launch.
 // blocks_merge_kernel: joins the partials of a row that several CTAs worked on, in their order: results do not depend on which one came first.
 // Measured, 4 heads on 1 at d = 128: int8, 8 lanes x 700 tokens 8.4 us (launch, one tile's chain of latencies, the cluster's joining), 8 x 32,810 26.5 (2.5 TB/s: 18 us of
@@ -162,9 +163,9 @@ struct Cols {
     int pos_min, pos_max;                              // of the group
 };
 
-// Scores of 16 tokens (rows g, g + 8) times their scales -> running softmax -> the weights as the value products' operand, as fp16 and (FINE) what that
+// Scores of 16 tokens (rows g, g + 8) times their scales -> running softmax -> the weights as the value products' operand, as fp16 and what that
 // leaves.  tok: token of row g.
-template <int D, bool FINE>
+template <int D>
 __device__ __forceinline__ void weights(float (&s)[4], float kn0, float kn1, float vn0, float vn1, bool masked, int tok, const Cols& c, int window, int sinks, WarpAcc<D, 0>& st,
                                         uint32_t (&bp)[2], uint32_t (&rest)[2]) {
     s[0] *= kn0 * c.scale[0]; s[1] *= kn0 * c.scale[1];
@@ -196,10 +197,8 @@ __device__ __forceinline__ void weights(float (&s)[4], float kn0, float kn1, flo
     for (int i = 0; i < 2; ++i) {
         const __half2 h = __floats2half2_rn(x[2 * i], x[2 * i + 1]);
         bp[i] = movm_t(*reinterpret_cast<const uint32_t*>(&h));
-        if (FINE) {
-            const float2 hf = __half22float2(h);
-            rest[i] = movm_t(pack_h2(x[2 * i] - hf.x, x[2 * i + 1] - hf.y));
-        }
+        const float2 hf = __half22float2(h);
+        rest[i] = movm_t(pack_h2(x[2 * i] - hf.x, x[2 * i + 1] - hf.y));
     }
 }
 
@@ -224,10 +223,10 @@ template <int N> __device__ __forceinline__ void digits_of(const float (&x)[4], 
     }
 }
 
-template <int D, bool E4M3, bool FINE> __global__ void __launch_bounds__(AW * 32, AttendPlan<D>::PER_SM) blocks_attend_kernel(const __grid_constant__ BlockAttendParams p, const __grid_constant__ AttendGrid z) {
+template <int D, bool E4M3, bool BF> __global__ void __launch_bounds__(AW * 32, AttendPlan<D>::PER_SM) blocks_attend_kernel(const __grid_constant__ BlockAttendParams p, const __grid_constant__ AttendGrid z) {
     using P = AttendPlan<D>;
     constexpr int ST = P::ST, N = E4M3 ? 2 : 3;       // words of a query's four coordinates: fp16 pairs, or digits
-    constexpr bool bf = !FINE;
+    constexpr bool bf = BF;
     extern __shared__ __align__(16) unsigned char smem[];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
     // a run of tiles, or the rank's share of a (lane, group)
@@ -401,7 +400,7 @@ template <int D, bool E4M3, bool FINE> __global__ void __launch_bounds__(AW * 32
             }
             const float kn = __uint_as_float(scales[0]), vn = __uint_as_float(scales[1]);
             uint32_t bp[2], rest[2];
-            weights<D, FINE>(s, kn, kn, vn, vn, !whole(tok), tok + g, c, p.window, p.sinks, st, bp, rest);
+            weights<D>(s, kn, kn, vn, vn, !whole(tok), tok + g, c, p.window, p.sinks, st, bp, rest);
             uint32_t v[4][P::VW];
 #pragma unroll
             for (int r = 0; r < 4; ++r) value_row<D>(src + P::SIDE, 2 * t + (r & 1) + 8 * (r >> 1), g, v[r]);
@@ -415,10 +414,8 @@ template <int D, bool E4M3, bool FINE> __global__ void __launch_bounds__(AW * 32
                 halves<E4M3>(__byte_perm(v[2][w], v[3][w], 0x7362), e[2], e[3]);
                 mma16816(st.o[2 * w], a[0], a[1], a[2], a[3], bp[0], bp[1]);
                 mma16816(st.o[2 * w + 1], e[0], e[1], e[2], e[3], bp[0], bp[1]);
-                if (FINE) {
-                    mma16816(st.o[2 * w], a[0], a[1], a[2], a[3], rest[0], rest[1]);
-                    mma16816(st.o[2 * w + 1], e[0], e[1], e[2], e[3], rest[0], rest[1]);
-                }
+                mma16816(st.o[2 * w], a[0], a[1], a[2], a[3], rest[0], rest[1]);
+                mma16816(st.o[2 * w + 1], e[0], e[1], e[2], e[3], rest[0], rest[1]);
             }
         }
         cp_async_wait<0>();
@@ -520,7 +517,7 @@ template <int D, bool E4M3, bool FINE> __global__ void __launch_bounds__(AW * 32
                 if (vn[r] != vn[r]) { kn[r] = vn[r]; vn[r] = 0.f; }
             }
             uint32_t bp[2], rest[2];
-            weights<D, FINE>(s, kn[0], kn[1], vn[0], vn[1], true, tok + g, ct, p.window, p.sinks, st, bp, rest);
+            weights<D>(s, kn[0], kn[1], vn[0], vn[1], true, tok + g, ct, p.window, p.sinks, st, bp, rest);
 #pragma unroll
             for (int w = 0; w < P::VW; ++w) {
 #pragma unroll
@@ -528,7 +525,7 @@ template <int D, bool E4M3, bool FINE> __global__ void __launch_bounds__(AW * 32
                     const uint32_t x0 = i ? v[0][w].y : v[0][w].x, x1 = i ? v[1][w].y : v[1][w].x, x2 = i ? v[2][w].y : v[2][w].x, x3 = i ? v[3][w].y : v[3][w].x;
                     const uint32_t a0 = __byte_perm(x0, x1, 0x5410), a1 = __byte_perm(x0, x1, 0x7632), a2 = __byte_perm(x2, x3, 0x5410), a3 = __byte_perm(x2, x3, 0x7632);
                     mma16816(st.o[2 * w + i], a0, a1, a2, a3, bp[0], bp[1]);
-                    if (FINE) mma16816(st.o[2 * w + i], a0, a1, a2, a3, rest[0], rest[1]);
+                    mma16816(st.o[2 * w + i], a0, a1, a2, a3, rest[0], rest[1]);
                 }
             }
         }
@@ -781,9 +778,9 @@ template <int D> int launch_split(const BlockAttendParams& p, cudaStream_t s) {
     cfg.stream = s;
     cfg.attrs = attr;
     cfg.numAttrs = z.cluster > 1 ? 2 : 1;
-    const bool fine = p.dtype == TQ_F16;
-    cudaLaunchKernelEx(&cfg, p.e4m3 ? (fine ? blocks_attend_kernel<D, true, true> : blocks_attend_kernel<D, true, false>)
-                                    : (fine ? blocks_attend_kernel<D, false, true> : blocks_attend_kernel<D, false, false>), p, z);
+    const bool bf = p.dtype == TQ_BF16;
+    cudaLaunchKernelEx(&cfg, p.e4m3 ? (bf ? blocks_attend_kernel<D, true, true> : blocks_attend_kernel<D, true, false>)
+                                    : (bf ? blocks_attend_kernel<D, false, true> : blocks_attend_kernel<D, false, false>), p, z);
     if (int rc = check_launch("tq_blocks_attend")) return rc;
     if (!z.merge) return TQ_OK;
     cfg.numAttrs = 1;

@@ -44,3 +44,27 @@ def test_queries_with_one_large_coordinate(d, codes, dtype, t):
         tol = torch.finfo(dtype).eps / 2 * ref.abs() + wv * (2.0 ** -11 + 2.0 ** -14 + 2 * delta)
         err = (blocks.attend_blocks(q, *store, length).double().cpu() - ref).abs()
         assert bool((err <= tol).all()), (float((err / tol).max()), float(err.max()), delta)
+
+
+@pytest.mark.parametrize("d", (64, 96, 128, 256))
+@pytest.mark.parametrize("codes", CODES)
+@pytest.mark.parametrize("dtype", (torch.float16, torch.bfloat16))
+@pytest.mark.parametrize("total", (2, 3, 17, 40, 330, 1000))
+def test_weights_of_few_queries_are_not_rounded_to_16_bits(d, codes, dtype, total):
+    """One token, and three: beside the result's own rounding 2^-14 of sum(w |v|), where weights rounded once would take 2^-11.
+
+    Queries in 22 bits move scores by 2^-22 max|q| sum|k| scale < 2^-22 * 5 * 256 * 2 / 8, 2^-15 of a weight at most, twice; exponentials, float32 scores and scales
+    2^-20; two fp16 parts 2^-22, or where they end 2^-25 of the largest weight for each token, 2^-15 over a thousand."""
+    from mlx_turboquant_b200 import blocks
+    b, hq, h, scale = 2, 16, 2, d ** -0.5
+    store = storage(b, h, total, d, 16, codes, dtype)
+    blocks.write_blocks(rows(b, h, total, d, dtype, 1, std=0), rows(b, h, total, d, dtype, 2), *store, 0)
+    kd, vd = dense(store, total)
+    for t in (1, 3):
+        if t > total:
+            continue
+        q = rows(b, hq, t, d, dtype, 3, std=0)
+        ref, wv = (attention(q.cpu(), kd, x, scale) for x in (vd, vd.abs()))
+        err = (blocks.attend_blocks(q, *store, total).double().cpu() - ref).abs()
+        tol = torch.finfo(dtype).eps / 2 * ref.abs() + 2.0 ** -14 * wv + (2.0 ** -25 if dtype is torch.float16 else 0.0)       # (half a step of fp16's subnormals)
+        assert bool((err <= tol).all()), (float((err / tol).max()), t)
