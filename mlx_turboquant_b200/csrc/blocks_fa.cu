@@ -6,7 +6,9 @@
 // blocks_fa_kernel: one CTA per SM takes a run of the flat sequence (lane x head group, row block, key tile): a row block each where there are few, otherwise whole row
 // blocks or equal runs wherever that cuts them, by what each costs (divide()); a row block is NQ tiles of 128 rows = 128 / GP query tokens x the GP query heads of a GQA group.
 //   * 8 NQ softmax warps, two rows' shares per thread: tcgen05.ld of the scores as fragments, one packed multiply-add each, ex2 (a quarter of them
-//     by a polynomial), P (fp16) back into tensor memory; a row's reference maximum is looked at through its sum.  They also lay out their rows of the queries, the next row block's before they write
+//     by a polynomial), P back into tensor memory: fp16 (rounded once, a tenth of what a bfloat16 result loses to its own rounding), for fp16 tokens in two parts (one part's
+//     rounding would be as large as the result's own: 0.00029 from float64 where two parts have the 0.00021 of the rounding alone; in one run of both 2048 queries over 16,384
+//     tokens took 472 us with one part, 593 with two, a window of 1024 72 and 81); a row's reference maximum is looked at through its sum.  They also lay out their rows of the queries, the next row block's before they write
 //     this one's results;
 //   * a warp per query tile issues S = Q K^T and O += P V, scores two key tiles ahead (N = 64: 48 clocks an instruction with Q in shared memory, of 32 with it in tensor
 //     memory, where there is no room for it; 620 a tile and query tile with the values' products);
@@ -17,7 +19,7 @@
 //       tiles per lane, where writing fp16 rows and reading them back would cost more than the products.
 // blocks_fa_merge_kernel joins the partials of row blocks that several CTAs worked on, in their order.
 //
-// Measured: 2048 queries over 16,384 tokens, 32 heads on 8, d = 128: 535 us, of 309 at the measured rate of products (960 TFLOP/s); expansion 20 and merge 19 of it.
+// Measured: 2048 queries over 16,384 tokens, 32 heads on 8, d = 128: 535 us = 960 TFLOP/s (309 at the 1668 that a large product reaches); expansion 20 and merge 19 of it.
 // Bound by both together: of some 1900 clocks per pair of query tiles and key tile the tensor pipe is busy 1240 and the special-function unit 770; a score buffer is full again some
 // 1600 after its weights (both query tiles' products, in one queue), and a tile's softmax takes 1350, issue slots shared with the other query tile's. Tried without gain: a warp for
 // scores and another for results (574), weights in tensor-memory buffers of their own (550), the values' scale in the exponent (542), naps between looks at barriers, key tiles of 128
@@ -155,7 +157,7 @@ __device__ __forceinline__ u64 ex2_by_fma(float x0, float x1) {
 }
 constexpr int POLY_EVERY = 4;                          // (none 551 us for 2048 queries x 16,384, every fourth pair 539, every second 570: issue)
 
-template <int D, bool FUSED>
+template <int D, bool FUSED, bool FINE>
 __global__ void __launch_bounds__(Plan<D, FUSED>::NT, 1) blocks_fa_kernel(const __grid_constant__ Params p) {
     using P = Plan<D, FUSED>;
     constexpr int NQ = P::NQ, DP = P::DP, SB = P::SB, ST = P::ST;
@@ -408,9 +410,11 @@ __global__ void __launch_bounds__(Plan<D, FUSED>::NT, 1) blocks_fa_kernel(const 
             auto issue_pv = [&](int j) {                           // O += P V
                 const uint32_t a = tmem + sbuf(q, j) * TN;
 #pragma unroll
-                for (int ks = 0; ks < TN / 16; ++ks)
-                    umma_ts(tmem + P::COL_O + q * DP, a + ks * 8, desc_mn(sbase + P::OFF_V + (j % ST) * P::K_TILE, P::KBLK, ks), idesc_of(DP, true),
-                            (j > j0 || ks > 0) ? 1u : 0u);
+                for (int ks = 0; ks < TN / 16; ++ks) {
+                    const uint64_t v = desc_mn(sbase + P::OFF_V + (j % ST) * P::K_TILE, P::KBLK, ks);
+                    umma_ts(tmem + P::COL_O + q * DP, a + ks * 8, v, idesc_of(DP, true), (j > j0 || ks > 0) ? 1u : 0u);
+                    if (FINE) umma_ts(tmem + P::COL_O + q * DP, a + TN / 2 + ks * 8, v, idesc_of(DP, true), 1u);
+                }
                 umma_commit(bar(O_DONE + q));
                 umma_commit(bar(V_FREE + j % ST));
                 if (j == j0 + n - 1) umma_commit(bar(ALL_DONE + q));       // (a barrier of its own: a parity wait on O_DONE could be two phases early or one late)
@@ -601,7 +605,7 @@ __global__ void __launch_bounds__(Plan<D, FUSED>::NT, 1) blocks_fa_kernel(const 
 #pragma unroll
                     for (int r = 0; r < NR; ++r) nv[r] = *reinterpret_cast<const u64*>(vn + 8 * r);
                 }
-                uint32_t w[2 * NR];
+                uint32_t w[2 * NR], rest[FINE ? 2 * NR : 1];       // the weights as fp16, and what that leaves
                 u64 ls[2];
                 auto weigh = [&](auto scale_of, auto sharing) {
                     ls[0] = ls[1] = pk(0.f, 0.f);
@@ -614,7 +618,12 @@ __global__ void __launch_bounds__(Plan<D, FUSED>::NT, 1) blocks_fa_kernel(const 
                             ls[k] = add2(ls[k], x);
                             float x0, x1;
                             upk(mul2(x, scale_of(r)), x0, x1);
-                            w[2 * r + k] = pack_h2(x0, x1);
+                            const __half2 h = __floats2half2_rn(x0, x1);
+                            w[2 * r + k] = *reinterpret_cast<const uint32_t*>(&h);
+                            if constexpr (FINE) {
+                                const float2 hf = __half22float2(h);
+                                rest[2 * r + k] = pack_h2(x0 - hf.x, x1 - hf.y);
+                            }
                         }
                 };
 #pragma unroll 1
@@ -686,6 +695,7 @@ __global__ void __launch_bounds__(Plan<D, FUSED>::NT, 1) blocks_fa_kernel(const 
                 l2[0] = add2(l2[0], ls[0]);
                 l2[1] = add2(l2[1], ls[1]);
                 tmem_st_half64(s_col, w);
+                if constexpr (FINE) tmem_st_half64(s_col + TN / 2, rest);
                 tmem_st_wait();
                 tc_fence_before();
                 mbar_arrive(bar(P_FULL + sbuf(q, j)));
@@ -962,7 +972,9 @@ template <int D, bool FUSED> int launch(const BlockAttendParams& a, unsigned cha
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess) dev = -1;
     if (dev < 0 || dev >= 64 || !set[dev].load()) {
-        const cudaError_t e = cudaFuncSetAttribute(blocks_fa_kernel<D, FUSED>, cudaFuncAttributeMaxDynamicSharedMemorySize, int(P::SMEM));
+        cudaError_t e = cudaSuccess;
+        for (auto* k : {blocks_fa_kernel<D, FUSED, false>, blocks_fa_kernel<D, FUSED, true>})
+            if (e == cudaSuccess) e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, int(P::SMEM));
         if (e != cudaSuccess) return fail(TQ_ERR_LAUNCH, "tq_blocks_attend: shared memory %zu B: %s", P::SMEM, cudaGetErrorString(e));
         if (dev >= 0 && dev < 64) set[dev].store(true);
     }
@@ -991,7 +1003,7 @@ template <int D, bool FUSED> int launch(const BlockAttendParams& a, unsigned cha
         cfg.gridDim = dim3(unsigned(p.ctas));
         cfg.blockDim = dim3(P::NT);
         cfg.dynamicSmemBytes = P::SMEM;
-        cudaLaunchKernelEx(&cfg, blocks_fa_kernel<D, FUSED>, p);
+        cudaLaunchKernelEx(&cfg, a.dtype == TQ_F16 ? blocks_fa_kernel<D, FUSED, true> : blocks_fa_kernel<D, FUSED, false>, p);
         if (int rc = check_launch("tq_blocks_attend")) return rc;
         bool split = false;
         for (int i = 1; i < p.ctas; ++i) split = split || p.start[i].tile > 0;

@@ -68,3 +68,22 @@ def test_weights_of_few_queries_are_not_rounded_to_16_bits(d, codes, dtype, tota
         err = (blocks.attend_blocks(q, *store, total).double().cpu() - ref).abs()
         tol = torch.finfo(dtype).eps / 2 * ref.abs() + 2.0 ** -14 * wv + (2.0 ** -25 if dtype is torch.float16 else 0.0)       # (half a step of fp16's subnormals)
         assert bool((err <= tol).all()), (float((err / tol).max()), t)
+
+
+@pytest.mark.parametrize("d", (64, 96, 128, 256))
+@pytest.mark.parametrize("codes", CODES)
+@pytest.mark.parametrize("block", (16, 64))
+@pytest.mark.parametrize("b,total,t", ((1, 70, 70), (1, 1000, 130), (2, 1500, 600), (16, 330, 40)))
+def test_fp16_prompts_are_as_precise_as_their_decoding(d, codes, block, b, total, t):
+    """Many query rows of fp16 tokens: 2^-14 of sum(w |v|) beside the result's own rounding, as above (exponentials to 2^-16.9, twice; fp16 queries are exact here)."""
+    from mlx_turboquant_b200 import blocks
+    h, hq, scale, dtype = 2, 16, d ** -0.5, torch.float16
+    store = storage(b, h, total, d, block, codes, dtype)
+    blocks.write_blocks(rows(b, h, total, d, dtype, 1, std=0), rows(b, h, total, d, dtype, 2), *store, 0)
+    kd, vd = dense(store, total)
+    q = rows(b, hq, t, d, dtype, 3, std=0)
+    for window, sinks in ((None, 0), (50, 4)):
+        ref, wv = (attention(q.cpu(), kd, x, scale, window, sinks) for x in (vd, vd.abs()))
+        err = (blocks.attend_blocks(q, *store, total, window=window, sinks=sinks).double().cpu() - ref).abs()
+        tol = torch.finfo(dtype).eps / 2 * ref.abs() + 2.0 ** -14 * wv + 2.0 ** -25
+        assert bool((err <= tol).all()), (float((err / tol).max()), window)
