@@ -424,9 +424,16 @@ typedef struct {
     int64_t window, sinks;
     tq_new_rows k_new, v_new;             /* (batch, n_kv_heads, 1, d), or x == NULL */
     void* out;                            /* (batch, n_q_heads, t_q, d) of store.dtype, contiguous */
-    void* workspace; size_t workspace_bytes;      /* tq_blocks_attend_workspace(...) bytes, 256-byte aligned, any content */
+    void* workspace; size_t workspace_bytes;      /* tq_blocks_attend_workspace(...) bytes, 256-byte aligned, any content; with fewer, or none, a slower way runs */
 } tq_blocks_attend_args;
+/* What the fastest way wants; what the fastest way wants that makes do with `room` bytes. */
 size_t tq_blocks_attend_workspace(const tq_blocks_attend_args* a);
+size_t tq_blocks_attend_workspace_within(const tq_blocks_attend_args* a, size_t room);
+/* The way that a call with workspace_bytes of scratch takes (the address is not looked at): CUDA cores; a CTA per (KV head, eight query rows), runs of the tokens over all CTAs and a
+ * merge, or a cluster of CTAs; tensor cores with codes converted in the attention kernel or once in front of it, row blocks whole or cut.  Negative: the arguments are invalid. */
+enum { TQ_BLOCKS_NOTHING = 0, TQ_BLOCKS_PLAIN = 1, TQ_BLOCKS_ALONE = 2, TQ_BLOCKS_RUNS = 3, TQ_BLOCKS_CLUSTER = 4, TQ_BLOCKS_FUSED = 5, TQ_BLOCKS_FUSED_CUT = 6,
+       TQ_BLOCKS_EXPANDED = 7, TQ_BLOCKS_EXPANDED_CUT = 8 };
+int tq_blocks_attend_choice(const tq_blocks_attend_args* a);
 int tq_blocks_attend(const tq_blocks_attend_args* a, void* stream);
 
 #ifdef __cplusplus

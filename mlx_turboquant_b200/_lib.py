@@ -162,6 +162,8 @@ PROTOTYPES = {
     "tq_blocks_write": (_i, [C.POINTER(BlockStore), C.POINTER(NewRows), C.POINTER(NewRows), _i64, _vp]),
     "tq_blocks_read": (_i, [C.POINTER(BlockStore), _vp, _vp, _i, _vp]),
     "tq_blocks_attend_workspace": (_sz, [C.POINTER(BlocksAttendArgs)]),
+    "tq_blocks_attend_workspace_within": (_sz, [C.POINTER(BlocksAttendArgs), _sz]),
+    "tq_blocks_attend_choice": (_i, [C.POINTER(BlocksAttendArgs)]),
     "tq_blocks_attend": (_i, [C.POINTER(BlocksAttendArgs), _vp]),
     "tq_peer_buffer_create": (_i, [_sz, C.POINTER(_vp), C.c_char_p]),
     "tq_peer_buffer_open": (_i, [C.c_char_p, _i, C.POINTER(_vp)]),

@@ -19,10 +19,11 @@ from typing import Any
 
 import torch
 
-from . import _lib
+from . import _lib, kernels
 
 CODE_TYPES = {torch.int8: _lib.TQ_CODE_INT8, torch.float8_e4m3fn: _lib.TQ_CODE_E4M3}
 BLOCKS = (16, 32, 64, 128)
+SMALL = 64 << 20               # scratch that a call makes do with on a card without room for what it would like
 
 
 def head_dim_ok(d: int) -> bool:
@@ -133,7 +134,9 @@ def attend_blocks(queries: torch.Tensor, k_codes, k_scales, v_codes, v_scales, k
     ``queries`` (B, H_q, T_q, D) of the tails' type; H_q a multiple of H.  With ``window`` a query sees the last ``window`` tokens up to its own and
     the first ``sinks`` of the cache.  ``new`` = (keys, values), (B, H, 1, D): one more token, which joins the cache and is attended to, in the
     same launch unless it completes a block (the cache then holds ``length + 1`` tokens).  ``out`` (contiguous, the queries' shape and type)
-    receives the result and must not overlap what is read."""
+    receives the result and must not overlap what is read.
+
+    Long pieces of a prompt take up to some 600 MB of scratch while they run; without room for that the call takes ways that need less."""
     if window != 0:
         res = _lib.host().blocks_attend(queries, k_codes, k_scales, v_codes, v_scales, k_tail, v_tail, length, window or 0, sinks, scale,
                                         *(new if new is not None else (None, None)), out)
@@ -177,11 +180,12 @@ def attend_blocks(queries: torch.Tensor, k_codes, k_scales, v_codes, v_scales, k
     a.window, a.sinks = min(int(window or 0), 1 << 62), min(int(sinks), 1 << 62)
     if out.numel() == 0:
         return out
-    # Any content, so that the allocator's memory serves: one call's scratch is its own, in captured graphs and on every stream.
+    # Any content, so that the allocator's memory serves: one call's scratch is its own, in captured graphs and on every stream.  On a card without room for it, slower ways run that
+    # make do with little, or with none.
     need = int(_lib.launch(dev, "tq_blocks_attend_workspace", C.byref(a)))
     if need:
-        ws = torch.empty(need, dtype=torch.uint8, device=dev)
-        a.workspace, a.workspace_bytes = ws.data_ptr(), need
+        ws = kernels.scratch(dev, lambda: need, lambda: int(_lib.launch(dev, "tq_blocks_attend_workspace_within", C.byref(a), min(need - 1, SMALL))))
+        a.workspace, a.workspace_bytes = (None, 0) if ws is None else (ws.data_ptr(), ws.numel())
     _lib.check(_lib.launch(dev, "tq_blocks_attend", C.byref(a), _lib.stream_ptr(dev)))
     return out
 

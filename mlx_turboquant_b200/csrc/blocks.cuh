@@ -33,12 +33,14 @@ struct BlockAttendParams {
     int window, sinks;                       // window: INT_MAX / 2 without one
     float scale_log2;                        // scale * log2(e)
     float* part;                             // workspace
+    size_t room;                             // its bytes; all there may be where only the need is asked
 };
 
 int launch_blocks_plain(const BlockAttendParams& p, cudaStream_t s);
 double blocks_split_us(const BlockAttendParams& p);      // what a call is expected to cost in blocks_attend.cu's kernel
 bool blocks_fa_takes(const BlockAttendParams& p);
 size_t blocks_fa_workspace(const BlockAttendParams& p);
+int blocks_fa_choice(const BlockAttendParams& p);        // TQ_BLOCKS_FUSED ... TQ_BLOCKS_EXPANDED_CUT
 int launch_blocks_fa(const BlockAttendParams& p, cudaStream_t s);
 
 // The first token that some query sees through its window, and how many sink tokens lie before it

@@ -731,12 +731,13 @@ template <int D> AttendGrid grid_of(const BlockAttendParams& p) {
     z.per = uint32_t(std::max<int64_t>(AW, (units + ctas - 1) / ctas));
     z.slots = std::min((z.n_units - 2) / int(z.per) + 2, z.n_units);
     z.merge = z.per % uint32_t(z.n_units) != 0;            // (otherwise every row has one CTA)
+    const bool fits = !z.merge || size_t(jobs) * z.slots * HPG * P::RS * sizeof(float) <= p.room;
     // A (lane, group) in one launch, by a cluster of up to eight CTAs, or runs of tiles over the whole card and a merge.  In us, fitted to 190 calls at d = 64, 128 and 256
     // (8 to 256 lanes, 1 to 16 groups, 100 to 16,000 tokens; the choice is within 1% of the best on the mean, 20% at the worst): a tile at d = 128 0.15 with one CTA on an SM
     // and 0.18 with two, a wave of CTAs 7, every further (lane, group) in a run 12, a cluster's joining 2.5, the merge 8 and 4 for every thousand partials.
     const double width = D <= 64 ? 0.52 : D <= 96 ? 0.76 : D <= 128 ? 1.0 : 1.3;
     auto tile_us = [&](int64_t n) { return width * (P::PER_SM == 2 && n * 2 > ctas ? 0.18 : 0.15); };
-    z.us = double(z.per) * tile_us((units + z.per - 1) / z.per) + 7.0 + 12.0 * std::max(0.0, double(z.per) / z.n_units - 0.5) + (z.merge ? 8.0 + 0.004 * double(jobs) * z.slots : 0.0);
+    z.us = !fits ? 1e29 : double(z.per) * tile_us((units + z.per - 1) / z.per) + 7.0 + 12.0 * std::max(0.0, double(z.per) / z.n_units - 0.5) + (z.merge ? 8.0 + 0.004 * double(jobs) * z.slots : 0.0);
     for (int c = 1; c <= 8 && (c == 1 || c * AW <= z.n_units + AW - 1); ++c) {
         const int64_t n = c == 1 ? ctas : clusters_at_once<D>(c);
         if (n <= 0) continue;
@@ -749,6 +750,11 @@ template <int D> size_t split_workspace(const BlockAttendParams& p) {
     const AttendGrid z = grid_of<D>(p);
     if (!z.merge) return 0;
     return size_t(z.jobs) * z.slots * HPG * AttendPlan<D>::RS * sizeof(float);
+}
+
+template <int D> int split_choice(const BlockAttendParams& p) {
+    const AttendGrid z = grid_of<D>(p);
+    return z.cluster > 1 ? TQ_BLOCKS_CLUSTER : z.merge ? TQ_BLOCKS_RUNS : TQ_BLOCKS_ALONE;
 }
 
 template <int D> int launch_split(const BlockAttendParams& p, cudaStream_t s) {
@@ -828,7 +834,9 @@ int prepare(const tq_blocks_attend_args* a, BlockAttendParams& p, bool& done) {
     p.window = a->window > 0 ? int(std::min<int64_t>(a->window, INT_MAX / 2)) : INT_MAX / 2;
     p.sinks = int(std::min<int64_t>(a->sinks, INT_MAX / 2));
     p.scale_log2 = a->scale * LOG2E;
+    if (a->workspace && !aligned(a->workspace, 256)) return fail(TQ_ERR_INVALID, "%s: the workspace must be 256-byte aligned", what);
     p.part = static_cast<float*>(a->workspace);
+    p.room = a->workspace_bytes;
     return TQ_OK;
 }
 
@@ -860,11 +868,24 @@ int launch_blocks_plain(const BlockAttendParams& p, cudaStream_t s) {
 
 }  // namespace tq
 
-extern "C" size_t tq_blocks_attend_workspace(const tq_blocks_attend_args* a) {
+extern "C" size_t tq_blocks_attend_workspace_within(const tq_blocks_attend_args* a, size_t room) {
     tq::BlockAttendParams p;
     bool done = false;
     if (tq::prepare(a, p, done) != TQ_OK || done) return 0;
+    p.room = room;
     return tq::workspace_of(p);
+}
+
+extern "C" size_t tq_blocks_attend_workspace(const tq_blocks_attend_args* a) { return tq_blocks_attend_workspace_within(a, SIZE_MAX); }
+
+extern "C" int tq_blocks_attend_choice(const tq_blocks_attend_args* a) {
+    tq::BlockAttendParams p;
+    bool done = false;
+    if (int rc = tq::prepare(a, p, done)) return rc;
+    if (done) return TQ_BLOCKS_NOTHING;
+    if (!tq::split_takes(p)) return TQ_BLOCKS_PLAIN;
+    if (tq::blocks_fa_takes(p)) return tq::blocks_fa_choice(p);
+    return p.D == 64 ? tq::split_choice<64>(p) : p.D == 96 ? tq::split_choice<96>(p) : p.D == 128 ? tq::split_choice<128>(p) : tq::split_choice<256>(p);
 }
 
 extern "C" int tq_blocks_attend(const tq_blocks_attend_args* a, void* stream) {
@@ -874,10 +895,8 @@ extern "C" int tq_blocks_attend(const tq_blocks_attend_args* a, void* stream) {
     if (int rc = prepare(a, p, done)) return rc;
     if (done) return TQ_OK;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
+    if (!a->workspace) p.room = 0;
     if (!split_takes(p)) return launch_blocks_plain(p, s);
-    const size_t need = workspace_of(p);
-    if (need > 0 && (!a->workspace || !aligned(a->workspace, 256) || a->workspace_bytes < need))
-        return fail(TQ_ERR_INVALID, "tq_blocks_attend: workspace %zu B < %zu B, or not 256-byte aligned", a->workspace_bytes, need);
     if (blocks_fa_takes(p)) return launch_blocks_fa(p, s);
     if (p.D == 64) return launch_split<64>(p, s);
     if (p.D == 96) return launch_split<96>(p, s);

@@ -899,21 +899,26 @@ size_t up(size_t v) { return (v + 255) / 256 * 256; }
 
 // How a call is laid out: row blocks, and in the workspace the partials, then (expanded) tiles and scales of `chunk` cache lanes at a time
 constexpr size_t WS_CAP = size_t(1) << 29;
-struct Layout { int HG, GP, QT, n_blk, chunk, ctas; Tiles all; size_t tiles, scales, bytes; };
+struct Layout { int HG, GP, QT, n_blk, chunk, ctas; Tiles all; size_t tiles, scales, bytes; int more; };      // more: rounds that want of room adds
 template <int D, bool FUSED> Layout layout_of(const BlockAttendParams& p) {
     using P = Plan<D, FUSED>;
     const int g = std::min(p.G, HPG), lanes = p.B * p.Hkv;
-    Layout l{(p.G + HPG - 1) / HPG, g <= 1 ? 1 : g <= 2 ? 2 : g <= 4 ? 4 : 8, 0, 0, lanes, 0, Tiles(p, p.total - p.Tq, p.total - 1), 0, 0, 0};
+    Layout l{(p.G + HPG - 1) / HPG, g <= 1 ? 1 : g <= 2 ? 2 : g <= 4 ? 4 : 8, 0, 0, lanes, 0, Tiles(p, p.total - p.Tq, p.total - 1), 0, 0, 0, 0};
     l.QT = TM / l.GP;
     l.n_blk = (p.Tq + P::NQ * l.QT - 1) / (P::NQ * l.QT);
     const int sms = std::min(blocks_sm_count(), MAX_CTAS);
     const size_t lane_tiles = size_t(l.all.n) * 2 * P::K_TILE, lane_scales = size_t(l.all.n) * P::SC;
+    auto set = [&]() {
+        l.ctas = int(std::min<int64_t>(sms, int64_t(l.chunk) * l.HG * l.n_blk * l.all.n));
+        l.tiles = up(size_t(l.ctas) * 2 * P::ROWS * (D + 4) * sizeof(float));
+        l.scales = l.tiles + (FUSED ? 0 : up(l.chunk * lane_tiles));
+        l.bytes = l.scales + (FUSED ? 0 : up(l.chunk * lane_scales));
+    };
     if (!FUSED)
         while (l.chunk > 1 && size_t(l.chunk) * (lane_tiles + lane_scales) > WS_CAP) l.chunk = (l.chunk + 1) / 2;
-    l.ctas = int(std::min<int64_t>(sms, int64_t(l.chunk) * l.HG * l.n_blk * l.all.n));
-    l.tiles = up(size_t(l.ctas) * 2 * P::ROWS * (D + 4) * sizeof(float));
-    l.scales = l.tiles + (FUSED ? 0 : up(l.chunk * lane_tiles));
-    l.bytes = l.scales + (FUSED ? 0 : up(l.chunk * lane_scales));
+    const int chunk = l.chunk;
+    for (set(); !FUSED && l.chunk > 1 && l.bytes > p.room; set()) l.chunk = (l.chunk + 1) / 2;
+    l.more = (lanes + l.chunk - 1) / l.chunk - (lanes + chunk - 1) / chunk;
     return l;
 }
 
@@ -965,6 +970,15 @@ template <int D, bool FUSED> void divide(Params& p, int lanes) {
     if (double(whole - (total + most - 1) / most) * tile_us > cut_us) fill(false);
 }
 
+Params params_of(const BlockAttendParams& a, const Layout& l, unsigned char* ws) {
+    return Params{a, 0, l.HG, l.GP, l.QT, l.n_blk, l.ctas, {}, reinterpret_cast<float*>(ws), ws + l.tiles, reinterpret_cast<const float*>(ws + l.scales), l.all, nullptr};
+}
+bool cuts(const Params& p) {
+    bool any = false;
+    for (int i = 1; i < p.ctas; ++i) any = any || p.start[i].tile > 0;
+    return any;
+}
+
 template <int D, bool FUSED> int launch(const BlockAttendParams& a, unsigned char* ws, cudaStream_t st) {
     using P = Plan<D, FUSED>;
     const Layout l = layout_of<D, FUSED>(a);
@@ -978,8 +992,8 @@ template <int D, bool FUSED> int launch(const BlockAttendParams& a, unsigned cha
         if (e != cudaSuccess) return fail(TQ_ERR_LAUNCH, "tq_blocks_attend: shared memory %zu B: %s", P::SMEM, cudaGetErrorString(e));
         if (dev >= 0 && dev < 64) set[dev].store(true);
     }
-    Params p{a, 0, l.HG, l.GP, l.QT, l.n_blk, 0, {}, reinterpret_cast<float*>(ws), ws + l.tiles, reinterpret_cast<const float*>(ws + l.scales), l.all, decode_status_ptr()};
-    if (!p.status) return fail(TQ_ERR_LAUNCH, "tq_blocks_attend: cannot locate the status word");
+    Params p = params_of(a, l, ws);
+    if (!(p.status = decode_status_ptr())) return fail(TQ_ERR_LAUNCH, "tq_blocks_attend: cannot locate the status word");
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
@@ -1005,9 +1019,7 @@ template <int D, bool FUSED> int launch(const BlockAttendParams& a, unsigned cha
         cfg.dynamicSmemBytes = P::SMEM;
         cudaLaunchKernelEx(&cfg, a.dtype == TQ_F16 ? blocks_fa_kernel<D, FUSED, true> : blocks_fa_kernel<D, FUSED, false>, p);
         if (int rc = check_launch("tq_blocks_attend")) return rc;
-        bool split = false;
-        for (int i = 1; i < p.ctas; ++i) split = split || p.start[i].tile > 0;
-        if (!split) continue;
+        if (!cuts(p)) continue;
         cfg.gridDim = dim3(unsigned(p.ctas - 1) * (P::ROWS / 8));
         cfg.blockDim = dim3(256);
         cfg.dynamicSmemBytes = 0;
@@ -1023,13 +1035,14 @@ template <int D, bool FUSED> int launch(const BlockAttendParams& a, unsigned cha
 // 217 / 221, 384 322 / 296, 512 432 / 319; 64 lanes x 700, 256 22 / 32, 1024 67 / 48.
 template <int D, bool FUSED> double cost(const BlockAttendParams& p) {
     const Layout l = layout_of<D, FUSED>(p);
+    if (l.bytes > p.room) return 1e30;
     const int64_t lanes = int64_t(p.B) * p.Hkv, jobs = lanes * l.HG * l.n_blk, sms = blocks_sm_count();
     const int rows = Plan<D, FUSED>::NQ * l.QT;
     double n = 0;                                          // tiles of a row block, on the mean of the first and the last
     for (int blk : {0, l.n_blk - 1}) n += 0.5 * Tiles(p, p.total - p.Tq + blk * rows, p.total - p.Tq + std::min((blk + 1) * rows, p.Tq) - 1).n;
     const double tile = (FUSED ? 1.3 : 1.1) * (D <= 64 ? 0.7 : D <= 96 ? 0.85 : D <= 128 ? 1.0 : 0.86), runs = std::min(double(sms), double(jobs) * n / 4);
     const double whole = double((jobs + sms - 1) / sms) * n * tile, cut = std::max(4.0, double(jobs) * n / double(sms)) * tile + 3.2 + 4.6e-7 * runs * 2 * Plan<D, FUSED>::ROWS * (D + 4) * 4;
-    return 7.7 + (runs < double(jobs) ? whole : std::min(whole, cut)) + (FUSED ? 0.0 : 4.0 + 2.1e-7 * double(lanes) * l.all.n * TN * 6 * D);
+    return 7.7 + 12.0 * l.more + (runs < double(jobs) ? whole : std::min(whole, cut)) + (FUSED ? 0.0 : 4.0 + 2.1e-7 * double(lanes) * l.all.n * TN * 6 * D);
 }
 // Whether the codes are converted in the attention kernel (not at d = 256, where its eight converting warps cannot keep up: 3 times the other way's time).
 template <int D> bool fused(const BlockAttendParams& p) {
@@ -1044,6 +1057,17 @@ template <int D> size_t workspace(const BlockAttendParams& p) {
     if constexpr (D <= 128)
         if (fused<D>(p)) return layout_of<D, true>(p).bytes;
     return layout_of<D, false>(p).bytes;
+}
+template <int D, bool FUSED> int choice(const BlockAttendParams& a) {
+    const Layout l = layout_of<D, FUSED>(a);
+    Params p = params_of(a, l, nullptr);
+    divide<D, FUSED>(p, std::min(l.chunk, a.B * a.Hkv));
+    return (FUSED ? TQ_BLOCKS_FUSED : TQ_BLOCKS_EXPANDED) + (cuts(p) ? 1 : 0);
+}
+template <int D> int choice_any(const BlockAttendParams& p) {
+    if constexpr (D <= 128)
+        if (fused<D>(p)) return choice<D, true>(p);
+    return choice<D, false>(p);
 }
 template <int D> int launch_any(const BlockAttendParams& p, unsigned char* ws, cudaStream_t s) {
     if constexpr (D <= 128)
@@ -1065,6 +1089,9 @@ bool blocks_fa_takes(const BlockAttendParams& p) {
 }
 size_t blocks_fa_workspace(const BlockAttendParams& p) {
     return p.D == 64 ? bfa::workspace<64>(p) : p.D == 96 ? bfa::workspace<96>(p) : p.D == 128 ? bfa::workspace<128>(p) : bfa::workspace<256>(p);
+}
+int blocks_fa_choice(const BlockAttendParams& p) {
+    return p.D == 64 ? bfa::choice_any<64>(p) : p.D == 96 ? bfa::choice_any<96>(p) : p.D == 128 ? bfa::choice_any<128>(p) : bfa::choice_any<256>(p);
 }
 int launch_blocks_fa(const BlockAttendParams& p, cudaStream_t s) {
     unsigned char* ws = reinterpret_cast<unsigned char*>(p.part);

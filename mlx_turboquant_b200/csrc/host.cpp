@@ -455,9 +455,14 @@ PyObject* blocks_attend(PyObject*, PyObject* const* a, Py_ssize_t n) {
         if (!here(out, device) || out.sizes() != q.sizes() || out.scalar_type() != q.scalar_type() || !out.is_contiguous() || reinterpret_cast<uintptr_t>(out.data_ptr()) % 16) return none();
     }
     r.out = out.data_ptr();
+    // without room for the scratch that the call would like: Python takes it from here, with less
     r.workspace_bytes = tq_blocks_attend_workspace(&r);
     if (r.workspace_bytes) {
-        ws = empty({int64_t(r.workspace_bytes)}, at::kByte, device);
+        try {
+            ws = empty({int64_t(r.workspace_bytes)}, at::kByte, device);
+        } catch (const c10::OutOfMemoryError&) {
+            return none();
+        }
         r.workspace = ws.data_ptr();
     }
     int rc;

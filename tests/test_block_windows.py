@@ -125,3 +125,27 @@ def test_head_dims_without_kernels_leave_the_layers_as_they_were(head_dim):
         apply_turboquant(m, head_dim=head_dim, skip_layers=[0], block_cache="int8")
     assert [type(c).__name__ for c in m.make_cache()] == ["KVCache", "TurboQuantKVCache", "_RotatingKVCache", "TurboQuantKVCache"]
     assert "block_cache" not in m._turboquant_config
+
+
+def test_what_a_call_wants_and_what_it_makes_do_with():
+    """Host logic of the library: no GPU is asked."""
+    import ctypes as C
+    from mlx_turboquant_b200 import _lib
+    lib = _lib.lib()
+    for b, h, hq, d, total, t, dtype in ((1, 8, 32, 128, 16384, 2048, 1), (40, 8, 32, 64, 700, 64, 0), (3, 1, 4, 256, 5000, 300, 1), (1, 1, 1, 96, 9000, 1, 0), (2, 2, 4, 128, 300, 5, 2)):
+        a = _lib.BlocksAttendArgs()
+        a.store = _lib.BlockStore(b, h, d, 64, 0, dtype, *(4096,) * 6, -(-total // 64) * 64, total)
+        a.n_q_heads, a.t_q, a.q, a.out, a.scale = hq, t, _lib.NewRows(4096, 0, 128, 128), 4096, 1.0
+        most = lib.tq_blocks_attend_workspace(C.byref(a))
+        a.workspace_bytes = (1 << 64) - 1
+        way, room, last = lib.tq_blocks_attend_choice(C.byref(a)), most, None
+        assert way > 0 and lib.tq_blocks_attend_workspace_within(C.byref(a), most) == most
+        while room:
+            a.workspace_bytes = room
+            assert room != most or lib.tq_blocks_attend_choice(C.byref(a)) == way
+            last, room = room, lib.tq_blocks_attend_workspace_within(C.byref(a), room - 1)
+            assert room < last
+        a.workspace_bytes = 0
+        assert lib.tq_blocks_attend_choice(C.byref(a)) in (1, 2, 4)
+        a.workspace = 4100
+        assert lib.tq_blocks_attend_choice(C.byref(a)) == -1                          # 256-byte aligned
