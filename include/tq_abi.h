@@ -392,7 +392,8 @@ int tq_rotary(const tq_rotary_args* a, void* stream);
 
 /* Keys and values of a cache whose whole blocks of `block` tokens are held in 8 bits, a scale for each block and head.  Lane = b*n_kv_heads + h;
  * token t < length / block * block is row t of the lane's codes and stands for code * scale[t / block]; the tokens behind are rows t % block of
- * the lane's tail, as they came.  Contiguous arrays, 16-byte aligned. */
+ * the lane's tail, as they came.  Contiguous arrays, 16-byte aligned.  Codes are finite: tq_blocks_write marks a block that is not by its scale, and e4m3 storage that
+ * comes from elsewhere must not hold NaN codes (attention would let some of its exponentials pass over them). */
 enum { TQ_CODE_INT8 = 0, TQ_CODE_E4M3 = 1 };
 typedef struct {
     int batch, n_kv_heads, d, block;      /* d a multiple of 32 up to 256; block 16, 32, 64 or 128 */

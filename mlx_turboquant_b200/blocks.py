@@ -6,7 +6,7 @@ reference leaves on the model's uncompressed default cache (patch.py:238-340).
 Storage, six tensors: ``k_codes`` and ``v_codes`` (B, H, capacity, D), ``torch.int8`` or ``torch.float8_e4m3fn``; ``k_scales`` and ``v_scales``
 (B, H, capacity / block), float32; ``k_tail`` and ``v_tail`` (B, H, block, D), the tokens behind the last whole block as they came.  Blocks of
 16, 32, 64 or 128 tokens.  A block is quantised once, when its last token arrives: what the cache holds depends on the tokens, not on the calls
-they came in.
+they came in.  Codes are finite (the scale of a block that is not is NaN); storage from elsewhere must keep to that.
 
 * ``write_blocks`` appends tokens, ``read_blocks`` gives all of them dense, ``attend_blocks`` computes attention from the storage;
 * ``BlockKVCache`` keeps the storage of a layer behind the protocol of ``TurboQuantKVCache``.
