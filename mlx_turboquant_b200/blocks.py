@@ -235,9 +235,10 @@ class BlockKVCache:
     def _allocate(self, b: int, h: int, cap: int, dtype, device) -> tuple:
         codes = torch.int8 if self.codes == "int8" else torch.float8_e4m3fn
         out = []
-        for _ in range(2):
-            out += [torch.empty((b, h, cap, self.head_dim), dtype=codes, device=device), torch.empty((b, h, cap // self.block), dtype=torch.float32, device=device)]
-        return tuple(out + [torch.empty((b, h, self.block, self.head_dim), dtype=dtype, device=device) for _ in range(2)])
+        with torch.inference_mode(False):                      # (the storage outlives the mode that its first tokens came in, and is written to in any)
+            for _ in range(2):
+                out += [torch.empty((b, h, cap, self.head_dim), dtype=codes, device=device), torch.empty((b, h, cap // self.block), dtype=torch.float32, device=device)]
+            return tuple(out + [torch.empty((b, h, self.block, self.head_dim), dtype=dtype, device=device) for _ in range(2)])
 
     def _reserve(self, keys: torch.Tensor, t: int) -> None:
         """Room for the whole blocks that ``t`` more tokens fill: drops what no query can see any more, or grows."""
@@ -386,7 +387,8 @@ class BlockKVCache:
             self._store, self.offset, self._dropped = None, 0, 0
             return
         _lib.require_cuda(*v)
-        store = tuple(t.clone(memory_format=torch.contiguous_format) for t in v)       # (the cache that the state came from goes on writing to its own)
+        with torch.inference_mode(False):
+            store = tuple(t.clone(memory_format=torch.contiguous_format) for t in v)   # (the cache that the state came from goes on writing to its own)
         _store(*store, 0)
         if store[4].shape[2] != self.block or store[0].shape[3] != self.head_dim or store[0].dtype is not (torch.int8 if self.codes == "int8" else torch.float8_e4m3fn):
             raise ValueError("the state is of a cache with other blocks, codes or head_dim")

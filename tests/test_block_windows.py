@@ -149,3 +149,44 @@ def test_what_a_call_wants_and_what_it_makes_do_with():
         assert lib.tq_blocks_attend_choice(C.byref(a)) in (1, 2, 4)
         a.workspace = 4100
         assert lib.tq_blocks_attend_choice(C.byref(a)) == -1                          # 256-byte aligned
+
+
+def test_storage_from_inference_mode_is_written_to_outside_of_it():
+    """A prompt under torch.inference_mode(), steps under torch.no_grad(): what the window has passed is dropped in place.  (The storage's own bookkeeping; no kernel runs.)"""
+    c = BlockKVCache(32, 1, "int8", 16, window=20, sinks=3)
+    row = torch.zeros(1, 1, 1, 32)
+    with torch.inference_mode():
+        c._reserve(row.expand(1, 1, 600, 32), 600)
+    cap = c._store[0].shape[2]
+    for t in c._store:
+        assert not t.is_inference()
+        t.view(torch.uint8 if t.element_size() == 1 else t.dtype).zero_()
+    c.offset = cap + 15
+    c._store[0][0, 0, :, 0] = torch.arange(cap) // 16 % 100
+    c._store[1][0, 0] = torch.arange(cap // 16).float()
+    with torch.no_grad():
+        c._reserve(row, 1)
+    low = c.offset - 20 + 1
+    assert c._dropped == low // 16 * 16 - 16 and c._store[0].shape[2] == cap
+    kept = [0, *range(low // 16, cap // 16)]                # the sinks' block, and the window's
+    assert c._store[1][0, 0, :len(kept)].tolist() == kept and c._store[0][0, 0, :16 * len(kept):16, 0].tolist() == [k % 100 for k in kept]
+
+
+@pytest.mark.gpu
+def test_a_windowed_life_across_modes():
+    c, z = (BlockKVCache(64, 2, "int8", 32, 50, 4) for _ in range(2))
+    x = tokens(1, 2, 1400, 64, torch.float16, 1)
+    q = tokens(1, 4, 1, 64, torch.float16, 2)
+    with torch.inference_mode():
+        c.update(x[:, :, :1000], -x[:, :, :1000])
+    z.update(x[:, :, :1000], -x[:, :, :1000])
+    for i in range(1000, 1400):
+        k = x[:, :, i:i + 1]
+        assert torch.equal(c.decode_step(q, k, -k), z.decode_step(q, k, -k))
+    assert c._dropped > 0
+    with torch.inference_mode():
+        y = BlockKVCache(64, 2, "int8", 32, 50, 4)
+        y.state, y.meta_state = c.state, c.meta_state
+    for i in range(400):
+        k = x[:, :, i:i + 1]
+        assert torch.equal(y.decode_step(q, k, -k), c.decode_step(q, k, -k))
