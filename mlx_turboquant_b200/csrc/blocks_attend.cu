@@ -223,6 +223,7 @@ template <int N> __device__ __forceinline__ void digits_of(const float (&x)[4], 
     }
 }
 
+// (128 registers at two CTAs an SM: the bfloat16 instances spill some 50 to 190 bytes, d = 64 none; the fp16 ones, whose loop over the blocks is the same and whose tail needs no conversion, none.)
 template <int D, bool E4M3, bool BF> __global__ void __launch_bounds__(AW * 32, AttendPlan<D>::PER_SM) blocks_attend_kernel(const __grid_constant__ BlockAttendParams p, const __grid_constant__ AttendGrid z) {
     using P = AttendPlan<D>;
     constexpr int ST = P::ST, N = E4M3 ? 2 : 3;       // words of a query's four coordinates: fp16 pairs, or digits

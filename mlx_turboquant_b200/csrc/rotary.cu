@@ -10,6 +10,9 @@
 #include "decode_dev.cuh"
 
 namespace tq {
+
+int blocks_sm_count();                                 // blocks.cu
+
 namespace {
 
 constexpr int RT = 256;                                // threads per CTA
@@ -229,9 +232,9 @@ extern "C" int tq_rotary(const tq_rotary_args* a, void* stream) {
     // Tokens per CTA: some eight vectors a thread, so that the angles cost little, and whole waves of four CTAs per SM (8192 tokens x 40 heads, d = 128: 34 us with
     // 2.3 waves); heads shared between CTAs where there are fewer tokens than that.
     const int items = heads * std::max(1, (a->d - (a->interleaved ? 0 : a->dims / 2)) / vec);
-    const int64_t slots = 592, most = std::max<int64_t>(1, std::min<int64_t>(10 * RT / items, RT_ANGLES / p.half)), waves = (p.tokens + slots * most - 1) / (slots * most);
+    const int64_t sms = blocks_sm_count(), slots = 4 * sms, most = std::max<int64_t>(1, std::min<int64_t>(10 * RT / items, RT_ANGLES / p.half)), waves = (p.tokens + slots * most - 1) / (slots * most);
     p.per_cta = int((p.tokens + slots * waves - 1) / (slots * waves));
-    p.groups = p.per_cta > 1 ? 1 : int(std::max<int64_t>(1, std::min<int64_t>({(int64_t(items) + RT - 1) / RT, 296 / p.tokens, heads})));
+    p.groups = p.per_cta > 1 ? 1 : int(std::max<int64_t>(1, std::min<int64_t>({(int64_t(items) + RT - 1) / RT, 2 * sms / p.tokens, heads})));
     const int64_t blocks = (p.tokens + p.per_cta - 1) / p.per_cta * p.groups;
     if (blocks >= (int64_t(1) << 31)) return fail(TQ_ERR_UNSUPPORTED, "tq_rotary: too many tokens");
     cudaLaunchAttribute attr[1];
