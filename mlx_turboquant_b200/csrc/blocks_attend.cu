@@ -18,7 +18,7 @@
 //     without it in turn, at the card's power limit; a window of 4096 34.2 and 34.7).
 // Where few (lane, group)s have few tiles each, a cluster of CTAs shares one and joins its sums over distributed shared memory: one launch.
 // blocks_merge_kernel: joins the partials of a row that several CTAs worked on, in their order: results do not depend on which one came first.
-// Measured, 4 heads on 1 at d = 128: int8, 8 lanes x 700 tokens 8.4 us (launch, one tile's chain of latencies, the cluster's joining), 8 x 32,810 26.5 (2.5 TB/s: 18 us of
+// Measured, 4 heads on 1 at d = 128: int8, 8 lanes x 700 tokens 8.1 us (launch, one tile's chain of latencies, the cluster's joining), 8 x 32,810 27.4 (2.4 TB/s: 19 us of
 // loop, then the merge's launch), e4m3, 128 lanes x a window of 4096 32 to 35 (4 TB/s); int8, 512 lanes x 16,380 390 to 450 as the card is cooled (4.8 to 5.5 TB/s of the 6.55 that
 // a copy reaches; at its power limit, some 1.5 GHz).
 // blocks_plain_kernel: a warp per token on CUDA cores, float32 throughout: float32 tokens, head dims without a layout above.
