@@ -342,7 +342,7 @@ class BlockKVCache:
 
     def make_mask(self, N: int, offset: int = 0, return_array: bool = False, window_size: int | None = None) -> Any | None:
         """The mask of ``N`` new tokens over what ``update_and_fetch`` returns for them; asked before that call.  ``None`` for a single token, ``"causal"`` where
-        that is all, otherwise a boolean tensor (N, tokens returned), true where a query sees a token.  ``attend`` needs none: the window is part of it.
+        that is all, otherwise a boolean tensor (N, tokens returned), true where a query sees a token (before the first tokens on the current device).  ``attend`` needs none: the window is part of it.
         ``window_size`` may be the window, or what the model's own cache calls its size: window and sinks together."""
         if window_size is not None and (self.window is None or window_size not in (self.window, self.window + self.sinks)):
             raise NotImplementedError(f"this cache has a window of {self.window} and {self.sinks} sinks, not {window_size}")

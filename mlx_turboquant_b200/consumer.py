@@ -130,7 +130,8 @@ class Attention(torch.nn.Module):
             mask = None
             if cache is not None:
                 if getattr(cache, "window", None) is not None:                          # (its own mask: it returns what the window leaves)
-                    mask = cache.make_mask(L)
+                    mask = cache.make_mask(L)                                           # (before the first tokens on the current device, wherever they will be)
+                    mask = mask.to(x.device) if isinstance(mask, torch.Tensor) else mask
                 keys, values = cache.update_and_fetch(keys.contiguous(), values.contiguous())
             q = queries.float() if keys.dtype == torch.float32 else queries
             T = keys.shape[2]

@@ -190,3 +190,34 @@ def test_a_windowed_life_across_modes():
     for i in range(400):
         k = x[:, :, i:i + 1]
         assert torch.equal(y.decode_step(q, k, -k), c.decode_step(q, k, -k))
+
+
+def test_the_callers_dense_route_asks_a_windowed_cache_for_its_mask():
+    """On the CPU, with a cache that keeps everything and returns what a windowed one would: the same logits whatever pieces the tokens come in."""
+    from mlx_turboquant_b200.consumer import LlamaShaped, ModelArgs
+
+    class Windowed:
+        window, sinks = 6, 2
+
+        def __init__(self):
+            self.offset, self.kv = 0, None
+
+        def make_mask(self, n):
+            return None if n == 1 else "causal" if self.offset + n - self.window <= self.sinks else window_mask(self.offset, n, self.window, self.sinks, "cpu")
+
+        def update_and_fetch(self, k, v):
+            low = max(0, self.offset - self.window + 1)
+            self.kv = (k, v) if self.kv is None else tuple(torch.cat(x, 2) for x in zip(self.kv, (k, v)))
+            self.offset += k.shape[2]
+            return tuple(torch.cat([x[:, :, :min(self.sinks, low)], x[:, :, low:]], 2) for x in self.kv)
+
+    m = LlamaShaped(ModelArgs(hidden_size=64, num_hidden_layers=2, num_attention_heads=4, num_key_value_heads=2, head_dim=32, intermediate_size=64, vocab_size=64), dtype=torch.float32, device="cpu", std=0.2)
+    tok = torch.randint(0, 64, (2, 25), generator=torch.Generator().manual_seed(3))
+    whole = m(tok, cache=[Windowed() for _ in range(2)], packed=False)
+    assert float((whole - m(tok)).abs().max()) > 1e-2                       # (the window does hide something)
+    for pieces in ((1,) * 25, (7, 1, 12, 5), (3, 22), (20, 1, 1, 3)):
+        cache, at, got = [Windowed() for _ in range(2)], 0, []
+        for n in pieces:
+            got.append(m(tok[:, at:at + n], cache=cache, packed=False))
+            at += n
+        assert torch.allclose(torch.cat(got, 1), whole, atol=2e-4)
